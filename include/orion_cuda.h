@@ -488,6 +488,40 @@ int orion_cuda_attn_bench_device_views(OrionAttnBench *bench, const void **q, co
                                        const uint32_t **block_table_offsets, uint32_t *max_position);
 void orion_cuda_attn_bench_destroy(OrionAttnBench *bench);
 
+/* ---- 4-bit weights (no reference counterpart) ----
+ * W[n][k] = (code - zero) * scale, codes and zeros 0..15, with one scale and one zero point for every `group` (32, 64 or
+ * 128) consecutive k of a row. All pointers are DEVICE pointers; the calls check what can be checked on the host, allocate
+ * nothing, only enqueue work on `stream` (a cudaStream_t, NULL = the default stream) of `device`, which is current during the
+ * call and put back, and can be captured into a graph. They hold no state: calls on different streams and from different
+ * threads do not touch one another. Results do not vary from run to run.
+ *   packed  u32 [out_features][in_features / 8], 16-byte aligned. Of eight consecutive k, number 2i is in bits 4i .. 4i + 3
+ *           of their word, number 2i + 1 in bits 16 + 4i .. 19 + 4i.
+ *   scales  bf16 [in_features / group][out_features]
+ *   zeros   u8, laid out like scales; NULL: 8 everywhere (the symmetric form). Values above 15 are not allowed.
+ * in_features is a multiple of `group`. Rows of values have unit stride and start on 16-byte boundaries. */
+typedef struct OrionW4Weight {
+  const void *packed, *scales, *zeros;
+  uint64_t out_features, in_features;
+  uint32_t group;
+} OrionW4Weight;
+enum { ORION_GATE_SILU = 0, ORION_GATE_GELU_TANH = 1 };
+/* Codes, scales and zero points of a matrix of f32 or bf16 values (`dtype`; row_stride in values). Symmetric (zeros NULL):
+ * scale = max|w| / 7, code = 8 + round(w / scale). With zero points: lo = min(w, 0), hi = max(w, 0), scale = (hi - lo) / 15,
+ * zero = round(-lo / scale), code = round(w / scale) + zero, held within 0..15. Scales are rounded to bf16 before anything is
+ * divided by them, one below 2^-126 is 0 (with every code the zero point); quotients go to the nearest whole number, ties to
+ * the even one. A group with an infinity or a NaN gets a scale of NaN. */
+int orion_cuda_w4_quantize(int device, int dtype, const void *weight, uint64_t out_features, uint64_t in_features,
+                           uint64_t row_stride, uint32_t group, void *packed, void *scales, void *zeros, void *stream);
+/* y = x W^T + bias: tensor::linear (tensor.rs:96-130) with such weights. x and out hold values of `dtype` (f32 or bf16), rows
+ * x_stride and out_stride values apart; bias is f32 [out_features] or NULL. Sums are held in f32 and rounded once. `out`
+ * overlaps no input. */
+int orion_cuda_w4_linear(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *weight,
+                         const float *bias, void *out, uint64_t out_stride, void *stream);
+/* y = f(x Wgate^T) * (x Wup^T), f = silu or the tanh form of GELU: both projections, the activation and the product (tensor.rs:
+ * 96-130, 175-189) in one kernel; the two matrices have the same sizes and groups. */
+int orion_cuda_w4_gated(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *gate,
+                        const OrionW4Weight *up, int activation, void *out, uint64_t out_stride, void *stream);
+
 /* ---- decode attention for callers that cannot allocate ----
  * This entry point has no counterpart in the reference. It is the paged GQA
  * decode attention above (bf16, head_dim 128, 16-token blocks, one query row

@@ -22,6 +22,7 @@ from .distributed import (Collective, CommunicationEstimate, NcclCollective, Ncc
 from . import engine, errors, ops
 from .engine import Engine, KvCacheManager, SamplingParams, Scheduler, SchedulerConfig, hash_block
 from .attn_bench import PagedAttentionBench
+from .w4 import W4Weight, gated_w4, linear_w4, quantize_w4
 
 __all__ = [
     "BackendError", "CudaUnavailable", "EngineError", "InternalError", "InvalidRequest", "ModelError",
@@ -32,5 +33,5 @@ __all__ = [
     "CommunicationEstimate", "NcclCollective", "NcclCollectiveId", "ParallelLayout", "Rank", "Shard", "ShardStrategy",
     "SingleRank", "shard_dimension", "ops", "PagedAttentionBench", "CacheExhausted", "ContextLengthExceeded",
     "QueueFull", "engine", "errors", "Engine", "KvCacheManager", "SamplingParams", "Scheduler", "SchedulerConfig",
-    "hash_block", "Bigram", "Loop", "QueryTemperature", "Yarn",
+    "hash_block", "Bigram", "Loop", "QueryTemperature", "Yarn", "W4Weight", "quantize_w4", "linear_w4", "gated_w4",
 ]

@@ -62,6 +62,12 @@ class OrionLayeredDesc(C.Structure):
                 ("bigram_mul_prev", C.c_uint64), ("bigram_mul_cur", C.c_uint64)]
 
 
+class OrionW4Weight(C.Structure):
+    _fields_ = [("packed", C.c_void_p), ("scales", C.c_void_p), ("zeros", C.c_void_p), ("out_features", C.c_uint64),
+                ("in_features", C.c_uint64), ("group", C.c_uint32)]
+
+
+GATE_SILU, GATE_GELU_TANH = 0, 1
 MIXER_MIN_GRU, MIXER_LATENT_ATTENTION, MIXER_ATTENTION, MIXER_GLA = 0, 1, 2, 3
 BLOCK_PARALLEL, BLOCK_SANDWICH, BLOCK_PRENORM, BLOCK_GATED_POSTNORM = 0, 1, 2, 3
 ACT_GELU_TANH, ACT_RELU2, ACT_GEGLU_TANH = 0, 1, 2
@@ -146,6 +152,9 @@ SIGNATURES = {
     "orion_cuda_attn_bench_destroy": (None, [_vp]),
     "orion_cuda_paged_decode_attention_noalloc": (_int, [_int, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp,
                                                          _vp, _u32, _u32, _u32, _vp, _vp]),
+    "orion_cuda_w4_quantize": (_int, [_int, _int, _vp, _u64, _u64, _u64, _u32, _vp, _vp, _vp, _vp]),
+    "orion_cuda_w4_linear": (_int, [_int, _int, _vp, _u64, _u64, _vp, _vp, _vp, _u64, _vp]),
+    "orion_cuda_w4_gated": (_int, [_int, _int, _vp, _u64, _u64, _vp, _vp, _int, _vp, _u64, _vp]),
 }
 
 

@@ -23,6 +23,7 @@ class CudaBackend:
         """``CudaBackend::new(ordinal)``; raises ``CudaUnavailable`` when no usable device exists."""
         self._h = C.c_void_p()
         check(_ffi.lib().orion_cuda_backend_create(int(ordinal), C.byref(self._h)))
+        self._ordinal = int(ordinal)
 
     def __del__(self):
         if getattr(self, "_h", None):

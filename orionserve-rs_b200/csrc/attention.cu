@@ -864,20 +864,6 @@ constexpr int kMaxDevices = kMaxDeviceOrdinals;
 // cudaGetSymbolAddress while that device is current.
 std::atomic<float *> g_noalloc_ptr[kMaxDevices] = {};
 std::mutex g_noalloc_mu;
-
-// Makes `device` current for the scope and puts the caller's device back afterwards.
-struct ScopedDevice {
-  int prev = -1;
-  cudaError_t status;
-  explicit ScopedDevice(int device) {
-    status = cudaGetDevice(&prev);
-    if (status == cudaSuccess && prev != device) status = cudaSetDevice(device);
-  }
-  ~ScopedDevice() {
-    int now = -1;
-    if (prev >= 0 && cudaGetDevice(&now) == cudaSuccess && now != prev) cudaSetDevice(prev);
-  }
-};
 }  // namespace
 
 int noalloc_decode_attention(int device, const bf16 *q, const bf16 *arena, uint32_t num_blocks,

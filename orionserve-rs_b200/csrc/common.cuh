@@ -43,6 +43,20 @@ inline const void *device_symbol(const S &symbol) {
   return cudaGetSymbolAddress(&p, symbol) == cudaSuccess ? p : nullptr;
 }
 
+// Makes `device` current for the scope and puts the caller's device back afterwards.
+struct ScopedDevice {
+  int prev = -1;
+  cudaError_t status;
+  explicit ScopedDevice(int device) {
+    status = cudaGetDevice(&prev);
+    if (status == cudaSuccess && prev != device) status = cudaSetDevice(device);
+  }
+  ~ScopedDevice() {
+    int now = -1;
+    if (prev >= 0 && cudaGetDevice(&now) == cudaSuccess && now != prev) cudaSetDevice(prev);
+  }
+};
+
 // Number of kernels launched through launch accounting since the last reset.
 extern thread_local uint64_t g_launch_count;
 inline void count_launch() { ++g_launch_count; }

@@ -1,0 +1,181 @@
+"""4-bit weights: a quantiser, projections and gated feed-forwards over torch tensors on the GPU.
+
+``W[n][k] = (code - zero) * scale`` with a bf16 scale, and in the asymmetric form a zero point, per group of 32, 64 or 128 consecutive ``k`` of a row.
+Codes are packed eight to an int32: of eight consecutive ``k``, number ``2i`` is in bits ``4i .. 4i + 3``, number ``2i + 1`` in bits ``16 + 4i ..
+19 + 4i``. The functions stand beside ``ops.linear`` and ``ops.swiglu`` for tensors that are on the device already: they run on torch's current
+stream of the tensors' device, allocate only what they return, and can be captured into a CUDA graph. Activations are f32 or bf16. Nothing here
+has a gradient; tensors that require one are refused.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+from . import _ffi
+from .backend import CudaBackend
+from .errors import InvalidRequest, check
+
+GROUPS = (32, 64, 128)
+_ACTIVATIONS = {"silu": _ffi.GATE_SILU, "gelu_tanh": _ffi.GATE_GELU_TANH}
+_torch = None
+_dtypes = {}  # torch dtype -> OrionDType
+_linear = _gated = None  # entry points of the library
+
+
+def _load():
+    """torch and the library, at the first call: the rest of the package does without torch."""
+    global _torch, _linear, _gated
+    import torch
+
+    lib = _ffi.lib()
+    _linear, _gated = lib.orion_cuda_w4_linear, lib.orion_cuda_w4_gated
+    _dtypes.update({torch.float32: 0, torch.bfloat16: 2})
+    _torch = torch
+
+
+def _on_device(name, t, dtype, shape=None):
+    if not isinstance(t, _torch.Tensor) or not t.is_cuda:
+        raise InvalidRequest(f"{name}: a CUDA tensor is needed")
+    if t.dtype != dtype:
+        raise InvalidRequest(f"{name}: {dtype} is needed, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != shape:
+        raise InvalidRequest(f"{name}: shape {shape} is needed, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise InvalidRequest(f"{name}: not contiguous")
+
+
+class W4Weight:
+    """A matrix of 4-bit codes ``[out_features, in_features]``, kept by a program for as long as it uses the matrix.
+
+    ``packed`` is int32 ``[out, in / 8]``, ``scales`` bf16 ``[in / group, out]``, ``zeros`` uint8 like ``scales`` with values of at most 15, or None:
+    8 everywhere. The tensors are kept and must not be resized; their values may be written."""
+
+    __slots__ = ("packed", "scales", "zeros", "group", "out_features", "in_features", "device_index", "_desc", "_address")
+
+    def __init__(self, packed, scales, zeros=None, group: int = 128):
+        if _torch is None:
+            _load()
+        if group not in GROUPS:
+            raise InvalidRequest(f"groups of 4-bit weights hold 32, 64 or 128 values, got {group}")
+        if not isinstance(packed, _torch.Tensor) or packed.dim() != 2:
+            raise InvalidRequest("packed: a matrix is needed")
+        n, k = packed.shape[0], packed.shape[1] * 8
+        if n == 0 or k == 0 or k % group != 0:
+            raise InvalidRequest(f"a matrix of {n} x {k} has no whole groups of {group}")
+        _on_device("packed", packed, _torch.int32)
+        _on_device("scales", scales, _torch.bfloat16, (k // group, n))
+        if zeros is not None:
+            _on_device("zeros", zeros, _torch.uint8, (k // group, n))
+        if scales.device != packed.device or (zeros is not None and zeros.device != packed.device):
+            raise InvalidRequest("packed, scales and zeros are on different devices")
+        if packed.data_ptr() % 16:
+            raise InvalidRequest("packed: must start on a 16-byte boundary")
+        self.packed, self.scales, self.zeros, self.group = packed, scales, zeros, group
+        self.out_features, self.in_features, self.device_index = n, k, packed.device.index
+        self._desc = _ffi.OrionW4Weight(packed.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), n, k, group)
+        self._address = C.addressof(self._desc)
+
+    @classmethod
+    def from_codes(cls, codes, scales, zeros=None, group: int = 128) -> "W4Weight":
+        """Packs codes ``[out, in]`` of 0..15, as other formats hold them, on their device; ``scales`` and ``zeros`` as in the constructor."""
+        if _torch is None:
+            _load()
+        if not isinstance(codes, _torch.Tensor) or codes.dim() != 2 or codes.shape[1] % 8 or codes.dtype.is_floating_point:
+            raise InvalidRequest("codes: a matrix of whole numbers is needed, with a multiple of 8 columns")
+        if codes.numel() and (int(codes.min()) < 0 or int(codes.max()) > 15):
+            raise InvalidRequest("codes: values of 0 to 15 are needed")
+        at = _torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=_torch.int32, device=codes.device)
+        words = (codes.to(_torch.int32).view(codes.shape[0], -1, 8) << at).sum(-1, dtype=_torch.int32)
+        return cls(words, scales, zeros, group)
+
+
+def _rows(backend: CudaBackend, x, weight: W4Weight):
+    """Checks a call's activations; returns (dtype, rows, row stride)."""
+    if x.__class__ is not _torch.Tensor and not isinstance(x, _torch.Tensor):
+        raise InvalidRequest("x: a CUDA tensor is needed")
+    dtype = _dtypes.get(x.dtype)
+    if dtype is None:
+        raise InvalidRequest(f"x: float32 or bfloat16 is needed, got {x.dtype}")
+    if x.dim() != 2 or x.shape[1] != weight.in_features:
+        raise InvalidRequest(f"x: shape [rows, {weight.in_features}] is needed, got {tuple(x.shape)}")
+    if x.get_device() != backend._ordinal or weight.device_index != backend._ordinal:
+        raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
+    if x.requires_grad and _torch.is_grad_enabled():
+        raise InvalidRequest("x: 4-bit operators have no gradient")
+    stride, unit = x.stride()
+    if unit != 1:
+        raise InvalidRequest("x: the values of a row must be neighbours")
+    return dtype, x.shape[0], stride
+
+
+def _output(x, out, rows, n):
+    if out is None:
+        return x.new_empty((rows, n)), n
+    if not isinstance(out, _torch.Tensor) or out.dtype != x.dtype or out.device != x.device or tuple(out.shape) != (rows, n) or (n > 1 and out.stride(1) != 1):
+        raise InvalidRequest(f"out: a {x.dtype} tensor of shape [{rows}, {n}] on {x.device} is needed, its rows' values neighbours")
+    if out.requires_grad and _torch.is_grad_enabled():
+        raise InvalidRequest("out: 4-bit operators have no gradient")
+    return out, out.stride(0)
+
+
+def _stream(device: int) -> int:
+    return _torch.cuda.current_stream(device).cuda_stream
+
+
+def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
+    """``x W^T + bias`` (tensor.rs:96-130) over ``x`` ``[rows, in]``, f32 or bf16; ``bias`` f32 ``[out]``. Sums are f32, rounded once to the type of
+    ``x``. Rows may be apart (any stride that keeps them on 16-byte boundaries); ``out``, if given, is written and returned."""
+    if _torch is None:
+        _load()
+    dtype, rows, stride = _rows(backend, x, weight)
+    n = weight.out_features
+    if bias is not None:
+        _on_device("bias", bias, _torch.float32, (n,))
+        if bias.get_device() != backend._ordinal:
+            raise InvalidRequest(f"bias must be on the backend's device {backend._ordinal}")
+    out, out_stride = _output(x, out, rows, n)
+    check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, weight._address, None if bias is None else bias.data_ptr(), out.data_ptr(),
+                  out_stride, _stream(backend._ordinal)))
+    return out
+
+
+def gated_w4(backend: CudaBackend, x, gate: W4Weight, up: W4Weight, activation: str = "silu", out=None):
+    """``f(x Wgate^T) * (x Wup^T)`` in one kernel, ``f`` = "silu" or "gelu_tanh" (tensor.rs:96-130, 175-189); the matrices have the same sizes and
+    groups. Otherwise as ``linear_w4``."""
+    if _torch is None:
+        _load()
+    kind = _ACTIVATIONS.get(activation)
+    if kind is None:
+        raise InvalidRequest(f"unknown activation {activation!r}")
+    dtype, rows, stride = _rows(backend, x, gate)
+    if up.device_index != backend._ordinal:
+        raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
+    out, out_stride = _output(x, out, rows, gate.out_features)
+    check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride,
+                 _stream(backend._ordinal)))
+    return out
+
+
+def quantize_w4(backend: CudaBackend, weight, group: int = 128, zeros: bool = False) -> W4Weight:
+    """Codes, scales and (``zeros``) zero points of ``weight`` ``[out, in]``, f32 or bf16.
+
+    Symmetric: scale = max|w| / 7, code = 8 + round(w / scale). With zero points: lo = min(w, 0), hi = max(w, 0), scale = (hi - lo) / 15, zero =
+    round(-lo / scale), code = round(w / scale) + zero within 0..15. Scales are rounded to bf16 first, one below 2^-126 is 0; ties go to the even
+    number. A group with an infinity or a NaN gets a scale of NaN."""
+    if _torch is None:
+        _load()
+    if not isinstance(weight, _torch.Tensor) or weight.dim() != 2 or weight.dtype not in _dtypes:
+        raise InvalidRequest("weight: a float32 or bfloat16 matrix is needed")
+    if weight.get_device() != backend._ordinal:
+        raise InvalidRequest(f"weight must be on the backend's device {backend._ordinal}")
+    n, k = weight.shape
+    if group not in GROUPS or n == 0 or k == 0 or k % group != 0:
+        raise InvalidRequest(f"a matrix of {n} x {k} has no whole groups of {group} (32, 64 or 128)")
+    if weight.stride(1) != 1:
+        raise InvalidRequest("weight: the values of a row must be neighbours")
+    packed = weight.new_empty((n, k // 8), dtype=_torch.int32)
+    scales = weight.new_empty((k // group, n), dtype=_torch.bfloat16)
+    zero = weight.new_empty((k // group, n), dtype=_torch.uint8) if zeros else None
+    check(_ffi.lib().orion_cuda_w4_quantize(backend._ordinal, _dtypes[weight.dtype], weight.data_ptr(), n, k, weight.stride(0), group, packed.data_ptr(),
+                                            scales.data_ptr(), None if zero is None else zero.data_ptr(), _stream(backend._ordinal)))
+    return W4Weight(packed, scales, zero, group)
