@@ -496,8 +496,8 @@ void orion_cuda_attn_bench_destroy(OrionAttnBench *bench);
  * threads do not touch one another. Results do not vary from run to run.
  *   packed  u32 [out_features][in_features / 8], 16-byte aligned. Of eight consecutive k, number 2i is in bits 4i .. 4i + 3
  *           of their word, number 2i + 1 in bits 16 + 4i .. 19 + 4i.
- *   scales  bf16 [in_features / group][out_features]
- *   zeros   u8, laid out like scales; NULL: 8 everywhere (the symmetric form). Values above 15 are not allowed.
+ *   scales  bf16 [in_features / group][out_features], 4-byte aligned
+ *   zeros   u8, laid out like scales, 4-byte aligned; NULL: 8 everywhere (the symmetric form). Values above 15 are not allowed.
  * in_features is a multiple of `group`. Rows of values have unit stride and start on 16-byte boundaries. */
 typedef struct OrionW4Weight {
   const void *packed, *scales, *zeros;

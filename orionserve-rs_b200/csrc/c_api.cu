@@ -1,6 +1,7 @@
 // extern "C" entry points declared in include/orion_cuda.h.
 #include <cstring>
 #include <memory>
+#include <mutex>
 #include <new>
 #include <vector>
 
@@ -331,8 +332,23 @@ int orion_cuda_backend_create(int ordinal, OrionBackend **out) {
   if (n == 0) return set_error(ORION_ERR_UNAVAILABLE, "CUDA driver found but no devices available");
   if (ordinal < 0 || ordinal >= n)  // CudaUnavailable::NoSuchDevice
     return set_error(ORION_ERR_UNAVAILABLE, "CUDA device %d requested but only %d device(s) present", ordinal, n);
+  // The properties of a device stay, and asking for them takes 3 to 30 ms.
+  struct Known {
+    bool known = false;
+    cudaDeviceProp prop;
+  };
+  static Known known[kMaxDeviceOrdinals];
+  static std::mutex known_mu;
   cudaDeviceProp prop;
-  ORION_CUDA_CHECK("device properties", cudaGetDeviceProperties(&prop, ordinal));
+  {
+    std::lock_guard<std::mutex> lock(known_mu);
+    if (ordinal < kMaxDeviceOrdinals && known[ordinal].known) {
+      prop = known[ordinal].prop;
+    } else {
+      ORION_CUDA_CHECK("device properties", cudaGetDeviceProperties(&prop, ordinal));
+      if (ordinal < kMaxDeviceOrdinals) known[ordinal].prop = prop, known[ordinal].known = true;
+    }
+  }
   if (prop.major != 10)
     return set_error(ORION_ERR_UNAVAILABLE, "CUDA device %d is sm_%d%d; this library is built for sm_100a only",
                      ordinal, prop.major, prop.minor);

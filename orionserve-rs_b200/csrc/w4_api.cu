@@ -40,8 +40,8 @@ int check_matrix(const char *what, const void *p, uint64_t rows, uint64_t cols, 
 int check_weight(const char *what, const OrionW4Weight *w) {
   if (!w || !w->packed || !w->scales) return set_error(ORION_ERR_INVALID_REQUEST, "%s: null pointer argument", what);
   ORION_TRY(check_sizes(w->out_features, w->in_features, w->group));
-  if (!aligned(w->packed, 16) || !aligned(w->scales, 2))
-    return set_error(ORION_ERR_INVALID_REQUEST, "%s: packed weights must start on a 16-byte boundary, scales on a 2-byte one", what);
+  if (!aligned(w->packed, 16) || !aligned(w->scales, 4) || !aligned(w->zeros, 4))
+    return set_error(ORION_ERR_INVALID_REQUEST, "%s: packed weights must start on a 16-byte boundary, scales and zeros on a 4-byte one", what);
   return ORION_OK;
 }
 W4View view(const OrionW4Weight *w) {
@@ -84,8 +84,8 @@ int orion_cuda_w4_quantize(int device, int dtype, const void *weight, uint64_t o
   ORION_TRY(check_sizes(out_features, in_features, group));
   ORION_TRY(check_matrix("weight", weight, out_features, in_features, row_stride, dtype));
   if (!packed || !scales) return set_error(ORION_ERR_INVALID_REQUEST, "null pointer argument");
-  if (!aligned(packed, 16) || !aligned(scales, 2))
-    return set_error(ORION_ERR_INVALID_REQUEST, "packed weights must start on a 16-byte boundary, scales on a 2-byte one");
+  if (!aligned(packed, 16) || !aligned(scales, 4) || !aligned(zeros, 4))
+    return set_error(ORION_ERR_INVALID_REQUEST, "packed weights must start on a 16-byte boundary, scales and zeros on a 4-byte one");
   if ((out_features + 31) / 32 * ((in_features + 255) / 256) > 0x7fffffffull)
     return set_error(ORION_ERR_INVALID_REQUEST, "a matrix of %llu x %llu is too large for one call", (unsigned long long)out_features, (unsigned long long)in_features);
   ScopedDevice current(device);

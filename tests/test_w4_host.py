@@ -29,7 +29,7 @@ def quantize(pkg, dtype=2, w=P, n=64, k=128, stride=128, group=32, packed=P, sca
     return pkg._ffi.lib().orion_cuda_w4_quantize(0, dtype, w, n, k, stride, group, packed, scales, zeros, None)
 
 
-BAD_WEIGHTS = [dict(packed=0), dict(scales=0), dict(packed=P + 8), dict(scales=P + 1), dict(group=0), dict(group=16), dict(group=48), dict(group=256),
+BAD_WEIGHTS = [dict(packed=0), dict(scales=0), dict(packed=P + 8), dict(scales=P + 1), dict(scales=P + 2), dict(zeros=P + 2), dict(group=0), dict(group=16), dict(group=48), dict(group=256),
                dict(in_features=0), dict(in_features=130), dict(in_features=1 << 31), dict(out_features=0), dict(out_features=1 << 31)]
 BAD_ROWS = [dict(dtype=1), dict(dtype=4), dict(dtype=-1), dict(x=0), dict(x=P + 2), dict(x=P + 8), dict(stride=127), dict(stride=0), dict(stride=132),
             dict(stride=1 << 50), dict(rows=1 << 31), dict(out=0), dict(out=P + 1), dict(out_stride=63), dict(out_stride=1 << 50)]
@@ -58,7 +58,7 @@ def test_other_refusals(pkg):
     for over in (dict(out_features=65), dict(in_features=160), dict(group=64)):
         assert gated(pkg, None, weight(pkg, **over)) == bad
     for over in (dict(dtype=1), dict(w=0), dict(w=P + 4), dict(n=0), dict(n=1 << 31), dict(k=0), dict(k=100), dict(stride=96), dict(stride=129), dict(group=8),
-                 dict(packed=0), dict(packed=P + 4), dict(scales=0), dict(scales=P + 1), dict(n=1 << 30, k=1 << 20, stride=1 << 20)):
+                 dict(packed=0), dict(packed=P + 4), dict(scales=0), dict(scales=P + 2), dict(zeros=P + 1), dict(n=1 << 30, k=1 << 20, stride=1 << 20)):
         assert quantize(pkg, **over) == bad, over
 
 
