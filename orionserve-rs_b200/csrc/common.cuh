@@ -46,14 +46,15 @@ inline const void *device_symbol(const S &symbol) {
 // Makes `device` current for the scope and puts the caller's device back afterwards.
 struct ScopedDevice {
   int prev = -1;
+  bool changed = false;
   cudaError_t status;
   explicit ScopedDevice(int device) {
     status = cudaGetDevice(&prev);
-    if (status == cudaSuccess && prev != device) status = cudaSetDevice(device);
+    changed = status == cudaSuccess && prev != device;
+    if (changed) status = cudaSetDevice(device);
   }
   ~ScopedDevice() {
-    int now = -1;
-    if (prev >= 0 && cudaGetDevice(&now) == cudaSuccess && now != prev) cudaSetDevice(prev);
+    if (changed) cudaSetDevice(prev);
   }
 };
 

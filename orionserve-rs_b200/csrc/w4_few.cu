@@ -81,6 +81,13 @@ __device__ __forceinline__ void dequant(uint32_t word, uint32_t minus_zero, uint
   pair[2] = fma_bf16x2(rest & 0x000f000fu, kLow, minus_zero);
   pair[3] = fma_bf16x2(rest & 0x00f000f0u, kHigh, minus_zero);
 }
+// d = a b (+ c)
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 // What is left of x beyond its first eight bits; nothing of an infinity.
 __device__ __forceinline__ float beyond(float x, float first) { return x == first ? 0.f : x - first; }
 __device__ __forceinline__ float first_bits(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
@@ -101,7 +108,7 @@ struct FewConfig {
   static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + kZeroRow);
   static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows;         // floats of the sums that meet in shared memory
   // Slabs in the ring, and sets of sums: with few tokens two CTAs share an SM, with many one takes what there is.
-  static constexpr uint32_t kStages = NT == 1 || (sizeof(T) == 4) ? 3 : 4, kSets = NT <= 2 ? 2 : 1;
+  static constexpr uint32_t kStages = sizeof(T) == 4 ? 3 : 4, kSets = NT <= 2 ? 2 : 1;
   static uint32_t stage(uint32_t tokens) { return (kWStage + tokens * kXRow + kSStage + 15) / 16 * 16; }
   static uint32_t smem(uint32_t tokens) { return kKGroups * kStages * stage(tokens) + kSets * kSums * 4; }
 };
@@ -130,50 +137,92 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   auto matrix_of = [&](uint32_t rt) { return rt / kTilesPerMatrix; };
   pdl_wait();
 
+  const bool words = (c.n & 3) == 0, any_zeros = c.w.zeros || c.up.zeros;
+  // Scales and zero points of a slab, in words. An odd number of outputs leaves them at any place within theirs; the first word then holds something before
+  // them. Pieces beyond the arrays are filled with zeros.
+  constexpr uint32_t kScaleWords = Cfg::kOutputs / 2, kZeroWords = Cfg::kOutputs / 4, kRowsOfParams = Cfg::kMatrices * kPerSlab;
+  auto load_params = [&](uint32_t s_at, uint32_t slab, uint32_t n0) {
+    const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
+    if (words) {
+#pragma unroll
+      for (uint32_t j = 0; j < (kRowsOfParams * kScaleWords + WR * 32 - 1) / (WR * 32); ++j) {
+        const uint32_t i = in_kg + j * WR * 32, row = i / kScaleWords, col = i % kScaleWords * 2, group = slab * kPerSlab + row % kPerSlab;
+        if (row < kRowsOfParams) {
+          const bf16 *p = row >= kPerSlab ? c.up.scales : c.w.scales;
+          const bool some = group < groups && n0 + col < c.n;
+          cp_async4(s_at + row * Cfg::kScaleRow + col * 2, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
+        }
+      }
+      if (!any_zeros) return;
+#pragma unroll
+      for (uint32_t j = 0; j < (kRowsOfParams * kZeroWords + WR * 32 - 1) / (WR * 32); ++j) {
+        const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords, col = i % kZeroWords * 4, group = slab * kPerSlab + row % kPerSlab;
+        const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
+        if (row < kRowsOfParams && p) {
+          const bool some = group < groups && n0 + col < c.n;
+          cp_async4(z_at + row * Cfg::kZeroRow + col, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
+        }
+      }
+    } else {
+      const uint64_t all = (uint64_t)groups * c.n;
+#pragma unroll 1
+      for (uint32_t row = 0; row < kRowsOfParams; ++row) {
+        const W4View &w = row >= kPerSlab ? c.up : c.w;
+        const uint32_t group = slab * kPerSlab + row % kPerSlab;
+        const uint64_t first = (uint64_t)group * c.n + n0;
+        for (uint32_t i = in_kg; i < kScaleWords + 1; i += WR * 32) {
+          const uint64_t at = (first & ~1ull) + 2 * i;
+          const uint32_t left = group < groups && at < all ? (uint32_t)min(all - at, (uint64_t)2) * 2 : 0;
+          cp_async4(s_at + row * Cfg::kScaleRow + i * 4, left ? w.scales + at : w.scales, left);
+        }
+        for (uint32_t i = in_kg; w.zeros && i < kZeroWords + 1; i += WR * 32) {
+          const uint64_t at = (first & ~3ull) + 4 * i;
+          const uint32_t left = group < groups && at < all ? (uint32_t)min(all - at, (uint64_t)4) : 0;
+          cp_async4(z_at + row * Cfg::kZeroRow + i * 4, left ? w.zeros + at : w.zeros, left);
+        }
+      }
+    }
+  };
   // What is loaded next: a slab of a tile. The loads run ahead of the products across tiles, so that the ring never drains.
-  uint32_t load_tile = blockIdx.x, load_index = 0, load_slot = 0;
+  //
+  // Weight rows of 64 bytes, 16-byte pieces permuted by (row / 2) & 3 so that the eight rows of a fragment lie in different banks; a lane copies piece t of
+  // the rows g, g + 8, .. of its warp's tiles. Token rows: every other one with its halves of 64 bytes exchanged.
+  constexpr uint32_t kPieces = Cfg::kXRow / 16, kPer = 16 / sizeof(T), kXTurns = (Cfg::kTokens * kPieces + WR * 32 - 1) / (WR * 32);
+  const uint32_t w_to = wr * RT * 16 * kWRow + g * kWRow + (t ^ ((g >> 1) & 3)) * 16;
+  const uint64_t eight_rows = (uint64_t)c.k * 4;  // bytes
+  uint32_t load_tile = blockIdx.x, load_index = 0, load_slot = 0, load_n0 = 0, load_tokens = 0;
+  const uint8_t *load_w[Cfg::kMatrices] = {};
+  const T *load_x = nullptr;
   auto load = [&] {
     if (load_tile < tiles && mine > 0) {
-      const uint32_t n0 = load_tile / tiles_m * Cfg::kOutputs, m0 = load_tile % tiles_m * Cfg::kTokens, tokens = min(Cfg::kTokens, c.rows - m0);
+      if (load_index == 0) {
+        load_n0 = load_tile / tiles_m * Cfg::kOutputs;
+        const uint32_t m0 = load_tile % tiles_m * Cfg::kTokens;
+        load_tokens = min(Cfg::kTokens, c.rows - m0);
+        const uint64_t at = ((uint64_t)(load_n0 + wr * kTilesPerMatrix * 16 + g) * (c.k / 8) + unit * (kSlab / 8) + t * 4) * 4;
+        load_w[0] = reinterpret_cast<const uint8_t *>(c.w.packed) + at;
+        if (GATED) load_w[Cfg::kMatrices - 1] = reinterpret_cast<const uint8_t *>(c.up.packed) + at;
+        load_x = static_cast<const T *>(c.x) + (uint64_t)m0 * c.ldx;
+      }
       const uint32_t slab = unit + load_index * units, k0 = slab * kSlab, base = ring + load_slot * stage_bytes;
-      // Weight rows of 64 bytes, 16-byte pieces permuted by (row / 2) & 3 so that the eight rows of a fragment lie in different banks; eight of a
-      // tile's 16 rows at a time
+      const bool inside = k0 + t * 32 < c.k;
 #pragma unroll
       for (uint32_t i = 0; i < 2 * RT; ++i) {
-        const uint32_t rt = i >> 1, r = (i & 1) * 8 + g, row = n0 + col_of(rt) + r, at = (wr * RT + rt) * 16 + r;
-        const bool some = row < c.n && k0 + t * 32 < c.k;
-        const uint32_t *from = matrix_of(rt) ? c.up.packed : c.w.packed;
-        cp_async16(base + at * kWRow + (t ^ ((at >> 1) & 3)) * 16, some ? from + (uint64_t)row * (c.k / 8) + k0 / 8 + t * 4 : from, some);
+        const uint32_t m = i / (2 * kTilesPerMatrix), r = i % (2 * kTilesPerMatrix);
+        const bool some = inside && load_n0 + wr * kTilesPerMatrix * 16 + r * 8 + g < c.n;
+        cp_async16(base + w_to + i * 8 * kWRow, some ? load_w[m] + r * eight_rows : reinterpret_cast<const uint8_t *>(c.w.packed), some);
       }
-      // token rows, every other one with its halves of 64 bytes exchanged
-      constexpr uint32_t kPieces = Cfg::kXRow / 16, kPer = 16 / sizeof(T);
-      const T *x = static_cast<const T *>(c.x);
-      for (uint32_t i = in_kg; i < stored_tokens * kPieces; i += WR * 32) {
-        const uint32_t row = i / kPieces, piece = i % kPieces;
-        const bool some = row < tokens && k0 + piece * kPer < c.k;
-        cp_async16(base + Cfg::kWStage + row * Cfg::kXRow + (piece ^ ((row & 1) << 2)) * 16, some ? x + (uint64_t)(m0 + row) * c.ldx + k0 + piece * kPer : x, some);
-      }
-      // scales and zero points, in words: an odd number of outputs leaves them at any place within theirs
-      const uint32_t s_at = base + Cfg::kWStage + stored_tokens * Cfg::kXRow;
-      constexpr uint32_t kWords = Cfg::kScaleRow / 4, kZeroWords = Cfg::kZeroRow / 4;
 #pragma unroll
-      for (uint32_t j = 0; j < Cfg::kMatrices * kPerSlab; ++j) {
-        const W4View &w = j >= kPerSlab ? c.up : c.w;
-        const uint32_t group = slab * kPerSlab + j % kPerSlab;
-        const uint64_t first = (uint64_t)group * c.n + n0, scales = (uint64_t)groups * c.n;
-        for (uint32_t i = in_kg; i < kWords; i += WR * 32) {
-          const uint64_t at = (first & ~1ull) + 2 * i;
-          const uint32_t left = group < groups && at < scales ? (uint32_t)min(scales - at, (uint64_t)2) * 2 : 0;
-          cp_async4(s_at + j * Cfg::kScaleRow + i * 4, left ? w.scales + at : w.scales, left);
-        }
-        if (w.zeros) {
-          for (uint32_t i = in_kg; i < kZeroWords; i += WR * 32) {
-            const uint64_t at = (first & ~3ull) + 4 * i;
-            const uint32_t left = group < groups && at < scales ? (uint32_t)min(scales - at, (uint64_t)4) : 0;
-            cp_async4(s_at + Cfg::kMatrices * kPerSlab * Cfg::kScaleRow + j * Cfg::kZeroRow + i * 4, left ? w.zeros + at : w.zeros, left);
-          }
+      for (uint32_t m = 0; m < Cfg::kMatrices; ++m) load_w[m] += units * kWRow;
+#pragma unroll
+      for (uint32_t j = 0; j < kXTurns; ++j) {
+        const uint32_t i = in_kg + j * WR * 32, row = i / kPieces, piece = i % kPieces;
+        if (row < stored_tokens) {
+          const bool some = row < load_tokens && k0 + piece * kPer < c.k;
+          cp_async16(base + Cfg::kWStage + row * Cfg::kXRow + (piece ^ ((row & 1) << 2)) * 16, some ? load_x + row * c.ldx + k0 + piece * kPer : load_x, some);
         }
       }
+      load_params(base + Cfg::kWStage + stored_tokens * Cfg::kXRow, slab, load_n0);
       if (++load_index == mine) load_index = 0, load_tile += gridDim.x;
       load_slot = load_slot + 1 == kStages ? 0 : load_slot + 1;
     }
@@ -181,6 +230,14 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   };
 #pragma unroll
   for (uint32_t s = 0; s + 1 < kStages; ++s) load();
+
+  // Offsets of this lane's words in a stage: piece q of its weight rows, and its 16 (bf16) or 32 bytes of the tokens' 32 k, the latter for even and odd q
+  uint32_t w_from[kSlab / 32], x_from[2];
+#pragma unroll
+  for (uint32_t q = 0; q < kSlab / 32; ++q) w_from[q] = (wr * RT * 16 + g) * kWRow + (q ^ ((g >> 1) & 3)) * 16 + t * 4;
+#pragma unroll
+  for (uint32_t q = 0; q < 2; ++q)
+    x_from[q] = Cfg::kWStage + g * Cfg::kXRow + (kF32 ? (2 * t ^ ((g & 1) << 2)) * 16 : (q ^ (g & 1)) * 64 + t * 16);
 
   uint32_t slot = 0, turn = 0;
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= Cfg::kSets - 1) {
@@ -200,62 +257,56 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
       else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(WR * 32) : "memory");
       load();
 
-      const uint32_t w_at = ring + slot * stage_bytes, x_at = w_at + Cfg::kWStage, s_at = x_at + stored_tokens * Cfg::kXRow;
-      const uint32_t z_at = s_at + Cfg::kMatrices * kPerSlab * Cfg::kScaleRow;
+      const uint32_t base = ring + slot * stage_bytes, s_at = base + Cfg::kWStage + stored_tokens * Cfg::kXRow;
+      const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
       slot = slot + 1 == kStages ? 0 : slot + 1;
       float part[RT][NT][4];
       uint32_t minus_zero[RT][2];
-      float scale[RT][2];
 #pragma unroll
       for (uint32_t q = 0; q < kSlab / 32; ++q) {  // 32 k: one 16-byte piece of a weight row
-        if (q * 32 % GROUP == 0) {  // a group begins
-          const uint32_t first = ((unit + index * units) * kPerSlab + q * 32 / GROUP) * c.n + n0;  // its place within words: the low bits
+        const bool begins = q * 32 % GROUP == 0, ends = (q + 1) * 32 % GROUP == 0;
+        if (begins) {
 #pragma unroll
           for (uint32_t rt = 0; rt < RT; ++rt) {
-            const uint32_t j = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
-            const bool zeros = (matrix_of(rt) ? c.up : c.w).zeros != nullptr;
+            constexpr uint32_t kEight = 0xba80ba80u;  // -8 / kUnit
+            minus_zero[rt][0] = minus_zero[rt][1] = kEight;
+            if ((matrix_of(rt) ? c.up : c.w).zeros) {
+              const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
+              const uint32_t in_word = words ? 0 : (((unit + index * units) * kPerSlab + q * 32 / GROUP) * c.n + n0) & 3;
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-              const uint32_t at = col_of(rt) + h * 8 + g;
-              scale[rt][h] = __uint_as_float(lds16(s_at + j * Cfg::kScaleRow + ((first & 1) + at) * 2) << 16) * kUnit;
-              float z = -8.f / kUnit;
-              if (zeros) z = -(float)lds8(z_at + j * Cfg::kZeroRow + (first & 3) + at) / kUnit;  // eight bits at most: exact in bf16
-              minus_zero[rt][h] = upper_halves(z, z);
+              for (uint32_t h = 0; h < 2; ++h) {
+                const float z = (float)lds8(z_at + row * Cfg::kZeroRow + in_word + col_of(rt) + h * 8 + g) * (-1.f / kUnit);  // at most eight bits: exact in bf16
+                minus_zero[rt][h] = upper_halves(z, z);
+              }
             }
-#pragma unroll
-            for (uint32_t nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (uint32_t i = 0; i < 4; ++i) part[rt][nt][i] = 0.f;
           }
         }
         uint32_t a[RT][2][4];  // [rows 0-7 / 8-15][pair]
 #pragma unroll
         for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
-            const uint32_t at = (wr * RT + rt) * 16 + h * 8 + g;
-            dequant(lds32(w_at + at * kWRow + (q ^ ((at >> 1) & 3)) * 16 + t * 4), minus_zero[rt][h], a[rt][h]);
-          }
+          for (uint32_t h = 0; h < 2; ++h) dequant(lds32(base + w_from[q] + (rt * 16 + h * 8) * kWRow), minus_zero[rt][h], a[rt][h]);
 #pragma unroll
         for (uint32_t nt = 0; nt < NT; ++nt) {
-          const uint32_t row = nt * 8 + g;
-          auto multiply = [&](const uint32_t (&b)[4]) {
+          const bool stored = nt * 8 + g < stored_tokens;
+          auto multiply = [&](const uint32_t (&b)[4], bool first) {
 #pragma unroll
             for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
               for (uint32_t half = 0; half < 2; ++half) {
                 const uint32_t frag[4] = {a[rt][0][2 * half], a[rt][1][2 * half], a[rt][0][2 * half + 1], a[rt][1][2 * half + 1]};
-                mma_bf16_16816(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
+                if (first && half == 0) mma_first(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
+                else mma_bf16_16816(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
               }
           };
+          const uint32_t x_at = base + x_from[q & 1] + nt * 8 * Cfg::kXRow;
           if constexpr (kF32) {
             float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (row < stored_tokens) {
-#pragma unroll
-              for (uint32_t i = 0; i < 2; ++i) {
-                const uint4 r = lds128(x_at + row * Cfg::kXRow + ((q * 8 + t * 2 + i) ^ ((row & 1) << 2)) * 16);
-                v[4 * i] = __uint_as_float(r.x), v[4 * i + 1] = __uint_as_float(r.y), v[4 * i + 2] = __uint_as_float(r.z), v[4 * i + 3] = __uint_as_float(r.w);
-              }
+            if (stored) {
+              const uint32_t at = base + x_from[0] + nt * 8 * Cfg::kXRow + q * 128;
+              const uint4 lo = lds128(at), hi = lds128(at + 16);
+              v[0] = __uint_as_float(lo.x), v[1] = __uint_as_float(lo.y), v[2] = __uint_as_float(lo.z), v[3] = __uint_as_float(lo.w);
+              v[4] = __uint_as_float(hi.x), v[5] = __uint_as_float(hi.y), v[6] = __uint_as_float(hi.z), v[7] = __uint_as_float(hi.w);
             }
 #pragma unroll
             for (uint32_t term = 0; term < 3; ++term) {
@@ -266,22 +317,28 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
                 v[2 * i] = beyond(v[2 * i], first_bits(v[2 * i]));
                 v[2 * i + 1] = beyond(v[2 * i + 1], first_bits(v[2 * i + 1]));
               }
-              multiply(b);
+              multiply(b, begins && term == 0);
             }
           } else {
             uint4 r = make_uint4(0, 0, 0, 0);
-            if (row < stored_tokens) r = lds128(x_at + row * Cfg::kXRow + ((q * 4 + t) ^ ((row & 1) << 2)) * 16);
+            if (stored) r = lds128(x_at + (q >> 1) * 128);
             const uint32_t b[4] = {r.x, r.y, r.z, r.w};
-            multiply(b);
+            multiply(b, begins);
           }
         }
-        if ((q + 1) * 32 % GROUP == 0) {  // a group ends
+        if (ends) {
+          const uint32_t in_word = words ? 0 : (((unit + index * units) * kPerSlab + q * 32 / GROUP) * c.n + n0) & 1;
 #pragma unroll
           for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (uint32_t nt = 0; nt < NT; ++nt)
+            for (uint32_t h = 0; h < 2; ++h) {
+              const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
+              const float scale = __uint_as_float(lds16(s_at + row * Cfg::kScaleRow + (in_word + col_of(rt) + h * 8 + g) * 2) << 16);
 #pragma unroll
-              for (uint32_t i = 0; i < 4; ++i) sum[rt][nt][i] = fmaf(part[rt][nt][i], scale[rt][i >> 1], sum[rt][nt][i]);
+              for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (uint32_t i = 2 * h; i < 2 * h + 2; ++i) sum[rt][nt][i] = fmaf(part[rt][nt][i], scale, sum[rt][nt][i]);
+            }
         }
       }
     }
@@ -299,7 +356,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
           const uint32_t token = nt * 8 + t * 2 + (i & 1);
-          if (token < stored_tokens) mine_at[(kg * Cfg::kTokens + token) * Cfg::kTileRows + (wr * RT + rt) * 16 + (i >> 1) * 8 + g] = sum[rt][nt][i];
+          if (token < stored_tokens) mine_at[(kg * Cfg::kTokens + token) * Cfg::kTileRows + (wr * RT + rt) * 16 + (i >> 1) * 8 + g] = sum[rt][nt][i] * kUnit;
         }
     if (ranks > 1) cluster_barrier();
     else __syncthreads();
@@ -342,11 +399,16 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
   const uint32_t stored = std::min(c.rows, Cfg::kTokens), smem = Cfg::smem(stored);
   const uint64_t tiles = (uint64_t)tiles_n * tiles_m;
   if (tiles > 0x7fffffffull) return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
-  // k over a cluster while the tiles leave SMs without work and every k group keeps two slabs
+  // k over a cluster of `ranks` CTAs: as many as make the rounds of tiles shortest, a tile's end counted as two slabs
   const uint32_t resident = 148 * (NT == 1 && smem + 1024 <= 114 * 1024 ? 2 : 1), slabs = (c.k + kSlab - 1) / kSlab;
   uint32_t ranks = 1;
-  while (ranks < 8 && tiles * ranks * 2 <= resident && slabs >= Cfg::kKGroups * ranks * 4) ranks *= 2;
-  const uint32_t ctas = (uint32_t)std::min<uint64_t>(tiles, resident);
+  uint64_t best = ~0ull;
+  for (uint32_t r = 1; r <= 8; ++r) {
+    const uint64_t at_once = std::max(1u, resident / r), rounds = (tiles + at_once - 1) / at_once;
+    const uint64_t cost = rounds * ((slabs + Cfg::kKGroups * r - 1) / (Cfg::kKGroups * r) + 2);
+    if (cost < best) best = cost, ranks = r;
+  }
+  const uint32_t ctas = (uint32_t)std::min<uint64_t>(tiles, resident / ranks);
   ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(kernel, dim3(ctas, 1, ranks), dim3(kThreads), dim3(1, 1, ranks), smem, stream, c, (uint32_t)tiles, tiles_m,
                                                        stored, Cfg::stage(stored)));
   count_launch();
@@ -355,8 +417,8 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
 
 template <typename T, bool GATED, uint32_t GROUP>
 int launch_shape(const W4Call &c, cudaStream_t stream) {
-  if (c.rows <= 8) return launch_config<T, GATED, GROUP, 2, 1, 2>(c, stream);
-  if (c.rows <= 16) return launch_config<T, GATED, GROUP, 2, 2, 2>(c, stream);
+  if (c.rows <= 8) return launch_config<T, GATED, GROUP, 2, 1, 4>(c, stream);
+  if (c.rows <= 16) return launch_config<T, GATED, GROUP, 2, 2, 4>(c, stream);
   if constexpr (sizeof(T) == 2) {
     if (c.rows > 32) return launch_config<T, GATED, GROUP, 2, 8, 8>(c, stream);
   }
