@@ -30,6 +30,12 @@ constexpr float kUnit = 8192.f;        // dequantised codes are multiples of 1 /
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool some) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16u : 0u) : "memory");
 }
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void *src, bool some) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src), "r"((uint32_t)some) : "memory");
+}
+__device__ __forceinline__ void sts128_zero(uint32_t addr) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0u) : "memory"); }
+__device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((uint16_t)v) : "memory"); }
+__device__ __forceinline__ void sts8(uint32_t addr, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -103,22 +109,20 @@ struct FewConfig {
   static constexpr uint32_t kXRow = kSlab * sizeof(T);
   static constexpr uint32_t kWStage = kTileRows * kWRow;
   static constexpr uint32_t kPerSlab = kSlab / GROUP;                       // groups in a slab
-  // scales, and zero points, of a group and matrix: the outputs' and what stands before them in their first word
-  static constexpr uint32_t kScaleRow = kOutputs * 2 + 4, kZeroRow = kOutputs + 4;
+  static constexpr uint32_t kScaleRow = kOutputs * 2, kZeroRow = kOutputs;  // scales, and zero points, of a group and matrix
   static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + kZeroRow);
   static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows;         // floats of the sums that meet in shared memory
   // Slabs in the ring, and sets of sums: with few tokens two CTAs share an SM, with many one takes what there is.
   static constexpr uint32_t kStages = sizeof(T) == 4 ? 3 : 4, kSets = NT <= 2 ? 2 : 1;
-  static uint32_t stage(uint32_t tokens) { return (kWStage + tokens * kXRow + kSStage + 15) / 16 * 16; }
-  static uint32_t smem(uint32_t tokens) { return kKGroups * kStages * stage(tokens) + kSets * kSums * 4; }
+  static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kSmem = kKGroups * kStages * kStage + kSets * kSums * 4;
 };
 
 template <typename T, bool GATED, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
-w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, const uint32_t stored_tokens, const uint32_t stage_bytes) {
+w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, const uint32_t stored_tokens) {
   using Cfg = FewConfig<T, GATED, GROUP, RT, NT, WR>;
   constexpr bool kF32 = sizeof(T) == 4;
-  constexpr uint32_t kPerSlab = Cfg::kPerSlab, kStages = Cfg::kStages;
+  constexpr uint32_t kPerSlab = Cfg::kPerSlab, kStages = Cfg::kStages, kStageBytes = Cfg::kStage;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
 
@@ -128,8 +132,8 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   const uint32_t slabs = (c.k + kSlab - 1) / kSlab, units = Cfg::kKGroups * ranks, unit = rank * Cfg::kKGroups + kg;
   const uint32_t mine = unit < slabs ? (slabs - unit + units - 1) / units : 0;  // slabs of a tile that this k group takes
   const uint32_t groups = c.k / GROUP;
-  const uint32_t ring = smem_u32(smem) + kg * kStages * stage_bytes;
-  float *const sums = reinterpret_cast<float *>(smem + Cfg::kKGroups * kStages * stage_bytes);
+  const uint32_t ring = smem_u32(smem) + kg * kStages * kStageBytes;
+  float *const sums = reinterpret_cast<float *>(smem + Cfg::kKGroups * kStages * kStageBytes);
 
   // First output of a tile of 16 rows within the CTA's; with a gate the first half of a warp's tiles are the gate's.
   constexpr uint32_t kTilesPerMatrix = RT / Cfg::kMatrices;
@@ -137,12 +141,25 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   auto matrix_of = [&](uint32_t rt) { return rt / kTilesPerMatrix; };
   pdl_wait();
 
-  const bool words = (c.n & 3) == 0, any_zeros = c.w.zeros || c.up.zeros;
-  // Scales and zero points of a slab, in words. An odd number of outputs leaves them at any place within theirs; the first word then holds something before
-  // them. Pieces beyond the arrays are filled with zeros.
+  // Scales and zero points of a slab. Where the outputs are whole words (n a multiple of 4) they come by cp.async like the rest, zeros in place of groups
+  // beyond the last. Else they pass through registers: asked for with a slab, stored with the next one, long before they are read.
   constexpr uint32_t kScaleWords = Cfg::kOutputs / 2, kZeroWords = Cfg::kOutputs / 4, kRowsOfParams = Cfg::kMatrices * kPerSlab;
+  constexpr uint32_t kParamTurns = (kRowsOfParams * Cfg::kOutputs + WR * 32 - 1) / (WR * 32);
+  const bool words = (c.n & 3) == 0, any_zeros = c.w.zeros || c.up.zeros;
+  uint32_t held[kParamTurns], held_at = 0;  // scale | zero << 16, and where they go
+  auto store_held = [&] {
+    if (words || !held_at) return;
+#pragma unroll
+    for (uint32_t j = 0; j < kParamTurns; ++j) {
+      const uint32_t i = in_kg + j * WR * 32, row = i / Cfg::kOutputs, col = i % Cfg::kOutputs;
+      if (row < kRowsOfParams) {
+        sts16(held_at + row * Cfg::kScaleRow + col * 2, held[j] & 0xffffu);
+        sts8(held_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, held[j] >> 16);
+      }
+    }
+    held_at = 0;
+  };
   auto load_params = [&](uint32_t s_at, uint32_t slab, uint32_t n0) {
-    const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
     if (words) {
 #pragma unroll
       for (uint32_t j = 0; j < (kRowsOfParams * kScaleWords + WR * 32 - 1) / (WR * 32); ++j) {
@@ -160,74 +177,78 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
         const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
         if (row < kRowsOfParams && p) {
           const bool some = group < groups && n0 + col < c.n;
-          cp_async4(z_at + row * Cfg::kZeroRow + col, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
+          cp_async4(s_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
         }
       }
     } else {
-      const uint64_t all = (uint64_t)groups * c.n;
-#pragma unroll 1
-      for (uint32_t row = 0; row < kRowsOfParams; ++row) {
-        const W4View &w = row >= kPerSlab ? c.up : c.w;
-        const uint32_t group = slab * kPerSlab + row % kPerSlab;
-        const uint64_t first = (uint64_t)group * c.n + n0;
-        for (uint32_t i = in_kg; i < kScaleWords + 1; i += WR * 32) {
-          const uint64_t at = (first & ~1ull) + 2 * i;
-          const uint32_t left = group < groups && at < all ? (uint32_t)min(all - at, (uint64_t)2) * 2 : 0;
-          cp_async4(s_at + row * Cfg::kScaleRow + i * 4, left ? w.scales + at : w.scales, left);
-        }
-        for (uint32_t i = in_kg; w.zeros && i < kZeroWords + 1; i += WR * 32) {
-          const uint64_t at = (first & ~3ull) + 4 * i;
-          const uint32_t left = group < groups && at < all ? (uint32_t)min(all - at, (uint64_t)4) : 0;
-          cp_async4(z_at + row * Cfg::kZeroRow + i * 4, left ? w.zeros + at : w.zeros, left);
+      held_at = s_at;
+#pragma unroll
+      for (uint32_t j = 0; j < kParamTurns; ++j) {
+        const uint32_t i = in_kg + j * WR * 32, row = i / Cfg::kOutputs, col = i % Cfg::kOutputs, group = slab * kPerSlab + row % kPerSlab;
+        held[j] = 0;
+        if (row < kRowsOfParams && group < groups && n0 + col < c.n) {
+          const W4View &w = row >= kPerSlab ? c.up : c.w;
+          const uint64_t at = (uint64_t)group * c.n + n0 + col;
+          held[j] = __ldg(reinterpret_cast<const uint16_t *>(w.scales) + at) | (w.zeros ? (uint32_t)__ldg(w.zeros + at) << 16 : 0);
         }
       }
     }
   };
+
   // What is loaded next: a slab of a tile. The loads run ahead of the products across tiles, so that the ring never drains.
   //
   // Weight rows of 64 bytes, 16-byte pieces permuted by (row / 2) & 3 so that the eight rows of a fragment lie in different banks; a lane copies piece t of
-  // the rows g, g + 8, .. of its warp's tiles. Token rows: every other one with its halves of 64 bytes exchanged.
+  // the rows g, g + 8, .. of its warp's tiles. Rows beyond the last are left as they are: nothing of them is stored. Token rows: every other one with its
+  // halves of 64 bytes exchanged, zeros beyond the last k.
   constexpr uint32_t kPieces = Cfg::kXRow / 16, kPer = 16 / sizeof(T), kXTurns = (Cfg::kTokens * kPieces + WR * 32 - 1) / (WR * 32);
+  constexpr uint32_t kXStep = WR * 32 / kPieces;  // token rows from one turn to the next, an even number
+  static_assert(kXStep % 2 == 0, "rows of a lane's turns are permuted alike");
   const uint32_t w_to = wr * RT * 16 * kWRow + g * kWRow + (t ^ ((g >> 1) & 3)) * 16;
-  const uint64_t eight_rows = (uint64_t)c.k * 4;  // bytes
-  uint32_t load_tile = blockIdx.x, load_index = 0, load_slot = 0, load_n0 = 0, load_tokens = 0;
-  const uint8_t *load_w[Cfg::kMatrices] = {};
-  const T *load_x = nullptr;
+  const uint32_t x_row = in_kg / kPieces, x_piece = in_kg % kPieces, x_to = Cfg::kWStage + x_row * Cfg::kXRow + (x_piece ^ ((x_row & 1) << 2)) * 16;
+  const uint64_t eight_rows = (uint64_t)c.k * 4, x_step = kXStep * c.ldx * sizeof(T);  // bytes
+  uint32_t load_tile = blockIdx.x, load_index = 0, load_slot = 0, load_n0 = 0, load_tokens = 0, load_rows = 0;
+  const uint8_t *load_w[Cfg::kMatrices] = {}, *load_x = nullptr;
   auto load = [&] {
+    store_held();
     if (load_tile < tiles && mine > 0) {
       if (load_index == 0) {
         load_n0 = load_tile / tiles_m * Cfg::kOutputs;
-        const uint32_t m0 = load_tile % tiles_m * Cfg::kTokens;
+        const uint32_t m0 = load_tile % tiles_m * Cfg::kTokens, row = load_n0 + wr * kTilesPerMatrix * 16 + g;
         load_tokens = min(Cfg::kTokens, c.rows - m0);
-        const uint64_t at = ((uint64_t)(load_n0 + wr * kTilesPerMatrix * 16 + g) * (c.k / 8) + unit * (kSlab / 8) + t * 4) * 4;
+        load_rows = row < c.n ? (c.n - row + 7) / 8 : 0;  // of this lane's, per matrix
+        const uint64_t at = ((uint64_t)row * (c.k / 8) + unit * (kSlab / 8) + t * 4) * 4;
         load_w[0] = reinterpret_cast<const uint8_t *>(c.w.packed) + at;
         if (GATED) load_w[Cfg::kMatrices - 1] = reinterpret_cast<const uint8_t *>(c.up.packed) + at;
-        load_x = static_cast<const T *>(c.x) + (uint64_t)m0 * c.ldx;
+        load_x = static_cast<const uint8_t *>(c.x) + ((uint64_t)(m0 + x_row) * c.ldx + unit * kSlab + x_piece * kPer) * sizeof(T);
       }
-      const uint32_t slab = unit + load_index * units, k0 = slab * kSlab, base = ring + load_slot * stage_bytes;
-      const bool inside = k0 + t * 32 < c.k;
+      const uint32_t slab = unit + load_index * units, k0 = slab * kSlab, base = ring + load_slot * kStageBytes;
+      const uint32_t rows = k0 + t * 32 < c.k ? load_rows : 0;
 #pragma unroll
       for (uint32_t i = 0; i < 2 * RT; ++i) {
         const uint32_t m = i / (2 * kTilesPerMatrix), r = i % (2 * kTilesPerMatrix);
-        const bool some = inside && load_n0 + wr * kTilesPerMatrix * 16 + r * 8 + g < c.n;
-        cp_async16(base + w_to + i * 8 * kWRow, some ? load_w[m] + r * eight_rows : reinterpret_cast<const uint8_t *>(c.w.packed), some);
+        cp_async16_if(base + w_to + i * 8 * kWRow, load_w[m] + r * eight_rows, r < rows);
       }
 #pragma unroll
       for (uint32_t m = 0; m < Cfg::kMatrices; ++m) load_w[m] += units * kWRow;
+      const bool x_inside = k0 + x_piece * kPer < c.k;
 #pragma unroll
       for (uint32_t j = 0; j < kXTurns; ++j) {
-        const uint32_t i = in_kg + j * WR * 32, row = i / kPieces, piece = i % kPieces;
+        const uint32_t row = x_row + j * kXStep;
         if (row < stored_tokens) {
-          const bool some = row < load_tokens && k0 + piece * kPer < c.k;
-          cp_async16(base + Cfg::kWStage + row * Cfg::kXRow + (piece ^ ((row & 1) << 2)) * 16, some ? load_x + row * c.ldx + k0 + piece * kPer : load_x, some);
+          const bool some = row < load_tokens && x_inside;
+          cp_async16(base + x_to + j * kXStep * Cfg::kXRow, some ? load_x + j * x_step : static_cast<const uint8_t *>(c.x), some);
         }
       }
-      load_params(base + Cfg::kWStage + stored_tokens * Cfg::kXRow, slab, load_n0);
+      load_x += (uint64_t)units * kSlab * sizeof(T);
+      load_params(base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow, slab, load_n0);
       if (++load_index == mine) load_index = 0, load_tile += gridDim.x;
       load_slot = load_slot + 1 == kStages ? 0 : load_slot + 1;
     }
     cp_async_commit();
   };
+  // token rows that nothing is loaded to
+  for (uint32_t s = 0; s < kStages; ++s)
+    for (uint32_t i = stored_tokens * kPieces + in_kg; i < Cfg::kTokens * kPieces; i += WR * 32) sts128_zero(ring + s * kStageBytes + Cfg::kWStage + i * 16);
 #pragma unroll
   for (uint32_t s = 0; s + 1 < kStages; ++s) load();
 
@@ -257,7 +278,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
       else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(WR * 32) : "memory");
       load();
 
-      const uint32_t base = ring + slot * stage_bytes, s_at = base + Cfg::kWStage + stored_tokens * Cfg::kXRow;
+      const uint32_t base = ring + slot * kStageBytes, s_at = base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow;
       const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
       slot = slot + 1 == kStages ? 0 : slot + 1;
       float part[RT][NT][4];
@@ -272,10 +293,9 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
             minus_zero[rt][0] = minus_zero[rt][1] = kEight;
             if ((matrix_of(rt) ? c.up : c.w).zeros) {
               const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
-              const uint32_t in_word = words ? 0 : (((unit + index * units) * kPerSlab + q * 32 / GROUP) * c.n + n0) & 3;
 #pragma unroll
               for (uint32_t h = 0; h < 2; ++h) {
-                const float z = (float)lds8(z_at + row * Cfg::kZeroRow + in_word + col_of(rt) + h * 8 + g) * (-1.f / kUnit);  // at most eight bits: exact in bf16
+                const float z = (float)lds8(z_at + row * Cfg::kZeroRow + col_of(rt) + h * 8 + g) * (-1.f / kUnit);  // at most eight bits: exact in bf16
                 minus_zero[rt][h] = upper_halves(z, z);
               }
             }
@@ -288,7 +308,6 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
           for (uint32_t h = 0; h < 2; ++h) dequant(lds32(base + w_from[q] + (rt * 16 + h * 8) * kWRow), minus_zero[rt][h], a[rt][h]);
 #pragma unroll
         for (uint32_t nt = 0; nt < NT; ++nt) {
-          const bool stored = nt * 8 + g < stored_tokens;
           auto multiply = [&](const uint32_t (&b)[4], bool first) {
 #pragma unroll
             for (uint32_t rt = 0; rt < RT; ++rt)
@@ -301,13 +320,10 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
           };
           const uint32_t x_at = base + x_from[q & 1] + nt * 8 * Cfg::kXRow;
           if constexpr (kF32) {
-            float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (stored) {
-              const uint32_t at = base + x_from[0] + nt * 8 * Cfg::kXRow + q * 128;
-              const uint4 lo = lds128(at), hi = lds128(at + 16);
-              v[0] = __uint_as_float(lo.x), v[1] = __uint_as_float(lo.y), v[2] = __uint_as_float(lo.z), v[3] = __uint_as_float(lo.w);
-              v[4] = __uint_as_float(hi.x), v[5] = __uint_as_float(hi.y), v[6] = __uint_as_float(hi.z), v[7] = __uint_as_float(hi.w);
-            }
+            const uint32_t at = base + x_from[0] + nt * 8 * Cfg::kXRow + q * 128;
+            const uint4 lo = lds128(at), hi = lds128(at + 16);
+            float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
+                          __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
 #pragma unroll
             for (uint32_t term = 0; term < 3; ++term) {
               uint32_t b[4];
@@ -320,20 +336,18 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
               multiply(b, begins && term == 0);
             }
           } else {
-            uint4 r = make_uint4(0, 0, 0, 0);
-            if (stored) r = lds128(x_at + (q >> 1) * 128);
+            const uint4 r = lds128(x_at + (q >> 1) * 128);
             const uint32_t b[4] = {r.x, r.y, r.z, r.w};
             multiply(b, begins);
           }
         }
         if (ends) {
-          const uint32_t in_word = words ? 0 : (((unit + index * units) * kPerSlab + q * 32 / GROUP) * c.n + n0) & 1;
 #pragma unroll
           for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
               const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
-              const float scale = __uint_as_float(lds16(s_at + row * Cfg::kScaleRow + (in_word + col_of(rt) + h * 8 + g) * 2) << 16);
+              const float scale = __uint_as_float(lds16(s_at + row * Cfg::kScaleRow + (col_of(rt) + h * 8 + g) * 2) << 16);
 #pragma unroll
               for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -394,9 +408,9 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
   using Cfg = FewConfig<T, GATED, GROUP, RT, NT, WR>;
   static bool done[kMaxDeviceOrdinals] = {};
   const auto kernel = w4_few_kernel<T, GATED, GROUP, RT, NT, WR>;
-  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(kernel, (int)Cfg::smem(Cfg::kTokens), done));
+  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(kernel, (int)Cfg::kSmem, done));
   const uint32_t tiles_n = (c.n + Cfg::kOutputs - 1) / Cfg::kOutputs, tiles_m = (c.rows + Cfg::kTokens - 1) / Cfg::kTokens;
-  const uint32_t stored = std::min(c.rows, Cfg::kTokens), smem = Cfg::smem(stored);
+  const uint32_t stored = std::min(c.rows, Cfg::kTokens), smem = Cfg::kSmem;
   const uint64_t tiles = (uint64_t)tiles_n * tiles_m;
   if (tiles > 0x7fffffffull) return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
   // k over a cluster of `ranks` CTAs: as many as make the rounds of tiles shortest, a tile's end counted as two slabs
@@ -410,7 +424,7 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
   }
   const uint32_t ctas = (uint32_t)std::min<uint64_t>(tiles, resident / ranks);
   ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(kernel, dim3(ctas, 1, ranks), dim3(kThreads), dim3(1, 1, ranks), smem, stream, c, (uint32_t)tiles, tiles_m,
-                                                       stored, Cfg::stage(stored)));
+                                                       stored));
   count_launch();
   return ORION_OK;
 }
