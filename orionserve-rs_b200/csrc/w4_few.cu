@@ -34,6 +34,7 @@ __device__ __forceinline__ void cp_async16_if(uint32_t dst, const void *src, boo
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src), "r"((uint32_t)some) : "memory");
 }
 __device__ __forceinline__ void sts128_zero(uint32_t addr) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0u) : "memory"); }
+__device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((uint16_t)v) : "memory"); }
 __device__ __forceinline__ void sts8(uint32_t addr, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, uint32_t bytes) {
@@ -99,7 +100,7 @@ __device__ __forceinline__ float beyond(float x, float first) { return x == firs
 __device__ __forceinline__ float first_bits(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
 
-template <typename T, bool GATED, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
+template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
 struct FewConfig {
   static constexpr uint32_t kKGroups = kWarps / WR;
   static constexpr uint32_t kTileRows = 16 * RT * WR;                       // rows of weights per CTA, gate and up together
@@ -110,17 +111,17 @@ struct FewConfig {
   static constexpr uint32_t kWStage = kTileRows * kWRow;
   static constexpr uint32_t kPerSlab = kSlab / GROUP;                       // groups in a slab
   static constexpr uint32_t kScaleRow = kOutputs * 2, kZeroRow = kOutputs;  // scales, and zero points, of a group and matrix
-  static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + kZeroRow);
+  static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + (ZEROS ? kZeroRow : 0));
   static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows;         // floats of the sums that meet in shared memory
   // Slabs in the ring, and sets of sums: with few tokens two CTAs share an SM, with many one takes what there is.
   static constexpr uint32_t kStages = sizeof(T) == 4 ? 3 : 4, kSets = NT <= 2 ? 2 : 1;
   static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kSmem = kKGroups * kStages * kStage + kSets * kSums * 4;
 };
 
-template <typename T, bool GATED, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
+template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
 w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, const uint32_t stored_tokens) {
-  using Cfg = FewConfig<T, GATED, GROUP, RT, NT, WR>;
+  using Cfg = FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr uint32_t kPerSlab = Cfg::kPerSlab, kStages = Cfg::kStages, kStageBytes = Cfg::kStage;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -145,7 +146,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   // beyond the last. Else they pass through registers: asked for with a slab, stored with the next one, long before they are read.
   constexpr uint32_t kScaleWords = Cfg::kOutputs / 2, kZeroWords = Cfg::kOutputs / 4, kRowsOfParams = Cfg::kMatrices * kPerSlab;
   constexpr uint32_t kParamTurns = (kRowsOfParams * Cfg::kOutputs + WR * 32 - 1) / (WR * 32);
-  const bool words = (c.n & 3) == 0, any_zeros = c.w.zeros || c.up.zeros;
+  const bool words = (c.n & 3) == 0;
   uint32_t held[kParamTurns], held_at = 0;  // scale | zero << 16, and where they go
   auto store_held = [&] {
     if (words || !held_at) return;
@@ -154,7 +155,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
       const uint32_t i = in_kg + j * WR * 32, row = i / Cfg::kOutputs, col = i % Cfg::kOutputs;
       if (row < kRowsOfParams) {
         sts16(held_at + row * Cfg::kScaleRow + col * 2, held[j] & 0xffffu);
-        sts8(held_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, held[j] >> 16);
+        if (ZEROS) sts8(held_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, held[j] >> 16);
       }
     }
     held_at = 0;
@@ -170,12 +171,14 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
           cp_async4(s_at + row * Cfg::kScaleRow + col * 2, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
         }
       }
-      if (!any_zeros) return;
+      if (!ZEROS) return;
 #pragma unroll
       for (uint32_t j = 0; j < (kRowsOfParams * kZeroWords + WR * 32 - 1) / (WR * 32); ++j) {
         const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords, col = i % kZeroWords * 4, group = slab * kPerSlab + row % kPerSlab;
         const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
-        if (row < kRowsOfParams && p) {
+        if (row < kRowsOfParams && !p) {
+          sts32(s_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, 0x08080808u);
+        } else if (row < kRowsOfParams) {
           const bool some = group < groups && n0 + col < c.n;
           cp_async4(s_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
         }
@@ -189,7 +192,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
         if (row < kRowsOfParams && group < groups && n0 + col < c.n) {
           const W4View &w = row >= kPerSlab ? c.up : c.w;
           const uint64_t at = (uint64_t)group * c.n + n0 + col;
-          held[j] = __ldg(reinterpret_cast<const uint16_t *>(w.scales) + at) | (w.zeros ? (uint32_t)__ldg(w.zeros + at) << 16 : 0);
+          held[j] = __ldg(reinterpret_cast<const uint16_t *>(w.scales) + at) | (!ZEROS ? 0 : w.zeros ? (uint32_t)__ldg(w.zeros + at) << 16 : 8u << 16);
         }
       }
     }
@@ -288,18 +291,16 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
         const bool begins = q * 32 % GROUP == 0, ends = (q + 1) * 32 % GROUP == 0;
         if (begins) {
 #pragma unroll
-          for (uint32_t rt = 0; rt < RT; ++rt) {
-            constexpr uint32_t kEight = 0xba80ba80u;  // -8 / kUnit
-            minus_zero[rt][0] = minus_zero[rt][1] = kEight;
-            if ((matrix_of(rt) ? c.up : c.w).zeros) {
-              const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
+          for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-              for (uint32_t h = 0; h < 2; ++h) {
-                const float z = (float)lds8(z_at + row * Cfg::kZeroRow + col_of(rt) + h * 8 + g) * (-1.f / kUnit);  // at most eight bits: exact in bf16
-                minus_zero[rt][h] = upper_halves(z, z);
+            for (uint32_t h = 0; h < 2; ++h) {
+              minus_zero[rt][h] = 0xba80ba80u;  // -8 / kUnit
+              if (ZEROS) {
+                const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
+                // as the codes: at most eight bits, so exact
+                minus_zero[rt][h] = fma_bf16x2(lds8(z_at + row * Cfg::kZeroRow + col_of(rt) + h * 8 + g) * 0x10001u, 0xfb80fb80u, 0x80008000u);
               }
             }
-          }
         }
         uint32_t a[RT][2][4];  // [rows 0-7 / 8-15][pair]
 #pragma unroll
@@ -403,11 +404,11 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   if (ranks > 1) cluster_barrier();  // nobody leaves while its sums are being read
 }
 
-template <typename T, bool GATED, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
+template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
 int launch_config(const W4Call &c, cudaStream_t stream) {
-  using Cfg = FewConfig<T, GATED, GROUP, RT, NT, WR>;
+  using Cfg = FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   static bool done[kMaxDeviceOrdinals] = {};
-  const auto kernel = w4_few_kernel<T, GATED, GROUP, RT, NT, WR>;
+  const auto kernel = w4_few_kernel<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(kernel, (int)Cfg::kSmem, done));
   const uint32_t tiles_n = (c.n + Cfg::kOutputs - 1) / Cfg::kOutputs, tiles_m = (c.rows + Cfg::kTokens - 1) / Cfg::kTokens;
   const uint32_t stored = std::min(c.rows, Cfg::kTokens), smem = Cfg::kSmem;
@@ -429,22 +430,22 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
   return ORION_OK;
 }
 
-template <typename T, bool GATED, uint32_t GROUP>
+template <typename T, bool GATED, bool ZEROS, uint32_t GROUP>
 int launch_shape(const W4Call &c, cudaStream_t stream) {
-  if (c.rows <= 8) return launch_config<T, GATED, GROUP, 2, 1, 4>(c, stream);
-  if (c.rows <= 16) return launch_config<T, GATED, GROUP, 2, 2, 4>(c, stream);
+  if (c.rows <= 8) return launch_config<T, GATED, ZEROS, GROUP, 2, 1, 4>(c, stream);
+  if (c.rows <= 16) return launch_config<T, GATED, ZEROS, GROUP, 2, 2, 4>(c, stream);
   if constexpr (sizeof(T) == 2) {
-    if (c.rows > 32) return launch_config<T, GATED, GROUP, 2, 8, 8>(c, stream);
+    if (c.rows > 32) return launch_config<T, GATED, ZEROS, GROUP, 2, 8, 8>(c, stream);
   }
-  return launch_config<T, GATED, GROUP, 2, 4, 4>(c, stream);
+  return launch_config<T, GATED, ZEROS, GROUP, 2, 4, 4>(c, stream);
 }
 
-template <typename T, bool GATED>
+template <typename T, bool GATED, bool ZEROS>
 int launch_group(const W4Call &c, cudaStream_t stream) {
   switch (c.group) {
-    case 32: return launch_shape<T, GATED, 32>(c, stream);
-    case 64: return launch_shape<T, GATED, 64>(c, stream);
-    default: return launch_shape<T, GATED, 128>(c, stream);
+    case 32: return launch_shape<T, GATED, ZEROS, 32>(c, stream);
+    case 64: return launch_shape<T, GATED, ZEROS, 64>(c, stream);
+    default: return launch_shape<T, GATED, ZEROS, 128>(c, stream);
   }
 }
 
@@ -452,7 +453,9 @@ int launch_group(const W4Call &c, cudaStream_t stream) {
 
 template <typename T>
 int launch_w4_few(const W4Call &c, cudaStream_t stream) {
-  return c.up.packed ? launch_group<T, true>(c, stream) : launch_group<T, false>(c, stream);
+  const bool zeros = c.w.zeros || c.up.zeros;
+  if (c.up.packed) return zeros ? launch_group<T, true, true>(c, stream) : launch_group<T, true, false>(c, stream);
+  return zeros ? launch_group<T, false, true>(c, stream) : launch_group<T, false, false>(c, stream);
 }
 template int launch_w4_few<float>(const W4Call &, cudaStream_t);
 template int launch_w4_few<bf16>(const W4Call &, cudaStream_t);
