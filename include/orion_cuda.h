@@ -493,7 +493,8 @@ void orion_cuda_attn_bench_destroy(OrionAttnBench *bench);
  * 128) consecutive k of a row. All pointers are DEVICE pointers; the calls check what can be checked on the host, allocate
  * nothing, only enqueue work on `stream` (a cudaStream_t, NULL = the default stream) of `device`, which is current during the
  * call and put back, and can be captured into a graph. They hold no state: calls on different streams and from different
- * threads do not touch one another. Results do not vary from run to run.
+ * threads do not touch one another, given workspaces of their own. Results do not vary from run to run. A bounded wait inside
+ * the kernels for many rows that gives up sets the device's word of the projections (orion_cuda_poll_wait_timeouts, bit 0).
  *   packed  u32 [out_features][in_features / 8], 16-byte aligned. Of eight consecutive k, number 2i is in bits 4i .. 4i + 3
  *           of their word, number 2i + 1 in bits 16 + 4i .. 19 + 4i.
  *   scales  bf16 [in_features / group][out_features], 4-byte aligned
@@ -512,15 +513,21 @@ enum { ORION_GATE_SILU = 0, ORION_GATE_GELU_TANH = 1 };
  * the even one. A group with an infinity or a NaN gets a scale of NaN. */
 int orion_cuda_w4_quantize(int device, int dtype, const void *weight, uint64_t out_features, uint64_t in_features,
                            uint64_t row_stride, uint32_t group, void *packed, void *scales, void *zeros, void *stream);
+/* Bytes of device memory that orion_cuda_w4_linear (gated 0) or orion_cuda_w4_gated (gated 1) needs beside its arguments for
+ * `rows` rows: 0 for f32 and for few rows. */
+int orion_cuda_w4_workspace(int dtype, uint64_t rows, const OrionW4Weight *weight, int gated, uint64_t *bytes);
 /* y = x W^T + bias: tensor::linear (tensor.rs:96-130) with such weights. x and out hold values of `dtype` (f32 or bf16), rows
  * x_stride and out_stride values apart; bias is f32 [out_features] or NULL. Sums are held in f32 and rounded once. `out`
- * overlaps no input. */
+ * overlaps no input. `workspace` (256-byte aligned, orion_cuda_w4_workspace bytes; NULL where that is 0) belongs to the call
+ * until its work has ended; its contents need no preparation and are of no use afterwards. */
 int orion_cuda_w4_linear(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *weight,
-                         const float *bias, void *out, uint64_t out_stride, void *stream);
+                         const float *bias, void *out, uint64_t out_stride, void *workspace, uint64_t workspace_bytes,
+                         void *stream);
 /* y = f(x Wgate^T) * (x Wup^T), f = silu or the tanh form of GELU: both projections, the activation and the product (tensor.rs:
- * 96-130, 175-189) in one kernel; the two matrices have the same sizes and groups. */
+ * 96-130, 175-189); the two matrices have the same sizes and groups. */
 int orion_cuda_w4_gated(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *gate,
-                        const OrionW4Weight *up, int activation, void *out, uint64_t out_stride, void *stream);
+                        const OrionW4Weight *up, int activation, void *out, uint64_t out_stride, void *workspace,
+                        uint64_t workspace_bytes, void *stream);
 
 /* ---- decode attention for callers that cannot allocate ----
  * This entry point has no counterpart in the reference. It is the paged GQA

@@ -153,8 +153,9 @@ SIGNATURES = {
     "orion_cuda_paged_decode_attention_noalloc": (_int, [_int, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _vp,
                                                          _vp, _u32, _u32, _u32, _vp, _vp]),
     "orion_cuda_w4_quantize": (_int, [_int, _int, _vp, _u64, _u64, _u64, _u32, _vp, _vp, _vp, _vp]),
-    "orion_cuda_w4_linear": (_int, [_int, _int, _vp, _u64, _u64, _vp, _vp, _vp, _u64, _vp]),
-    "orion_cuda_w4_gated": (_int, [_int, _int, _vp, _u64, _u64, _vp, _vp, _int, _vp, _u64, _vp]),
+    "orion_cuda_w4_workspace": (_int, [_int, _u64, _vp, _int, _u64p]),
+    "orion_cuda_w4_linear": (_int, [_int, _int, _vp, _u64, _u64, _vp, _vp, _vp, _u64, _vp, _u64, _vp]),
+    "orion_cuda_w4_gated": (_int, [_int, _int, _vp, _u64, _u64, _vp, _vp, _int, _vp, _u64, _vp, _u64, _vp]),
 }
 
 

@@ -3,6 +3,8 @@
 #include "kernels.h"
 #include "w4.cuh"
 
+#include <atomic>
+
 namespace orion {
 namespace {
 
@@ -64,10 +66,37 @@ int check_product(int dtype, const void *x, uint64_t rows, uint64_t x_stride, co
   return ORION_OK;
 }
 
-int launch(int device, int dtype, const W4Call &c, cudaStream_t stream) {
+// The pairs of CTAs take bf16 products of more rows than this, and of at least a swizzle atom of k.
+constexpr uint64_t kFewRows = 16;
+bool takes_pairs(int dtype, uint64_t rows, uint64_t k) { return dtype == ORION_DTYPE_BF16 && rows > kFewRows && k >= 64; }
+
+// Address of the projections' error word, looked up once per device.
+int error_word(int device, uint32_t **word) {
+  static std::atomic<uint32_t *> known[kMaxDeviceOrdinals];
+  const bool tracked = device >= 0 && device < kMaxDeviceOrdinals;
+  *word = tracked ? known[device].load(std::memory_order_acquire) : nullptr;
+  if (*word) return ORION_OK;
+  *word = static_cast<uint32_t *>(const_cast<void *>(gemm_tc_error_word()));
+  if (!*word) return set_error(ORION_ERR_BACKEND, "backend cuda failed at error word: %s", cudaGetErrorString(cudaGetLastError()));
+  if (tracked) known[device].store(*word, std::memory_order_release);
+  return ORION_OK;
+}
+
+int launch(int device, int dtype, const W4Call &c, void *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
+  if (!takes_pairs(dtype, c.rows, c.k)) {
+    ScopedDevice current(device);
+    ORION_CUDA_CHECK("set device", current.status);
+    return dtype == ORION_DTYPE_F32 ? launch_w4_few<float>(c, stream) : launch_w4_few<bf16>(c, stream);
+  }
+  const uint64_t need = w4_pair_workspace(c.rows, c.up.packed ? 2 * c.n : c.n, c.k);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return set_error(ORION_ERR_INVALID_REQUEST, "a workspace of %llu bytes on a 256-byte boundary is needed, got %llu", (unsigned long long)need,
+                     (unsigned long long)(workspace ? workspace_bytes : 0));
   ScopedDevice current(device);
   ORION_CUDA_CHECK("set device", current.status);
-  return dtype == ORION_DTYPE_F32 ? launch_w4_few<float>(c, stream) : launch_w4_few<bf16>(c, stream);
+  uint32_t *error = nullptr;
+  ORION_TRY(error_word(device, &error));
+  return launch_w4_pair(c, workspace, error, stream);
 }
 
 }  // namespace
@@ -99,19 +128,30 @@ int orion_cuda_w4_quantize(int device, int dtype, const void *weight, uint64_t o
                                   : launch_w4_quantize(static_cast<const bf16 *>(weight), row_stride, n, k, group, p, s, z, st);
 }
 
+int orion_cuda_w4_workspace(int dtype, uint64_t rows, const OrionW4Weight *weight, int gated, uint64_t *bytes) {
+  clear_error();
+  if (!bytes) return set_error(ORION_ERR_INVALID_REQUEST, "null pointer argument");
+  *bytes = 0;
+  ORION_TRY(check_dtype(dtype));
+  ORION_TRY(check_weight("weight", weight));
+  if (rows > kMostRows) return set_error(ORION_ERR_INVALID_REQUEST, "%llu rows: at most 2^30 are possible", (unsigned long long)rows);
+  if (takes_pairs(dtype, rows, weight->in_features)) *bytes = w4_pair_workspace((uint32_t)rows, (uint32_t)weight->out_features * (gated ? 2 : 1), (uint32_t)weight->in_features);
+  return ORION_OK;
+}
+
 int orion_cuda_w4_linear(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *weight, const float *bias, void *out,
-                         uint64_t out_stride, void *stream) {
+                         uint64_t out_stride, void *workspace, uint64_t workspace_bytes, void *stream) {
   clear_error();
   W4Call c;
   ORION_TRY(check_product(dtype, x, rows, x_stride, weight, out, out_stride, &c));
   if (rows == 0) return ORION_OK;
   if (!aligned(bias, 4)) return set_error(ORION_ERR_INVALID_REQUEST, "bias: not aligned to its type");
   c.bias = bias;
-  return launch(device, dtype, c, static_cast<cudaStream_t>(stream));
+  return launch(device, dtype, c, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 int orion_cuda_w4_gated(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *gate, const OrionW4Weight *up,
-                        int activation, void *out, uint64_t out_stride, void *stream) {
+                        int activation, void *out, uint64_t out_stride, void *workspace, uint64_t workspace_bytes, void *stream) {
   clear_error();
   W4Call c;
   ORION_TRY(check_weight("up", up));
@@ -125,7 +165,7 @@ int orion_cuda_w4_gated(int device, int dtype, const void *x, uint64_t rows, uin
   if (rows == 0) return ORION_OK;
   c.up = view(up);
   c.act = activation == ORION_GATE_SILU ? kGatedSilu : kGatedGelu;
-  return launch(device, dtype, c, static_cast<cudaStream_t>(stream));
+  return launch(device, dtype, c, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -11,7 +11,7 @@
 //
 // A CTA of eight warps: WR of them side by side over weight rows, 8 / WR groups of them over k. Few tokens: WR = 1, every warp streams k slabs of its own
 // and only reads the tokens' values it needs; more tokens: warps share the tokens' slab, so that L2 delivers it less often. Each k group has a ring of
-// slabs of 128 k, weights, tokens and scales, filled by cp.async (no waits on barriers). CTAs stay and go from tile to tile, with the ring running ahead
+// slabs of 128 or 256 k, weights, tokens and scales, filled by cp.async (no waits on barriers). CTAs stay and go from tile to tile, with the ring running ahead
 // across tiles. Sums of k groups meet in shared memory, and where the rows of weights give too few CTAs the k of a tile is dealt to the CTAs of a cluster, whose sums meet over
 // distributed shared memory: in both places in a fixed order, so results do not vary from run to run, and no workspace is needed.
 #include "kernels.h"
@@ -23,8 +23,7 @@
 namespace orion {
 namespace {
 
-constexpr uint32_t kThreads = 256, kWarps = 8, kSlab = 128;
-constexpr uint32_t kWRow = kSlab / 2;  // bytes of a weight row in a slab
+constexpr uint32_t kThreads = 256, kWarps = 8;
 constexpr float kUnit = 8192.f;        // dequantised codes are multiples of 1 / kUnit
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool some) {
@@ -107,6 +106,7 @@ struct FewConfig {
   static constexpr uint32_t kMatrices = GATED ? 2 : 1;
   static constexpr uint32_t kOutputs = kTileRows / kMatrices;               // columns of y
   static constexpr uint32_t kTokens = 8 * NT;
+  static constexpr uint32_t kSlab = NT == 1 && sizeof(T) == 2 ? 256 : 128, kWRow = kSlab / 2;  // k of a slab, bytes of a weight row in it
   static constexpr uint32_t kXRow = kSlab * sizeof(T);
   static constexpr uint32_t kWStage = kTileRows * kWRow;
   static constexpr uint32_t kPerSlab = kSlab / GROUP;                       // groups in a slab
@@ -114,16 +114,16 @@ struct FewConfig {
   static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + (ZEROS ? kZeroRow : 0));
   static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows;         // floats of the sums that meet in shared memory
   // Slabs in the ring, and sets of sums: with few tokens two CTAs share an SM, with many one takes what there is.
-  static constexpr uint32_t kStages = sizeof(T) == 4 ? 3 : 4, kSets = NT <= 2 ? 2 : 1;
+  static constexpr uint32_t kStages = kSlab == 256 ? 2 : NT <= 2 || sizeof(T) == 4 ? 3 : 4, kSets = NT <= 2 ? 2 : 1;
   static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kSmem = kKGroups * kStages * kStage + kSets * kSums * 4;
 };
 
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, NT == 1 || (NT == 2 && sizeof(T) == 2) ? 2 : 1)
 w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, const uint32_t stored_tokens) {
   using Cfg = FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   constexpr bool kF32 = sizeof(T) == 4;
-  constexpr uint32_t kPerSlab = Cfg::kPerSlab, kStages = Cfg::kStages, kStageBytes = Cfg::kStage;
+  constexpr uint32_t kPerSlab = Cfg::kPerSlab, kStages = Cfg::kStages, kStageBytes = Cfg::kStage, kSlab = Cfg::kSlab, kWRow = Cfg::kWRow;
   extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
 
@@ -171,9 +171,8 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
           cp_async4(s_at + row * Cfg::kScaleRow + col * 2, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
         }
       }
-      if (!ZEROS) return;
 #pragma unroll
-      for (uint32_t j = 0; j < (kRowsOfParams * kZeroWords + WR * 32 - 1) / (WR * 32); ++j) {
+      for (uint32_t j = 0; ZEROS && j < (kRowsOfParams * kZeroWords + WR * 32 - 1) / (WR * 32); ++j) {
         const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords, col = i % kZeroWords * 4, group = slab * kPerSlab + row % kPerSlab;
         const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
         if (row < kRowsOfParams && !p) {
@@ -200,15 +199,18 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
 
   // What is loaded next: a slab of a tile. The loads run ahead of the products across tiles, so that the ring never drains.
   //
-  // Weight rows of 64 bytes, 16-byte pieces permuted by (row / 2) & 3 so that the eight rows of a fragment lie in different banks; a lane copies piece t of
-  // the rows g, g + 8, .. of its warp's tiles. Rows beyond the last are left as they are: nothing of them is stored. Token rows: every other one with its
+  // Weight rows of 64 or 128 bytes, their 16-byte pieces permuted so that the eight rows of a fragment lie in different banks; a lane copies one piece of
+  // every fourth or eighth row of its warp's tiles. Rows beyond the last are left as they are: nothing of them is stored. Token rows: every other one with its
   // halves of 64 bytes exchanged, zeros beyond the last k.
   constexpr uint32_t kPieces = Cfg::kXRow / 16, kPer = 16 / sizeof(T), kXTurns = (Cfg::kTokens * kPieces + WR * 32 - 1) / (WR * 32);
   constexpr uint32_t kXStep = WR * 32 / kPieces;  // token rows from one turn to the next, an even number
   static_assert(kXStep % 2 == 0, "rows of a lane's turns are permuted alike");
-  const uint32_t w_to = wr * RT * 16 * kWRow + g * kWRow + (t ^ ((g >> 1) & 3)) * 16;
+  constexpr uint32_t kWPieces = kSlab / 32, kWStep = 32 / kWPieces, kWTurns = kTilesPerMatrix * 16 / kWStep;  // rows from one turn to the next, turns per matrix
+  const uint32_t w_row = lane / kWPieces, w_piece = lane % kWPieces;
+  // a piece goes to the place at ^ (row & 7) of rows of 128 bytes, at ^ ((row / 2) & 3) of rows of 64; of the former every other turn has row & 4 set
+  const uint32_t w_to = wr * RT * 16 * kWRow + w_row * kWRow + (w_piece ^ (kWPieces == 8 ? w_row : (w_row >> 1) & 3)) * 16;
   const uint32_t x_row = in_kg / kPieces, x_piece = in_kg % kPieces, x_to = Cfg::kWStage + x_row * Cfg::kXRow + (x_piece ^ ((x_row & 1) << 2)) * 16;
-  const uint64_t eight_rows = (uint64_t)c.k * 4, x_step = kXStep * c.ldx * sizeof(T);  // bytes
+  const uint64_t w_step = (uint64_t)c.k / 2 * kWStep, x_step = kXStep * c.ldx * sizeof(T);  // bytes
   uint32_t load_tile = blockIdx.x, load_index = 0, load_slot = 0, load_n0 = 0, load_tokens = 0, load_rows = 0;
   const uint8_t *load_w[Cfg::kMatrices] = {}, *load_x = nullptr;
   auto load = [&] {
@@ -216,20 +218,20 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
     if (load_tile < tiles && mine > 0) {
       if (load_index == 0) {
         load_n0 = load_tile / tiles_m * Cfg::kOutputs;
-        const uint32_t m0 = load_tile % tiles_m * Cfg::kTokens, row = load_n0 + wr * kTilesPerMatrix * 16 + g;
+        const uint32_t m0 = load_tile % tiles_m * Cfg::kTokens, row = load_n0 + wr * kTilesPerMatrix * 16 + w_row;
         load_tokens = min(Cfg::kTokens, c.rows - m0);
-        load_rows = row < c.n ? (c.n - row + 7) / 8 : 0;  // of this lane's, per matrix
-        const uint64_t at = ((uint64_t)row * (c.k / 8) + unit * (kSlab / 8) + t * 4) * 4;
+        load_rows = row < c.n ? (c.n - row + kWStep - 1) / kWStep : 0;  // of this lane's, per matrix
+        const uint64_t at = ((uint64_t)row * (c.k / 8) + unit * (kSlab / 8) + w_piece * 4) * 4;
         load_w[0] = reinterpret_cast<const uint8_t *>(c.w.packed) + at;
         if (GATED) load_w[Cfg::kMatrices - 1] = reinterpret_cast<const uint8_t *>(c.up.packed) + at;
         load_x = static_cast<const uint8_t *>(c.x) + ((uint64_t)(m0 + x_row) * c.ldx + unit * kSlab + x_piece * kPer) * sizeof(T);
       }
       const uint32_t slab = unit + load_index * units, k0 = slab * kSlab, base = ring + load_slot * kStageBytes;
-      const uint32_t rows = k0 + t * 32 < c.k ? load_rows : 0;
+      const uint32_t rows = k0 + w_piece * 32 < c.k ? load_rows : 0;
 #pragma unroll
-      for (uint32_t i = 0; i < 2 * RT; ++i) {
-        const uint32_t m = i / (2 * kTilesPerMatrix), r = i % (2 * kTilesPerMatrix);
-        cp_async16_if(base + w_to + i * 8 * kWRow, load_w[m] + r * eight_rows, r < rows);
+      for (uint32_t i = 0; i < Cfg::kMatrices * kWTurns; ++i) {
+        const uint32_t m = i / kWTurns, r = i % kWTurns, to = base + (kWPieces == 8 && r % 2 ? w_to ^ 64 : w_to);
+        cp_async16_if(to + i * kWStep * kWRow, load_w[m] + r * w_step, r < rows);
       }
 #pragma unroll
       for (uint32_t m = 0; m < Cfg::kMatrices; ++m) load_w[m] += units * kWRow;
@@ -258,7 +260,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   // Offsets of this lane's words in a stage: piece q of its weight rows, and its 16 (bf16) or 32 bytes of the tokens' 32 k, the latter for even and odd q
   uint32_t w_from[kSlab / 32], x_from[2];
 #pragma unroll
-  for (uint32_t q = 0; q < kSlab / 32; ++q) w_from[q] = (wr * RT * 16 + g) * kWRow + (q ^ ((g >> 1) & 3)) * 16 + t * 4;
+  for (uint32_t q = 0; q < kSlab / 32; ++q) w_from[q] = (wr * RT * 16 + g) * kWRow + (q ^ (kWPieces == 8 ? g : (g >> 1) & 3)) * 16 + t * 4;
 #pragma unroll
   for (uint32_t q = 0; q < 2; ++q)
     x_from[q] = Cfg::kWStage + g * Cfg::kXRow + (kF32 ? (2 * t ^ ((g & 1) << 2)) * 16 : (q ^ (g & 1)) * 64 + t * 16);
@@ -415,7 +417,7 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
   const uint64_t tiles = (uint64_t)tiles_n * tiles_m;
   if (tiles > 0x7fffffffull) return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
   // k over a cluster of `ranks` CTAs: as many as make the rounds of tiles shortest, a tile's end counted as two slabs
-  const uint32_t resident = 148 * (NT == 1 && smem + 1024 <= 114 * 1024 ? 2 : 1), slabs = (c.k + kSlab - 1) / kSlab;
+  const uint32_t resident = 148 * (NT <= 2 && smem + 1024 <= 114 * 1024 ? 2 : 1), slabs = (c.k + Cfg::kSlab - 1) / Cfg::kSlab;
   uint32_t ranks = 1;
   uint64_t best = ~0ull;
   for (uint32_t r = 1; r <= 8; ++r) {

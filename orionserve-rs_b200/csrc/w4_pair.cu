@@ -1,0 +1,571 @@
+// Products with 4-bit weights for many rows of bf16 activations (w4.cuh has the layout): persistent CTA pairs on tcgen05, weights dequantised on their way
+// into shared memory.
+//
+// From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05. A pair of CTAs works as one MMA unit on 256 weight rows x
+// up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: eight warps of each CTA read the codes of its 128 rows straight
+// into registers, four stages of 128 k ahead, and write the operand tile into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
+//
+// The operands are f16, not bf16. (code - zero) * scale has at most 11 significant bits with a zero of 8 and 12 with any other, f16 holds 11: products are
+// exact, or off by 2^-12 of a weight, where bf16 would round every weight by 2^-9. Range is no matter, since both sides are scaled by powers of two, every
+// row of weights by the exponent of its largest scale and every token by that of its largest value (the same reason keeps every bf16 value exact in f16,
+// down to 2^-28 of the row's largest). A first kernel finds these exponents and converts the tokens; the epilogue scales back. Dequantisation costs a lane
+// 9 instructions for eight weights: the masked pairs, read as f16, are code * 2^-24 or code * 2^-20 (subnormal numbers and the first binade count in steps of
+// 2^-24), and one fused multiply-add each subtracts 8 and multiplies by the scale; zero points are subtracted first, which is exact.
+//
+// Where tiles are too few for 74 pairs, k is cut as well: the parts are stored in f32 and summed in order by a third kernel, so results do not vary.
+//
+// A CTA has 18 warps: 0 loads tokens (TMA), 1 of the leader issues the MMAs, 2-9 dequantise, 10-17 are the epilogue, which works under the next tile's main
+// loop. Every wait is bounded; one that runs out sets the projections' error word.
+#include "gemm_pair.cuh"
+#include "w4.cuh"
+
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+namespace orion {
+namespace {
+
+using Pair = PairConfig;
+constexpr uint32_t kDequantWarps = 8, kFirstDequant = 2, kFirstEpilogue = kFirstDequant + kDequantWarps, kWarps = kFirstEpilogue + Pair::kEpilogueWarps;
+constexpr uint32_t kAhead = 4;           // stages of codes in registers
+constexpr uint32_t kTileRows = 2 * Pair::kRows;
+constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to
+static_assert(Pair::kStageK == 128, "a stage is four pieces of 32 k");
+
+// What the first kernel leaves for the second, and the parts of k that the third one sums.
+struct Workspace {
+  __half *x = nullptr;        // [rows][k], scaled
+  float *x_unit = nullptr;    // [rows, rounded up to 32] what a token was divided by, but for 2^kTop
+  int32_t *w_exp = nullptr;   // [weight rows] exponent of the largest scale
+  float *parts = nullptr;     // [splits][rows][weight rows]
+};
+
+struct Plan {
+  uint32_t tokens = 256, splits = 1, tiles_w = 0, tiles_x = 0, stages = 0;
+};
+
+// Rounds of the 74 pairs times what a round takes, in cycles: a stage takes the tensor cores two cycles a token column and the dequantising warps some 420
+// cycles, a tile's end some 3000; parts of k are written and read again.
+Plan make_plan(uint32_t rows, uint32_t weight_rows, uint32_t k) {
+  Plan best;
+  double cost = 1e300;
+  const uint32_t stages = (k + Pair::kStageK - 1) / Pair::kStageK, tiles_w = (weight_rows + kTileRows - 1) / kTileRows;
+  const uint32_t most = std::min(256u, (rows + 31) / 32 * 32);
+  for (uint32_t tokens = most; tokens >= std::min(most, 128u); tokens -= 32) {
+    const uint32_t tiles_x = (rows + tokens - 1) / tokens;
+    for (uint32_t splits = 1; splits <= 8 && splits <= stages && (splits == 1 || (uint64_t)tiles_w * tiles_x <= 8 * kPairs); ++splits) {
+      const uint64_t jobs = (uint64_t)tiles_w * tiles_x * splits, rounds = (jobs + kPairs - 1) / kPairs;
+      double c = (double)rounds * ((stages + splits - 1) / splits * std::max(2.0 * tokens + 32.0, 420.0) + 3000.0);
+      if (splits > 1) c += 4000.0 + (double)splits * rows * weight_rows * 8.0 / 2500.0;
+      if (c < cost) cost = c, best = {tokens, splits, tiles_w, tiles_x, stages};
+    }
+  }
+  return best;
+}
+
+uint64_t place(uint64_t *at, uint64_t bytes) {
+  const uint64_t here = *at;
+  *at += (bytes + 255) / 256 * 256;
+  return here;
+}
+Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint32_t k, const Plan &plan, uint64_t *bytes) {
+  uint64_t at = 0;
+  Workspace w;
+  w.x = reinterpret_cast<__half *>(base + place(&at, (uint64_t)rows * k * 2));
+  w.x_unit = reinterpret_cast<float *>(base + place(&at, ((uint64_t)rows + 31) / 32 * 32 * 4));
+  w.w_exp = reinterpret_cast<int32_t *>(base + place(&at, (uint64_t)weight_rows * 4));
+  w.parts = reinterpret_cast<float *>(base + place(&at, plan.splits > 1 ? (uint64_t)plan.splits * rows * weight_rows * 4 : 0));
+  *bytes = at;
+  return w;
+}
+
+// ---- first kernel: tokens to f16, exponents of tokens and of weight rows ------------------------
+
+constexpr uint32_t kPrepThreads = 256, kHeld = 8;
+
+__global__ void __launch_bounds__(kPrepThreads)
+w4_prepare_kernel(const W4Call c, const Workspace ws, uint32_t matrices) {
+  pdl_wait();
+  pdl_trigger();  // after the wait: what the next kernel reads ahead of its own wait was complete before this one began
+  if (blockIdx.x >= c.rows) {
+    const uint32_t i = (blockIdx.x - c.rows) * kPrepThreads + threadIdx.x;
+    if (i >= c.n * matrices) return;
+    const uint32_t row = i % c.n, groups = c.k / c.group;
+    const uint16_t *s = reinterpret_cast<const uint16_t *>(i >= c.n ? c.up.scales : c.w.scales) + row;
+    uint32_t top = 0;
+#pragma unroll 8
+    for (uint32_t g = 0; g < groups; ++g) {
+      const uint32_t e = __ldg(s + (uint64_t)g * c.n) >> 7 & 255u;
+      top = max(top, e == 255u ? 0u : e);
+    }
+    ws.w_exp[i] = top ? (int32_t)top - 127 : 0;
+    return;
+  }
+  const uint32_t m = blockIdx.x, pieces = c.k / 8;
+  const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const bf16 *>(c.x) + (uint64_t)m * c.ldx);
+  uint4 held[kHeld];
+  uint32_t top = 0;  // the largest finite magnitude's bits
+  auto largest = [&](const uint4 &v) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = u[i] & 0x7fffu, hi = u[i] >> 16 & 0x7fffu;
+      top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+    }
+  };
+#pragma unroll
+  for (uint32_t j = 0; j < kHeld; ++j) {
+    const uint32_t i = threadIdx.x + j * kPrepThreads;
+    held[j] = i < pieces ? __ldg(x + i) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < kHeld; ++j) largest(held[j]);
+  for (uint32_t i = threadIdx.x + kHeld * kPrepThreads; i < pieces; i += kPrepThreads) largest(__ldg(x + i));
+  __shared__ uint32_t tops[kPrepThreads / 32];
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (uint32_t i = 0; i < kPrepThreads / 32; ++i) top = max(top, tops[i]);
+  const int e = top == 0 ? 0 : top >= 0x80u ? (int)(top >> 7) - 127 : 31 - __clz((int)top) - 133, up = kTop - e, half = up / 2;
+  // two factors: one alone would not be finite where the token's values are the smallest there are
+  const float f0 = __uint_as_float((uint32_t)(half + 127) << 23), f1 = __uint_as_float((uint32_t)(up - half + 127) << 23);
+  uint4 *out = reinterpret_cast<uint4 *>(ws.x + (uint64_t)m * c.k);
+  auto convert = [&](const uint4 &v) {
+    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(__uint_as_float(u[i] << 16) * f0 * f1, __uint_as_float(u[i] & 0xffff0000u) * f0 * f1);
+      r[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+  };
+#pragma unroll
+  for (uint32_t j = 0; j < kHeld; ++j) {
+    const uint32_t i = threadIdx.x + j * kPrepThreads;
+    if (i < pieces) out[i] = convert(held[j]);
+  }
+  for (uint32_t i = threadIdx.x + kHeld * kPrepThreads; i < pieces; i += kPrepThreads) out[i] = convert(__ldg(x + i));
+  if (threadIdx.x == 0) ws.x_unit[m] = ldexpf(1.f, e);
+}
+
+// ---- second kernel: the products ------------------------------------------------------------------
+
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// mbar_wait for barriers that threads of the other CTA arrive at
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const uint64_t start = global_timer_ns();
+  for (uint32_t i = 0; i < (1u << 30); ++i) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if ((i & 63u) == 63u && global_timer_ns() - start > 2000000000ull) return false;
+  }
+  return false;
+}
+__device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint4 load_codes(const uint32_t *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// f32 accumulation, f16 x f16
+__device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
+
+template <bool GATED, bool ZEROS>
+__global__ void __launch_bounds__(kWarps * 32, 1)
+w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const Workspace ws, const Plan plan, uint32_t *error) {
+  constexpr uint32_t kStages = Pair::kStages, kMatrices = GATED ? 2 : 1;
+  extern __shared__ uint8_t raw_smem[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t *w_ring = smem, *x_ring = smem + Pair::kXRingOffset;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Pair::kBarrierOffset);
+  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const bool leader = rank == 0;
+  const uint32_t total = plan.tiles_w * plan.tiles_x * plan.splits, weight_rows = kMatrices * c.n;
+
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < kStages; ++s) {
+      mbar_init(&full[s], 1 + 2 * kDequantWarps);  // the leader's announcement of the tokens' bytes, both CTAs' weights (used in the leader)
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, Pair::kTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive_release();  // the peer's barriers exist before anything of this CTA signals them
+  cluster_wait_acquire();
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tmem_base = *tmem_slot;
+  bool ok = true;
+  auto wait = [](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait_cluster(bar, parity)); };  // one answer for a warp
+
+  // A job: weight rows w_row .. + 255 against tokens x_row .. + cols - 1, stages kb .. end - 1 of k. Splits of a tile are neighbours: they share tokens and
+  // weights of L2.
+  struct Job {
+    uint32_t w_row, x_row, cols, kb, end, split;
+  };
+  auto job = [&](uint32_t id) {
+    const TileXy t = raster(id / plan.splits, plan.tiles_w, plan.tiles_x);
+    const uint32_t split = id % plan.splits, x_row = t.y * plan.tokens;
+    return Job{t.x * kTileRows, x_row, min(plan.tokens, (c.rows - x_row + 31) / 32 * 32), split * plan.stages / plan.splits, (split + 1) * plan.stages / plan.splits, split};
+  };
+
+  if (warp == 0) {
+    // Tokens: this CTA's half of a tile's; the bytes of both CTAs are counted on the leader's barrier. Nothing is there beyond the last token and k: zeros.
+    const bool elected = elect_one();
+    const uint32_t box = plan.tokens / 2;
+    uint32_t it = 0;
+    pdl_wait();
+    for (uint32_t t = pair; ok && t < total; t += pairs) {
+      const Job j = job(t);
+      for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
+        const uint32_t s = it % kStages;
+        if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
+        if (elected) {
+          const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
+          if (leader) mbar_arrive_expect_tx(&full[s], 2 * 2 * box * Pair::kSlabK * 2);
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h)
+            tma_load_2d_pair(x_ring + s * Pair::kXBytes + h * Pair::kXSlab, &map_x, (int)(kb * Pair::kStageK + h * Pair::kSlabK),
+                             (int)(j.x_row + rank * (j.cols / 2)), bar);
+        }
+        __syncwarp();
+      }
+    }
+    // the slots that are still being read: nobody signals a barrier of a CTA that is gone
+    for (uint32_t i = it > kStages ? it - kStages : 0; ok && i < it; ++i) ok = wait(&empty[i % kStages], (i / kStages) & 1);
+  } else if (warp == 1) {
+    if (leader) {  // issues for both CTAs
+      const uint64_t w_desc = desc_k_sw128(smem_u32(w_ring)), x_desc = desc_k_sw128(smem_u32(x_ring));
+      const bool elected = elect_one();
+      uint32_t it = 0, turn = 0;
+      for (uint32_t t = pair; ok && t < total; t += pairs, ++turn) {
+        const Job j = job(t);
+        const uint32_t id = idesc_f16(kTileRows, j.cols), buf = turn & 1, acc = tmem_base + buf * Pair::kMaxTokens;
+        if (!wait(&acc_empty[buf], ((turn >> 1) & 1) ^ 1)) { ok = false; break; }
+        tc_fence_after();
+        for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
+          const uint32_t s = it % kStages;
+          if (!wait(&full[s], (it / kStages) & 1)) { ok = false; break; }
+          tc_fence_after();
+          if (elected) {
+            const uint64_t a = w_desc + s * (Pair::kWBytes >> 4), b = x_desc + s * (Pair::kXBytes >> 4);
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+              for (uint32_t k = 0; k < Pair::kSlabK / 16; ++k)
+                umma_bf16_pair(acc, a + ((h * Pair::kWSlab + k * 32) >> 4), b + ((h * Pair::kXSlab + k * 32) >> 4), id, (kb > j.kb || h > 0 || k > 0) ? 1u : 0u);
+            umma_commit_both(&empty[s]);
+          }
+          __syncwarp();
+        }
+        if (ok && elected) umma_commit_both(&acc_full[buf]);
+      }
+    }
+  } else if (warp < kFirstEpilogue) {
+    // Weights: sixteen rows of the CTA's 128 a warp, as two sets of eight; a lane has 32 k (piece) of a row of each. With a gate every other row of a tile is
+    // the gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds both.
+    const uint32_t piece = lane & 3, in_tile = (warp - kFirstDequant) * 16 + (lane >> 2);
+    // chunks of 16 bytes are permuted by row & 7; lanes of the upper 64 k take theirs in another order, so that eight lanes meet eight different banks
+    const uint32_t turn_around = piece >= 2 ? 2 : 0;
+    const uint32_t to = smem_u32(w_ring) + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ turn_around ^ (in_tile & 7)) * 16;
+    struct Codes {
+      uint4 words[2];
+      uint32_t param[2];  // scale | zero << 16
+    };
+    Codes held[kAhead];
+    // What is read next
+    uint32_t load_t = pair, load_kb = 0, load_end = 0;
+    const uint32_t *from[2] = {};
+    const uint16_t *scale_from[2] = {};
+    const uint8_t *zero_from[2] = {};
+    bool there[2] = {};
+    auto aim = [&] {  // at the first stage of the next job
+      while (load_t < total) {
+        const Job j = job(load_t);
+        load_kb = j.kb, load_end = j.end;
+        if (load_kb < load_end) {
+#pragma unroll
+          for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t r = j.w_row + rank * Pair::kRows + in_tile + i * 8, row = GATED ? r >> 1 : r;
+            const W4View &w = GATED && (r & 1) ? c.up : c.w;
+            there[i] = row < c.n;
+            from[i] = w.packed + (uint64_t)(there[i] ? row : 0) * (c.k / 8) + piece * 4;
+            scale_from[i] = reinterpret_cast<const uint16_t *>(w.scales) + (there[i] ? row : 0);
+            zero_from[i] = w.zeros ? w.zeros + (there[i] ? row : 0) : nullptr;
+          }
+          return;
+        }
+        load_t += pairs;
+      }
+    };
+    auto load = [&](Codes &d) {
+      if (load_t >= total) return;
+      const uint32_t k = load_kb * Pair::kStageK + piece * 32;
+#pragma unroll
+      for (uint32_t i = 0; i < 2; ++i) {
+        d.words[i] = make_uint4(0, 0, 0, 0);
+        d.param[i] = 8u << 16;
+        if (there[i] && k < c.k) {
+          d.words[i] = load_codes(from[i] + load_kb * (Pair::kStageK / 8));
+          const uint64_t at = (uint64_t)(k / c.group) * c.n;
+          d.param[i] = __ldg(scale_from[i] + at) | (ZEROS && zero_from[i] ? (uint32_t)__ldg(zero_from[i] + at) << 16 : 8u << 16);
+        }
+      }
+      if (++load_kb == load_end) load_t += pairs, aim();
+    };
+    aim();
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) load(held[i]);
+    pdl_wait();
+
+    uint32_t it = 0, t = pair, kb = 0, end = 0;
+    int32_t raise[2] = {};  // what a row's scales are multiplied by, as an exponent
+    bool more = false;
+    auto next_job = [&] {
+      more = false;
+      for (; t < total; t += pairs) {
+        const Job j = job(t);
+        if (j.kb >= j.end) continue;
+        kb = j.kb, end = j.end, more = true;
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+          const uint32_t r = j.w_row + rank * Pair::kRows + in_tile + i * 8, row = GATED ? r >> 1 : r;
+          raise[i] = row < c.n ? kTop - ws.w_exp[(GATED && (r & 1) ? c.n : 0) + row] : 0;
+        }
+        break;
+      }
+    };
+    next_job();
+    while (ok && more) {
+#pragma unroll
+      for (uint32_t u = 0; u < kAhead; ++u) {
+        if (!ok || !more) break;
+        const uint32_t s = it % kStages;
+        if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+          const uint32_t p = held[u].param[i], e = p >> 7 & 255u;
+          const int32_t raised = (int32_t)e + raise[i];
+          // infinities and NaN stay, what is far below the row's largest scale vanishes
+          const uint32_t f = e == 255u ? p << 16 : raised <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise[i] << 23);
+          const __half h = __float2half_rn(__uint_as_float(f));
+          const uint32_t low = (uint32_t)__half_as_ushort(h) * 0x10001u, high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
+          const uint32_t eight = hmul2(low, 0x80088008u);                                                // -8 * 2^-24 * scale
+          const uint32_t zero = (p >> 16) * 0x10001u, zero_high = zero << 4;
+          uint32_t w[4] = {held[u].words[i].x, held[u].words[i].y, held[u].words[i].z, held[u].words[i].w};
+          if (turn_around) {
+            const uint32_t a = w[0], b = w[1];
+            w[0] = w[2], w[1] = w[3], w[2] = a, w[3] = b;
+          }
+#pragma unroll
+          for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t rest = w[j] >> 8;
+            uint32_t v[4] = {w[j] & 0x000f000fu, w[j] & 0x00f000f0u, rest & 0x000f000fu, rest & 0x00f000f0u};
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+              if (ZEROS) v[q] = hmul2(hsub2(v[q], q & 1 ? zero_high : zero), q & 1 ? high : low);
+              else v[q] = hfma2(v[q], q & 1 ? high : low, eight);
+            }
+            sts128(to + s * Pair::kWBytes + i * 8 * 128 + (chunk ^ (j * 16)), v[0], v[1], v[2], v[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&full[s]), 0));
+        load(held[u]);
+        ++it;
+        if (++kb == end) t += pairs, next_job();
+      }
+    }
+  } else {
+    // Epilogue: warp w reads tensor-memory lanes 32 * (w % 4) .. + 31 (lane = weight row, column = token); the two warps of the same lanes take turns, 16
+    // columns each.
+    pdl_wait();
+    uint32_t turn = 0;
+    for (uint32_t t = pair; ok && t < total; t += pairs, ++turn) {
+      const Job j = job(t);
+      const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * Pair::kMaxTokens;
+      const uint32_t r = j.w_row + rank * Pair::kRows + (warp & 3) * 32 + lane, row = GATED ? r >> 1 : r;
+      const bool inside = row < c.n;
+      // 2^exponent, and 2^-4 left of the powers that scales (2^14), codes (2^-24) and tokens (2^14) were brought to
+      const float unit = inside ? __uint_as_float((uint32_t)(ws.w_exp[(GATED && (r & 1) ? c.n : 0) + row] + 127) << 23) : 0.f;
+      const float bias = !GATED && inside && c.bias && plan.splits == 1 ? c.bias[row] : 0.f;
+      if (!wait(&acc_full[buf], (turn >> 1) & 1)) { ok = false; break; }
+      tc_fence_after();
+      constexpr uint32_t kStep = 16 * (Pair::kEpilogueWarps / 4);
+      uint32_t mb = 16 * ((warp - kFirstEpilogue) / 4);
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[buf]), 0));
+      };
+      if (mb >= j.cols) release();
+#pragma unroll 1
+      for (; mb < j.cols; mb += kStep) {
+        uint32_t rr[16];
+        tmem_ld16(acc + mb, rr);
+        tmem_ld_wait();
+        if (mb + kStep >= j.cols) release();
+        const uint32_t token = j.x_row + mb;
+        float v[16];
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q) {
+          const float4 f = *reinterpret_cast<const float4 *>(ws.x_unit + token + 4 * q);
+          v[4 * q] = __uint_as_float(rr[4 * q]) * 0.0625f * unit * f.x, v[4 * q + 1] = __uint_as_float(rr[4 * q + 1]) * 0.0625f * unit * f.y;
+          v[4 * q + 2] = __uint_as_float(rr[4 * q + 2]) * 0.0625f * unit * f.z, v[4 * q + 3] = __uint_as_float(rr[4 * q + 3]) * 0.0625f * unit * f.w;
+        }
+        if (plan.splits > 1) {
+          float *p = ws.parts + ((uint64_t)j.split * c.rows + token) * weight_rows + r;
+#pragma unroll
+          for (uint32_t q = 0; q < 16; ++q)
+            if (inside && token + q < c.rows) p[(uint64_t)q * weight_rows] = v[q];
+        } else if (GATED) {
+          const bool odd = lane & 1;
+          bf16 *p = static_cast<bf16 *>(c.out) + (uint64_t)(token + (odd ? 8 : 0)) * c.ldo + row;
+#pragma unroll
+          for (uint32_t q = 0; q < 8; ++q) {
+            const float other = __shfl_xor_sync(0xffffffffu, odd ? v[q] : v[8 + q], 1);
+            const float y = gated<bf16>(GatedAct{c.act, 0.f}, odd ? other : v[q], odd ? v[8 + q] : other);
+            if (inside && token + (odd ? 8 : 0) + q < c.rows) p[q * c.ldo] = __float2bfloat16_rn(y);
+          }
+        } else {
+          bf16 *p = static_cast<bf16 *>(c.out) + (uint64_t)token * c.ldo + row;
+#pragma unroll
+          for (uint32_t q = 0; q < 16; ++q)
+            if (inside && token + q < c.rows) p[q * c.ldo] = __float2bfloat16_rn(v[q] + bias);
+        }
+      }
+    }
+  }
+  if (!ok) atomicOr(error, 1u);
+  tc_fence_before();
+  __syncthreads();
+  // Neither CTA leaves, nor frees the tensor memory the pair allocated together, while the other may still be read by an MMA or be reading its accumulator.
+  cluster_arrive_release();
+  cluster_wait_acquire();
+  if (warp == 1) tmem_dealloc_pair(tmem_base, Pair::kTmemCols);
+}
+
+// ---- third kernel: the parts of k, in order --------------------------------------------------------
+
+template <bool GATED>
+__global__ void __launch_bounds__(256) w4_sum_kernel(const W4Call c, const float *__restrict__ parts, uint32_t splits, uint32_t blocks_n) {
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t m = blockIdx.x / blocks_n, n = blockIdx.x % blocks_n * 256 + threadIdx.x;
+  if (n >= c.n) return;
+  constexpr uint32_t kMatrices = GATED ? 2 : 1;
+  const uint64_t slab = (uint64_t)c.rows * kMatrices * c.n;
+  const float *p = parts + ((uint64_t)m * c.n + n) * kMatrices;
+  float y;
+  if constexpr (GATED) {
+    float g = 0.f, u = 0.f;
+    for (uint32_t s = 0; s < splits; ++s) {
+      const float2 v = *reinterpret_cast<const float2 *>(p + s * slab);
+      g += v.x, u += v.y;
+    }
+    y = gated<bf16>(GatedAct{c.act, 0.f}, g, u);
+  } else {
+    y = 0.f;
+    for (uint32_t s = 0; s < splits; ++s) y += p[s * slab];
+    if (c.bias) y += c.bias[n];
+  }
+  static_cast<bf16 *>(c.out)[(uint64_t)m * c.ldo + n] = __float2bfloat16_rn(y);
+}
+
+int token_map(CUtensorMap *map, const __half *x, uint32_t rows, uint32_t k, uint32_t box_rows) {
+  EncodeFn fn = encode_fn();
+  if (!fn) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: driver entry point missing");
+  const cuuint64_t dims[2] = {k, rows}, strides[1] = {(cuuint64_t)k * 2};
+  const cuuint32_t box[2] = {Pair::kSlabK, box_rows}, one[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half *>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: encode returned %d (rows %u k %u)", (int)r, rows, k);
+  return ORION_OK;
+}
+
+template <bool GATED, bool ZEROS>
+int launch_pair(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
+  static bool done[kMaxDeviceOrdinals] = {};
+  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_pair_kernel<GATED, ZEROS>, Pair::kSmemBytes, done));
+  CUtensorMap map;
+  ORION_TRY(token_map(&map, ws.x, c.rows, c.k, plan.tokens / 2));
+  const uint32_t matrices = GATED ? 2 : 1, jobs = plan.tiles_w * plan.tiles_x * plan.splits;
+  const uint32_t blocks = c.rows + (c.n * matrices + kPrepThreads - 1) / kPrepThreads;
+  ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices));
+  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_pair_kernel<GATED, ZEROS>, dim3(2 * std::min(jobs, kPairs)), dim3(kWarps * 32), dim3(2, 1, 1),
+                                                       Pair::kSmemBytes, stream, c, map, ws, plan, error));
+  count_launch();
+  count_launch();
+  if (plan.splits > 1) {
+    ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_sum_kernel<GATED>, dim3((c.n + 255) / 256 * c.rows), dim3(256), 0, stream, c, (const float *)ws.parts, plan.splits,
+                                                 (c.n + 255) / 256));
+    count_launch();
+  }
+  return ORION_OK;
+}
+
+}  // namespace
+
+uint64_t w4_pair_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k) {
+  uint64_t bytes = 0;
+  workspace_at(nullptr, rows, weight_rows, k, make_plan(rows, weight_rows, k), &bytes);
+  return bytes;
+}
+
+int launch_w4_pair(const W4Call &c, void *workspace, uint32_t *error, cudaStream_t stream) {
+  const uint32_t weight_rows = c.up.packed ? 2 * c.n : c.n;
+  const Plan plan = make_plan(c.rows, weight_rows, c.k);
+  if ((uint64_t)plan.tiles_w * plan.tiles_x * plan.splits > 0x7fffffffull || c.rows > 0x3fffffffu)
+    return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
+  uint64_t bytes = 0;
+  const Workspace ws = workspace_at(static_cast<uint8_t *>(workspace), c.rows, weight_rows, c.k, plan, &bytes);
+  const bool zeros = c.w.zeros || c.up.zeros;
+  if (c.up.packed) return zeros ? launch_pair<true, true>(c, ws, plan, error, stream) : launch_pair<true, false>(c, ws, plan, error, stream);
+  return zeros ? launch_pair<false, true>(c, ws, plan, error, stream) : launch_pair<false, false>(c, ws, plan, error, stream);
+}
+
+}  // namespace orion

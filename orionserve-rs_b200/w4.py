@@ -3,7 +3,7 @@
 ``W[n][k] = (code - zero) * scale`` with a bf16 scale, and in the asymmetric form a zero point, per group of 32, 64 or 128 consecutive ``k`` of a row.
 Codes are packed eight to an int32: of eight consecutive ``k``, number ``2i`` is in bits ``4i .. 4i + 3``, number ``2i + 1`` in bits ``16 + 4i ..
 19 + 4i``. The functions stand beside ``ops.linear`` and ``ops.swiglu`` for tensors that are on the device already: they run on torch's current
-stream of the tensors' device, allocate only what they return, and can be captured into a CUDA graph. Activations are f32 or bf16. Nothing here
+stream of the tensors' device, allocate what they return and, for many rows, a workspace, and can be captured into a CUDA graph. Activations are f32 or bf16. Nothing here
 has a gradient; tensors that require one are refused.
 """
 from __future__ import annotations
@@ -128,6 +128,18 @@ def _raw_stream():
     return getattr(_torch._C, "_cuda_getCurrentRawStream", _stream)
 
 
+def _workspace(x, dtype, rows, weight, gated):
+    """(tensor or None, address, bytes) of what a call needs beside its arguments, from torch's allocator: its own until later work of the stream."""
+    if rows == 0 or dtype == 0:
+        return None, None, 0
+    need = C.c_uint64()
+    check(_ffi.lib().orion_cuda_w4_workspace(dtype, rows, weight._address, gated, C.byref(need)))
+    if need.value == 0:
+        return None, None, 0
+    t = x.new_empty(need.value, dtype=_torch.uint8)
+    return t, t.data_ptr(), need.value
+
+
 def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
     """``x W^T + bias`` (tensor.rs:96-130) over ``x`` ``[rows, in]``, f32 or bf16; ``bias`` f32 ``[out]``. Sums are f32, rounded once to the type of
     ``x``. Rows may be apart (any stride that keeps them on 16-byte boundaries); ``out``, if given, is written and returned."""
@@ -140,8 +152,9 @@ def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
         if bias.get_device() != backend._ordinal:
             raise InvalidRequest(f"bias must be on the backend's device {backend._ordinal}")
     out, out_stride = _output(x, out, rows, n)
+    space, at, size = _workspace(x, dtype, rows, weight, 0)
     check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, weight._address, None if bias is None else bias.data_ptr(), out.data_ptr(),
-                  out_stride, _stream(backend._ordinal)))
+                  out_stride, at, size, _stream(backend._ordinal)))
     return out
 
 
@@ -157,7 +170,8 @@ def gated_w4(backend: CudaBackend, x, gate: W4Weight, up: W4Weight, activation: 
     if up.device_index != backend._ordinal:
         raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
     out, out_stride = _output(x, out, rows, gate.out_features)
-    check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride,
+    space, at, size = _workspace(x, dtype, rows, gate, 1)
+    check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride, at, size,
                  _stream(backend._ordinal)))
     return out
 

@@ -35,6 +35,10 @@ class Weight:
                                    None if self.zeros is None else torch.tensor(self.zeros, dtype=torch.uint8).cuda(), group)
 
 
+    def step(self, rows, dtype):
+        return plain.weight_step(rows, dtype, self.zeros)
+
+
 def host(t):
     torch.cuda.synchronize()
     return t.double().cpu().numpy()
@@ -53,7 +57,7 @@ def test_linear(pkg, backend, rows, dtype):
         x = values(rng, (rows, k), dtype)
         bias = values(rng, n, "f32") if i % 3 else None
         got = pkg.linear_w4(backend, device(x, dtype), w.handle, bias=None if bias is None else device(bias, "f32"))
-        want, bound = plain.product(x, w.w)
+        want, bound = plain.product(x, w.w, w.step(rows, dtype))
         if bias is not None:
             want, bound = want + bias, bound + 2.0 ** -23 * (np.abs(want) + np.abs(bias))
         assert got.dtype == DTYPES[dtype]
@@ -69,7 +73,7 @@ def test_gated(pkg, backend, rows, dtype, act):
         gate, up = (Weight(pkg, rng, n, k, group, zeros=(rows + i + j) % 2 == 0) for j in range(2))
         x = values(rng, (rows, k), dtype, 0.5)
         got = pkg.gated_w4(backend, device(x, dtype), gate.handle, up.handle, activation=act)
-        plain.check(host(got), *plain.gated(act, x, gate.w, up.w), dtype, f"{rows} x {k} to {n}, groups of {group}")
+        plain.check(host(got), *plain.gated(act, x, gate.w, up.w, gate.step(rows, dtype), up.step(rows, dtype)), dtype, f"{rows} x {k} to {n}, groups of {group}")
 
 
 @pytest.mark.parametrize("with_zeros", [False, True])
@@ -159,7 +163,7 @@ def test_rows_of_any_magnitude(pkg, backend, rows, scale):
     x[0] = plain.to_bf16(x[0] * scale)
     x[1, 17] = plain.to_bf16(np.float64(1e5))
     x[2] = 0.0
-    want, bound = plain.product(x, w.w)
+    want, bound = plain.product(x, w.w, w.step(rows, "bf16"))
     plain.check(host(pkg.linear_w4(backend, device(x, "bf16"), w.handle)), want, bound, "bf16")
 
 
@@ -174,7 +178,7 @@ def test_outputs_of_any_magnitude(pkg, backend, rows):
     w.scales[2, 4] *= 2.0 ** -20
     handle = pkg.W4Weight(w.handle.packed, device(w.scales, "bf16"), w.handle.zeros, 128)
     x = values(rng, (rows, 512), "bf16")
-    want, bound = plain.product(x, plain.dequantize(w.codes, w.scales, w.zeros, 128))
+    want, bound = plain.product(x, plain.dequantize(w.codes, w.scales, w.zeros, 128), w.step(rows, "bf16"))
     plain.check(host(pkg.linear_w4(backend, device(x, "bf16"), handle)), want, bound, "bf16")
 
 
@@ -189,7 +193,7 @@ def test_strided_rows_and_neighbours_of_the_output(pkg, backend, rows, dtype):
     out = torch.full((rows + 2, 99), -7.0, dtype=DTYPES[dtype], device="cuda")
     got = pkg.linear_w4(backend, wide[:, 16:336], w.handle, out=out[1:rows + 1, 11:88])
     assert got.data_ptr() == out[1:, 11:].data_ptr()
-    plain.check(host(got), *plain.product(x, w.w), dtype)
+    plain.check(host(got), *plain.product(x, w.w, w.step(rows, dtype)), dtype)
     rest = host(out)
     rest[1:rows + 1, 11:88] = -7.0
     assert (rest == -7.0).all()
@@ -239,10 +243,11 @@ def test_feed_forward_of_quantized_weights(pkg, backend, rows):
     wide = [plain.dequantize(*plain.quantize(r, 64, True)[:2], plain.quantize(r, 64, True)[2], 64) for r in raw]
     x = values(rng, (rows, 256), "bf16")
     h = pkg.gated_w4(backend, device(x, "bf16"), w[0], w[1])
-    want, bound = plain.gated("silu", x, wide[0], wide[1])
+    step = plain.weight_step(rows, "bf16", True)
+    want, bound = plain.gated("silu", x, wide[0], wide[1], step, step)
     plain.check(host(h), want, bound, "bf16")
     y = pkg.linear_w4(backend, h, w[2])
-    plain.check(host(y), *plain.product(host(h), wide[2]), "bf16")
+    plain.check(host(y), *plain.product(host(h), wide[2], step), "bf16")
 
 
 @pytest.mark.parametrize("rows", [1, 40, 260])

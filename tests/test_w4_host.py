@@ -15,14 +15,14 @@ def weight(pkg, **over):
     return pkg._ffi.OrionW4Weight(f["packed"], f["scales"], f["zeros"], f["out_features"], f["in_features"], f["group"])
 
 
-def linear(pkg, w=None, dtype=2, x=P, rows=4, stride=128, bias=0, out=P, out_stride=64):
+def linear(pkg, w=None, dtype=2, x=P, rows=4, stride=128, bias=0, out=P, out_stride=64, space=0, size=0):
     w = weight(pkg) if w is None else w
-    return pkg._ffi.lib().orion_cuda_w4_linear(0, dtype, x, rows, stride, C.addressof(w) if w else None, bias, out, out_stride, None)
+    return pkg._ffi.lib().orion_cuda_w4_linear(0, dtype, x, rows, stride, C.addressof(w) if w else None, bias, out, out_stride, space, size, None)
 
 
-def gated(pkg, gate=None, up=None, dtype=2, act=0, x=P, rows=4, stride=128, out=P, out_stride=64):
+def gated(pkg, gate=None, up=None, dtype=2, act=0, x=P, rows=4, stride=128, out=P, out_stride=64, space=0, size=0):
     gate, up = gate or weight(pkg), up or weight(pkg)
-    return pkg._ffi.lib().orion_cuda_w4_gated(0, dtype, x, rows, stride, C.addressof(gate), C.addressof(up), act, out, out_stride, None)
+    return pkg._ffi.lib().orion_cuda_w4_gated(0, dtype, x, rows, stride, C.addressof(gate), C.addressof(up), act, out, out_stride, space, size, None)
 
 
 def quantize(pkg, dtype=2, w=P, n=64, k=128, stride=128, group=32, packed=P, scales=P, zeros=0):
@@ -52,7 +52,7 @@ def test_rows_that_are_refused(pkg, over):
 
 def test_other_refusals(pkg):
     bad = pkg._ffi.ERR_INVALID_REQUEST
-    assert pkg._ffi.lib().orion_cuda_w4_linear(0, 2, P, 4, 128, None, None, P, 64, None) == bad
+    assert pkg._ffi.lib().orion_cuda_w4_linear(0, 2, P, 4, 128, None, None, P, 64, None, 0, None) == bad
     assert linear(pkg, bias=P + 2) == bad
     assert gated(pkg, act=2) == bad and gated(pkg, act=-1) == bad
     for over in (dict(out_features=65), dict(in_features=160), dict(group=64)):
@@ -60,6 +60,26 @@ def test_other_refusals(pkg):
     for over in (dict(dtype=1), dict(w=0), dict(w=P + 4), dict(n=0), dict(n=1 << 31), dict(k=0), dict(k=100), dict(stride=96), dict(stride=129), dict(group=8),
                  dict(packed=0), dict(packed=P + 4), dict(scales=0), dict(scales=P + 2), dict(zeros=P + 1), dict(n=1 << 30, k=1 << 20, stride=1 << 20)):
         assert quantize(pkg, **over) == bad, over
+
+
+@pytest.mark.parametrize("is_gated", [0, 1])
+def test_workspaces(pkg, is_gated):
+    """What a call for many rows needs, and that it is refused with less; few rows and f32 need nothing."""
+    lib, bad, w, need = pkg._ffi.lib(), pkg._ffi.ERR_INVALID_REQUEST, weight(pkg), C.c_uint64(5)
+    for dtype, rows in ((0, 1), (0, 5000), (2, 1), (2, 8), (2, 0)):
+        assert lib.orion_cuda_w4_workspace(dtype, rows, C.addressof(w), is_gated, C.byref(need)) == pkg._ffi.ORION_OK and need.value == 0
+    last = 0
+    for rows in (200, 1000, 5000, 70000):
+        assert lib.orion_cuda_w4_workspace(2, rows, C.addressof(w), is_gated, C.byref(need)) == pkg._ffi.ORION_OK
+        assert need.value >= rows * 128 * 2 and need.value > last
+        last, call = need.value, gated if is_gated else linear
+        for space, size in ((0, 0), (0, last), (P, last - 1), (P + 128, last)):
+            assert call(pkg, rows=rows, space=space, size=size) == bad
+    assert lib.orion_cuda_w4_workspace(1, 8, C.addressof(w), 0, C.byref(need)) == bad
+    assert lib.orion_cuda_w4_workspace(2, 1 << 31, C.addressof(w), 0, C.byref(need)) == bad
+    assert lib.orion_cuda_w4_workspace(2, 8, None, 0, C.byref(need)) == bad
+    assert lib.orion_cuda_w4_workspace(2, 8, C.addressof(w), 0, None) == bad
+    assert lib.orion_cuda_w4_workspace(2, 8, C.addressof(weight(pkg, group=5)), 0, C.byref(need)) == bad
 
 
 def test_no_rows_need_no_device(pkg):

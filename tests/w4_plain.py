@@ -54,10 +54,18 @@ def quantize(w, group, with_zeros):
     return codes.reshape(n, k).astype(np.int64), scale.T, zero.T if with_zeros else None
 
 
-def product(x, w):
-    """(x w^T, bound of the error of its f32 sum): k additions, each off by at most a unit in the last place of the sum of magnitudes."""
+def weight_step(rows, dtype, zeros):
+    """How far, relative to its size, a weight may be rounded. The kernels for many rows of bf16 hold (code - zero) * scale in f16. A code less 8 is at most 8 in
+    size: three bits, or one, times the eight of a bf16 scale are at most 11, which f16 holds. A code less any other zero is at most 15: four bits times eight
+    are at most 12, and rounding to 11 is off by at most half a step, 2^-12. Everywhere else codes and scales are not multiplied before the sum."""
+    return 2.0 ** -12 if rows > 16 and dtype == "bf16" and zeros is not None else 0.0
+
+
+def product(x, w, step=0.0):
+    """(x w^T, bound of the error of its f32 sum): k additions, each off by at most a unit in the last place of the sum of magnitudes, of weights that are off
+    by `step`."""
     with np.errstate(invalid="ignore", over="ignore"):
-        return x @ w.T, (w.shape[1] + 8) * 2.0 ** -23 * (np.abs(x) @ np.abs(w.T))
+        return x @ w.T, ((w.shape[1] + 8) * 2.0 ** -23 + step) * (np.abs(x) @ np.abs(w.T))
 
 
 def activate(name, g):
@@ -69,8 +77,8 @@ def activate(name, g):
     return f, (8.0 + 6.0 * np.abs(a)) * 2.0 ** -23
 
 
-def gated(name, x, wg, wu):
-    (g, dg), (u, du) = product(x, wg), product(x, wu)
+def gated(name, x, wg, wu, gate_step=0.0, up_step=0.0):
+    (g, dg), (u, du) = product(x, wg, gate_step), product(x, wu, up_step)
     f, rel = activate(name, g)
     df = 1.13 * dg + rel * np.abs(f)  # neither function is steeper than 1.13
     return f * u, df * np.abs(u) + np.abs(f) * du + df * du + 2.0 ** -23 * np.abs(f * u)
