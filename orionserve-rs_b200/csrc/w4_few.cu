@@ -147,15 +147,15 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   constexpr uint32_t kScaleWords = Cfg::kOutputs / 2, kZeroWords = Cfg::kOutputs / 4, kRowsOfParams = Cfg::kMatrices * kPerSlab;
   constexpr uint32_t kParamTurns = (kRowsOfParams * Cfg::kOutputs + WR * 32 - 1) / (WR * 32);
   const bool words = (c.n & 3) == 0;
-  uint32_t held[kParamTurns], held_at = 0;  // scale | zero << 16, and where they go
+  uint32_t held_s[kParamTurns], held_z[kParamTurns], held_at = 0;  // as loaded, and where they go
   auto store_held = [&] {
     if (words || !held_at) return;
 #pragma unroll
     for (uint32_t j = 0; j < kParamTurns; ++j) {
       const uint32_t i = in_kg + j * WR * 32, row = i / Cfg::kOutputs, col = i % Cfg::kOutputs;
       if (row < kRowsOfParams) {
-        sts16(held_at + row * Cfg::kScaleRow + col * 2, held[j] & 0xffffu);
-        if (ZEROS) sts8(held_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, held[j] >> 16);
+        sts16(held_at + row * Cfg::kScaleRow + col * 2, held_s[j]);
+        if (ZEROS) sts8(held_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, held_z[j]);
       }
     }
     held_at = 0;
@@ -187,11 +187,12 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
 #pragma unroll
       for (uint32_t j = 0; j < kParamTurns; ++j) {
         const uint32_t i = in_kg + j * WR * 32, row = i / Cfg::kOutputs, col = i % Cfg::kOutputs, group = slab * kPerSlab + row % kPerSlab;
-        held[j] = 0;
+        held_s[j] = 0, held_z[j] = 8;
         if (row < kRowsOfParams && group < groups && n0 + col < c.n) {
           const W4View &w = row >= kPerSlab ? c.up : c.w;
           const uint64_t at = (uint64_t)group * c.n + n0 + col;
-          held[j] = __ldg(reinterpret_cast<const uint16_t *>(w.scales) + at) | (!ZEROS ? 0 : w.zeros ? (uint32_t)__ldg(w.zeros + at) << 16 : 8u << 16);
+          held_s[j] = __ldg(reinterpret_cast<const uint16_t *>(w.scales) + at);
+          if (ZEROS && w.zeros) held_z[j] = __ldg(w.zeros + at);
         }
       }
     }

@@ -313,7 +313,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     const uint32_t to = smem_u32(w_ring) + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ turn_around ^ (in_tile & 7)) * 16;
     struct Codes {
       uint4 words[2];
-      uint32_t param[2];  // scale | zero << 16
+      uint32_t scale[2], zero[2];  // as loaded: anything done to them here would wait for them
     };
     Codes held[kAhead];
     // What is read next
@@ -347,11 +347,12 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
 #pragma unroll
       for (uint32_t i = 0; i < 2; ++i) {
         d.words[i] = make_uint4(0, 0, 0, 0);
-        d.param[i] = 8u << 16;
+        d.scale[i] = 0, d.zero[i] = 8;
         if (there[i] && k < c.k) {
           d.words[i] = load_codes(from[i] + load_kb * (Pair::kStageK / 8));
           const uint64_t at = (uint64_t)(k / c.group) * c.n;
-          d.param[i] = __ldg(scale_from[i] + at) | (ZEROS && zero_from[i] ? (uint32_t)__ldg(zero_from[i] + at) << 16 : 8u << 16);
+          d.scale[i] = __ldg(scale_from[i] + at);
+          if (ZEROS && zero_from[i]) d.zero[i] = __ldg(zero_from[i] + at);
         }
       }
       if (++load_kb == load_end) load_t += pairs, aim();
@@ -387,14 +388,14 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) {
-          const uint32_t p = held[u].param[i], e = p >> 7 & 255u;
+          const uint32_t p = held[u].scale[i], e = p >> 7 & 255u;
           const int32_t raised = (int32_t)e + raise[i];
           // infinities and NaN stay, what is far below the row's largest scale vanishes
           const uint32_t f = e == 255u ? p << 16 : raised <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise[i] << 23);
           const __half h = __float2half_rn(__uint_as_float(f));
           const uint32_t low = (uint32_t)__half_as_ushort(h) * 0x10001u, high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
           const uint32_t eight = hmul2(low, 0x80088008u);                                                // -8 * 2^-24 * scale
-          const uint32_t zero = (p >> 16) * 0x10001u, zero_high = zero << 4;
+          const uint32_t zero = held[u].zero[i] * 0x10001u, zero_high = zero << 4;
           uint32_t w[4] = {held[u].words[i].x, held[u].words[i].y, held[u].words[i].z, held[u].words[i].w};
           if (turn_around) {
             const uint32_t a = w[0], b = w[1];
