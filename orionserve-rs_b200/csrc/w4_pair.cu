@@ -218,7 +218,8 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1 + 2 * kDequantWarps);  // the leader's announcement of the tokens' bytes, both CTAs' weights (used in the leader)
+      // leader: the announcement of the tokens' bytes, its own weights, word of the peer's; peer: its weights
+      mbar_init(&full[s], leader ? 2 + kDequantWarps : kDequantWarps);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -303,6 +304,19 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         }
         if (ok && elected) umma_commit_both(&acc_full[buf]);
       }
+    } else {
+      // Hands word of this CTA's weights on to the leader. Were every dequantising warp to arrive there by itself, each would wait at every stage until its
+      // stores are visible to the cluster.
+      uint32_t it = 0;
+      for (uint32_t t = pair; ok && t < total; t += pairs) {
+        const Job j = job(t);
+        for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
+          if (!wait(&full[it % kStages], (it / kStages) & 1)) { ok = false; break; }
+          fence_proxy_async_all();
+          if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&full[it % kStages]), 0));
+          __syncwarp();
+        }
+      }
     }
   } else if (warp < kFirstEpilogue) {
     // Weights: sixteen rows of the CTA's 128 a warp, as two sets of eight; a lane has 32 k (piece) of a row of each. With a gate every other row of a tile is
@@ -316,6 +330,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       uint32_t scale[2], zero[2];  // as loaded: anything done to them here would wait for them
     };
     Codes held[kAhead];
+    const uint32_t group_bits = 31 - __clz((int)c.group);
     // What is read next
     uint32_t load_t = pair, load_kb = 0, load_end = 0;
     const uint32_t *from[2] = {};
@@ -350,7 +365,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         d.scale[i] = 0, d.zero[i] = 8;
         if (there[i] && k < c.k) {
           d.words[i] = load_codes(from[i] + load_kb * (Pair::kStageK / 8));
-          const uint64_t at = (uint64_t)(k / c.group) * c.n;
+          const uint64_t at = (uint64_t)(k >> group_bits) * c.n;
           d.scale[i] = __ldg(scale_from[i] + at);
           if (ZEROS && zero_from[i]) d.zero[i] = __ldg(zero_from[i] + at);
         }
@@ -415,7 +430,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&full[s]), 0));
+        if (lane == 0) mbar_arrive(&full[s]);
         load(held[u]);
         ++it;
         if (++kb == end) t += pairs, next_job();
