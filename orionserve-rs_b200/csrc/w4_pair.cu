@@ -2,8 +2,8 @@
 // into shared memory.
 //
 // From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05. A pair of CTAs works as one MMA unit on 256 weight rows x
-// up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: eight warps of each CTA read the codes of its 128 rows straight
-// into registers, four stages of 128 k ahead, and write the operand tile into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
+// up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: a ring of codes is filled by TMA, four stages of 128
+// k ahead, and eight warps of each CTA write the operand tiles of its 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
 //
 // The operands are f16, not bf16. (code - zero) * scale has at most 11 significant bits with a zero of 8 and 12 with any other, f16 holds 11: products are
 // exact, or off by 2^-12 of a weight, where bf16 would round every weight by 2^-9. Range is no matter, since both sides are scaled by powers of two, every
@@ -14,8 +14,8 @@
 //
 // Where tiles are too few for 74 pairs, k is cut as well: the parts are stored in f32 and summed in order by a third kernel, so results do not vary.
 //
-// A CTA has 18 warps: 0 loads tokens (TMA), 1 of the leader issues the MMAs, 2-9 dequantise, 10-17 are the epilogue, which works under the next tile's main
-// loop. Every wait is bounded; one that runs out sets the projections' error word.
+// A CTA has 27 warps: 0 loads tokens, 1 of the leader issues the MMAs, 2-17 dequantise, 18-25 are the epilogue, which works under the next tile's main loop,
+// 26 loads codes. Every wait is bounded; one that runs out sets the projections' error word.
 #include "gemm_pair.cuh"
 #include "w4.cuh"
 
@@ -27,8 +27,12 @@ namespace orion {
 namespace {
 
 using Pair = PairConfig;
-constexpr uint32_t kDequantWarps = 8, kFirstDequant = 2, kFirstEpilogue = kFirstDequant + kDequantWarps, kWarps = kFirstEpilogue + Pair::kEpilogueWarps;
-constexpr uint32_t kAhead = 4;           // stages of codes in registers
+constexpr uint32_t kDequantWarps = 16, kFirstDequant = 2, kFirstEpilogue = kFirstDequant + kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
+constexpr uint32_t kWarps = kCodesWarp + 1;
+constexpr uint32_t kCodeStages = 4, kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;  // ring of codes: 64 bytes a row and stage
+constexpr uint32_t kCodeRingOffset = Pair::kXRingOffset + Pair::kStages * Pair::kXBytes, kBarrierOffset = kCodeRingOffset + kCodeStages * kCodeBytes;
+constexpr int kSmemBytes = kBarrierOffset + 1024 /*align*/ + 512 /*barriers*/;
+static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
 constexpr uint32_t kTileRows = 2 * Pair::kRows;
 constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to
 static_assert(Pair::kStageK == 128, "a stage is four pieces of 32 k");
@@ -189,9 +193,9 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ uint4 load_codes(const uint32_t *p) {
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -202,14 +206,16 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) 
 
 template <bool GATED, bool ZEROS>
 __global__ void __launch_bounds__(kWarps * 32, 1)
-w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const Workspace ws, const Plan plan, uint32_t *error) {
+w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+               const __grid_constant__ CUtensorMap map_up, const Workspace ws, const Plan plan, uint32_t *error) {
   constexpr uint32_t kStages = Pair::kStages, kMatrices = GATED ? 2 : 1;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint8_t *w_ring = smem, *x_ring = smem + Pair::kXRingOffset;
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + Pair::kBarrierOffset);
-  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+  uint8_t *code_ring = smem + kCodeRingOffset;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kBarrierOffset);
+  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2, *code_full = acc_empty + 2, *code_empty = code_full + kCodeStages;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + kCodeStages);
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -225,6 +231,10 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], 2 * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
+    }
+    for (uint32_t s = 0; s < kCodeStages; ++s) {
+      mbar_init(&code_full[s], 1);
+      mbar_init(&code_empty[s], kDequantWarps);
     }
     mbar_fence_init();
   }
@@ -312,128 +322,99 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         const Job j = job(t);
         for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
           if (!wait(&full[it % kStages], (it / kStages) & 1)) { ok = false; break; }
-          fence_proxy_async_all();
           if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&full[it % kStages]), 0));
           __syncwarp();
         }
       }
     }
+  } else if (warp == kCodesWarp) {
+    // Codes, ahead of everything else: the weights were complete before the first kernel began, whose beginning this one's launch waited for.
+    const bool elected = elect_one();
+    uint32_t it = 0;
+    for (uint32_t t = pair; ok && t < total; t += pairs) {
+      const Job j = job(t);
+      const int row = (int)((j.w_row + rank * Pair::kRows) / kMatrices);
+      for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
+        const uint32_t s = it % kCodeStages;
+        if (it >= kCodeStages && !wait(&code_empty[s], ((it / kCodeStages) & 1) ^ 1)) { ok = false; break; }
+        if (elected) {
+          mbar_arrive_expect_tx(&code_full[s], kCodeBytes);
+          tma_load_2d(code_ring + s * kCodeBytes, &map_w, (int)(kb * kCodeRow), row, &code_full[s]);
+          if (GATED) tma_load_2d(code_ring + s * kCodeBytes + kCodeBytes / 2, &map_up, (int)(kb * kCodeRow), row, &code_full[s]);
+        }
+        __syncwarp();
+      }
+    }
   } else if (warp < kFirstEpilogue) {
-    // Weights: sixteen rows of the CTA's 128 a warp, as two sets of eight; a lane has 32 k (piece) of a row of each. With a gate every other row of a tile is
-    // the gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds both.
-    const uint32_t piece = lane & 3, in_tile = (warp - kFirstDequant) * 16 + (lane >> 2);
+    // Weights: eight rows of the CTA's 128 a warp, 32 k (piece) of a row a lane. With a gate every other row of a tile is the gate's and the next the other
+    // matrix's, so that a pair of lanes of the epilogue holds both; in the ring of codes the gate's 64 rows come first.
+    //
+    // The values are made before the place for them is free: what stands between the MMAs that leave a stage and those that take it next is four stores.
+    const uint32_t piece = lane & 3, q8 = lane >> 2;
+    const uint32_t in_tile = (warp - kFirstDequant) * 8 + (GATED ? 2 * (q8 & 3) + (q8 >> 2) : q8);
+    const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile;
+    const uint32_t code_from = smem_u32(code_ring) + code_row * kCodeRow + piece * 16;
     // chunks of 16 bytes are permuted by row & 7; lanes of the upper 64 k take theirs in another order, so that eight lanes meet eight different banks
-    const uint32_t turn_around = piece >= 2 ? 2 : 0;
-    const uint32_t to = smem_u32(w_ring) + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ turn_around ^ (in_tile & 7)) * 16;
-    struct Codes {
-      uint4 words[2];
-      uint32_t scale[2], zero[2];  // as loaded: anything done to them here would wait for them
-    };
-    Codes held[kAhead];
+    constexpr uint32_t kTurn = GATED ? 1 : 2;
+    const bool turned = piece >= 2;
+    const uint32_t to = smem_u32(w_ring) + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ (turned ? kTurn : 0) ^ (in_tile & 7)) * 16;
     const uint32_t group_bits = 31 - __clz((int)c.group);
-    // What is read next
-    uint32_t load_t = pair, load_kb = 0, load_end = 0;
-    const uint32_t *from[2] = {};
-    const uint16_t *scale_from[2] = {};
-    const uint8_t *zero_from[2] = {};
-    bool there[2] = {};
-    auto aim = [&] {  // at the first stage of the next job
-      while (load_t < total) {
-        const Job j = job(load_t);
-        load_kb = j.kb, load_end = j.end;
-        if (load_kb < load_end) {
-#pragma unroll
-          for (uint32_t i = 0; i < 2; ++i) {
-            const uint32_t r = j.w_row + rank * Pair::kRows + in_tile + i * 8, row = GATED ? r >> 1 : r;
-            const W4View &w = GATED && (r & 1) ? c.up : c.w;
-            there[i] = row < c.n;
-            from[i] = w.packed + (uint64_t)(there[i] ? row : 0) * (c.k / 8) + piece * 4;
-            scale_from[i] = reinterpret_cast<const uint16_t *>(w.scales) + (there[i] ? row : 0);
-            zero_from[i] = w.zeros ? w.zeros + (there[i] ? row : 0) : nullptr;
-          }
-          return;
-        }
-        load_t += pairs;
-      }
-    };
-    auto load = [&](Codes &d) {
-      if (load_t >= total) return;
-      const uint32_t k = load_kb * Pair::kStageK + piece * 32;
-#pragma unroll
-      for (uint32_t i = 0; i < 2; ++i) {
-        d.words[i] = make_uint4(0, 0, 0, 0);
-        d.scale[i] = 0, d.zero[i] = 8;
-        if (there[i] && k < c.k) {
-          d.words[i] = load_codes(from[i] + load_kb * (Pair::kStageK / 8));
-          const uint64_t at = (uint64_t)(k >> group_bits) * c.n;
-          d.scale[i] = __ldg(scale_from[i] + at);
-          if (ZEROS && zero_from[i]) d.zero[i] = __ldg(zero_from[i] + at);
-        }
-      }
-      if (++load_kb == load_end) load_t += pairs, aim();
-    };
-    aim();
-#pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) load(held[i]);
+    const W4View &w = GATED && (in_tile & 1) ? c.up : c.w;
     pdl_wait();
 
-    uint32_t it = 0, t = pair, kb = 0, end = 0;
-    int32_t raise[2] = {};  // what a row's scales are multiplied by, as an exponent
-    bool more = false;
-    auto next_job = [&] {
-      more = false;
-      for (; t < total; t += pairs) {
-        const Job j = job(t);
-        if (j.kb >= j.end) continue;
-        kb = j.kb, end = j.end, more = true;
-#pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) {
-          const uint32_t r = j.w_row + rank * Pair::kRows + in_tile + i * 8, row = GATED ? r >> 1 : r;
-          raise[i] = row < c.n ? kTop - ws.w_exp[(GATED && (r & 1) ? c.n : 0) + row] : 0;
-        }
-        break;
+    // Jobs and stages, one stage ahead with scales and zero points; these stay as loaded: anything done to them ahead of time would wait for them
+    uint32_t load_t = pair, load_kb = 0, load_end = 0, row = 0, next_scale = 0, next_zero = 8;
+    int32_t load_raise = 0;  // what a row's scales are multiplied by, as an exponent
+    auto aim = [&] {
+      if (load_t >= total) return;
+      const Job j = job(load_t);
+      load_kb = j.kb, load_end = j.end, row = (j.w_row + rank * Pair::kRows + in_tile) / kMatrices;
+      load_raise = row < c.n ? kTop - ws.w_exp[(GATED && (in_tile & 1) ? c.n : 0) + row] : 0;
+    };
+    auto load = [&] {
+      const uint32_t k = load_kb * Pair::kStageK + piece * 32;
+      next_scale = 0, next_zero = 8;
+      if (load_t < total && row < c.n && k < c.k) {
+        const uint64_t at = (uint64_t)(k >> group_bits) * c.n + row;
+        next_scale = __ldg(reinterpret_cast<const uint16_t *>(w.scales) + at);
+        if (ZEROS && w.zeros) next_zero = __ldg(w.zeros + at);
       }
     };
-    next_job();
-    while (ok && more) {
+    aim();
+    load();
+    for (uint32_t it = 0; ok && load_t < total; ++it) {
+      const uint32_t s = it % kStages, cs = it % kCodeStages, p = next_scale, e = p >> 7 & 255u;
+      if (!wait(&code_full[cs], (it / kCodeStages) & 1)) { ok = false; break; }
+      const uint4 codes = lds128(code_from + cs * kCodeBytes);
+      const int32_t raised = (int32_t)e + load_raise;
+      // infinities and NaN stay, what is far below the row's largest scale vanishes
+      const uint32_t f = e == 255u ? p << 16 : raised <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)load_raise << 23);
+      const __half h = __float2half_rn(__uint_as_float(f));
+      const uint32_t low = (uint32_t)__half_as_ushort(h) * 0x10001u, high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
+      const uint32_t eight = hmul2(low, 0x80088008u);                                                // -8 * 2^-24 * scale
+      const uint32_t zero = next_zero * 0x10001u, zero_high = zero << 4;
+      if (++load_kb == load_end) load_t += pairs, aim();
+      load();
+      uint32_t v[4][4];
 #pragma unroll
-      for (uint32_t u = 0; u < kAhead; ++u) {
-        if (!ok || !more) break;
-        const uint32_t s = it % kStages;
-        if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+        const uint32_t word = turned ? words[j ^ kTurn] : words[j], rest = word >> 8;
+        v[j][0] = word & 0x000f000fu, v[j][1] = word & 0x00f000f0u, v[j][2] = rest & 0x000f000fu, v[j][3] = rest & 0x00f000f0u;
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) {
-          const uint32_t p = held[u].scale[i], e = p >> 7 & 255u;
-          const int32_t raised = (int32_t)e + raise[i];
-          // infinities and NaN stay, what is far below the row's largest scale vanishes
-          const uint32_t f = e == 255u ? p << 16 : raised <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise[i] << 23);
-          const __half h = __float2half_rn(__uint_as_float(f));
-          const uint32_t low = (uint32_t)__half_as_ushort(h) * 0x10001u, high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
-          const uint32_t eight = hmul2(low, 0x80088008u);                                                // -8 * 2^-24 * scale
-          const uint32_t zero = held[u].zero[i] * 0x10001u, zero_high = zero << 4;
-          uint32_t w[4] = {held[u].words[i].x, held[u].words[i].y, held[u].words[i].z, held[u].words[i].w};
-          if (turn_around) {
-            const uint32_t a = w[0], b = w[1];
-            w[0] = w[2], w[1] = w[3], w[2] = a, w[3] = b;
-          }
-#pragma unroll
-          for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t rest = w[j] >> 8;
-            uint32_t v[4] = {w[j] & 0x000f000fu, w[j] & 0x00f000f0u, rest & 0x000f000fu, rest & 0x00f000f0u};
-#pragma unroll
-            for (uint32_t q = 0; q < 4; ++q) {
-              if (ZEROS) v[q] = hmul2(hsub2(v[q], q & 1 ? zero_high : zero), q & 1 ? high : low);
-              else v[q] = hfma2(v[q], q & 1 ? high : low, eight);
-            }
-            sts128(to + s * Pair::kWBytes + i * 8 * 128 + (chunk ^ (j * 16)), v[0], v[1], v[2], v[3]);
-          }
+        for (uint32_t q = 0; q < 4; ++q) {
+          if (ZEROS) v[j][q] = hmul2(hsub2(v[j][q], q & 1 ? zero_high : zero), q & 1 ? high : low);
+          else v[j][q] = hfma2(v[j][q], q & 1 ? high : low, eight);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
-        load(held[u]);
-        ++it;
-        if (++kb == end) t += pairs, next_job();
+      }
+      if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) sts128(to + s * Pair::kWBytes + (chunk ^ (j * 16)), v[j][0], v[j][1], v[j][2], v[j][3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&full[s]);
+        mbar_arrive(&code_empty[cs]);
       }
     }
   } else {
@@ -532,28 +513,35 @@ __global__ void __launch_bounds__(256) w4_sum_kernel(const W4Call c, const float
   static_cast<bf16 *>(c.out)[(uint64_t)m * c.ldo + n] = __float2bfloat16_rn(y);
 }
 
-int token_map(CUtensorMap *map, const __half *x, uint32_t rows, uint32_t k, uint32_t box_rows) {
+// [rows][cols] matrix of 16-bit or 8-bit elements, without gaps; boxes of box_cols x box_rows.
+int matrix_map(CUtensorMap *map, CUtensorMapDataType type, uint32_t size, CUtensorMapSwizzle swizzle, const void *base, uint64_t rows, uint64_t cols,
+               uint32_t box_cols, uint32_t box_rows) {
   EncodeFn fn = encode_fn();
   if (!fn) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: driver entry point missing");
-  const cuuint64_t dims[2] = {k, rows}, strides[1] = {(cuuint64_t)k * 2};
-  const cuuint32_t box[2] = {Pair::kSlabK, box_rows}, one[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half *>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: encode returned %d (rows %u k %u)", (int)r, rows, k);
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * size};
+  const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
+  const CUresult r = fn(map, type, 2, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: encode returned %d (%llu x %llu)", (int)r, (unsigned long long)rows, (unsigned long long)cols);
   return ORION_OK;
 }
 
 template <bool GATED, bool ZEROS>
 int launch_pair(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
   static bool done[kMaxDeviceOrdinals] = {};
-  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_pair_kernel<GATED, ZEROS>, Pair::kSmemBytes, done));
-  CUtensorMap map;
-  ORION_TRY(token_map(&map, ws.x, c.rows, c.k, plan.tokens / 2));
-  const uint32_t matrices = GATED ? 2 : 1, jobs = plan.tiles_w * plan.tiles_x * plan.splits;
+  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_pair_kernel<GATED, ZEROS>, kSmemBytes, done));
+  const uint32_t matrices = GATED ? 2 : 1;
+  CUtensorMap map_x, map_w, map_up;
+  ORION_TRY(matrix_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, ws.x, c.rows, c.k, Pair::kSlabK, plan.tokens / 2));
+  ORION_TRY(matrix_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_NONE, c.w.packed, c.n, c.k / 2, kCodeRow, Pair::kRows / matrices));
+  map_up = map_w;
+  if (GATED) ORION_TRY(matrix_map(&map_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_NONE, c.up.packed, c.n, c.k / 2, kCodeRow, Pair::kRows / 2));
+  const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
   const uint32_t blocks = c.rows + (c.n * matrices + kPrepThreads - 1) / kPrepThreads;
   ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices));
   ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_pair_kernel<GATED, ZEROS>, dim3(2 * std::min(jobs, kPairs)), dim3(kWarps * 32), dim3(2, 1, 1),
-                                                       Pair::kSmemBytes, stream, c, map, ws, plan, error));
+                                                       kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, error));
   count_launch();
   count_launch();
   if (plan.splits > 1) {
