@@ -33,9 +33,9 @@ struct W4Call {
 template <typename T>
 int launch_w4_few(const W4Call &c, cudaStream_t stream);
 
-// bf16 activations of many rows; `workspace` holds w4_pair_workspace() bytes, `error` is the word that waits which run out set.
-uint64_t w4_pair_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k);
-int launch_w4_pair(const W4Call &c, void *workspace, uint32_t *error, cudaStream_t stream);
+// bf16 activations of many rows; `workspace` holds w4_tiles_workspace() bytes, `error` is the word that waits which run out set.
+uint64_t w4_tiles_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k);
+int launch_w4_tiles(const W4Call &c, void *workspace, uint32_t *error, cudaStream_t stream);
 
 template <typename T>
 int launch_w4_quantize(const T *w, uint64_t ldw, uint32_t n, uint32_t k, uint32_t group, uint32_t *packed, bf16 *scales, uint8_t *zeros, cudaStream_t stream);

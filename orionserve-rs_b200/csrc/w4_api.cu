@@ -66,9 +66,9 @@ int check_product(int dtype, const void *x, uint64_t rows, uint64_t x_stride, co
   return ORION_OK;
 }
 
-// The pairs of CTAs take bf16 products of more rows than this, and of at least a stage of k.
+// The tiles of tcgen05 take bf16 products of more rows than this, and of at least a stage of k.
 constexpr uint64_t kFewRows = 16;
-bool takes_pairs(int dtype, uint64_t rows, uint64_t k) { return dtype == ORION_DTYPE_BF16 && rows > kFewRows && k >= 128; }
+bool takes_tiles(int dtype, uint64_t rows, uint64_t k) { return dtype == ORION_DTYPE_BF16 && rows > kFewRows && k >= 128; }
 
 // Address of the projections' error word, looked up once per device.
 int error_word(int device, uint32_t **word) {
@@ -83,12 +83,12 @@ int error_word(int device, uint32_t **word) {
 }
 
 int launch(int device, int dtype, const W4Call &c, void *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
-  if (!takes_pairs(dtype, c.rows, c.k)) {
+  if (!takes_tiles(dtype, c.rows, c.k)) {
     ScopedDevice current(device);
     ORION_CUDA_CHECK("set device", current.status);
     return dtype == ORION_DTYPE_F32 ? launch_w4_few<float>(c, stream) : launch_w4_few<bf16>(c, stream);
   }
-  const uint64_t need = w4_pair_workspace(c.rows, c.up.packed ? 2 * c.n : c.n, c.k);
+  const uint64_t need = w4_tiles_workspace(c.rows, c.up.packed ? 2 * c.n : c.n, c.k);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return set_error(ORION_ERR_INVALID_REQUEST, "a workspace of %llu bytes on a 256-byte boundary is needed, got %llu", (unsigned long long)need,
                      (unsigned long long)(workspace ? workspace_bytes : 0));
@@ -96,7 +96,7 @@ int launch(int device, int dtype, const W4Call &c, void *workspace, uint64_t wor
   ORION_CUDA_CHECK("set device", current.status);
   uint32_t *error = nullptr;
   ORION_TRY(error_word(device, &error));
-  return launch_w4_pair(c, workspace, error, stream);
+  return launch_w4_tiles(c, workspace, error, stream);
 }
 
 }  // namespace
@@ -135,7 +135,7 @@ int orion_cuda_w4_workspace(int dtype, uint64_t rows, const OrionW4Weight *weigh
   ORION_TRY(check_dtype(dtype));
   ORION_TRY(check_weight("weight", weight));
   if (rows > kMostRows) return set_error(ORION_ERR_INVALID_REQUEST, "%llu rows: at most 2^30 are possible", (unsigned long long)rows);
-  if (takes_pairs(dtype, rows, weight->in_features)) *bytes = w4_pair_workspace((uint32_t)rows, (uint32_t)weight->out_features * (gated ? 2 : 1), (uint32_t)weight->in_features);
+  if (takes_tiles(dtype, rows, weight->in_features)) *bytes = w4_tiles_workspace((uint32_t)rows, (uint32_t)weight->out_features * (gated ? 2 : 1), (uint32_t)weight->in_features);
   return ORION_OK;
 }
 

@@ -30,10 +30,20 @@ using Pair = PairConfig;
 constexpr uint32_t kDequantWarps = 16, kFirstDequant = 2, kFirstEpilogue = kFirstDequant + kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
 constexpr uint32_t kWarps = kCodesWarp + 1;
 constexpr uint32_t kCodeStages = 4, kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;  // ring of codes: 64 bytes a row and stage
-constexpr uint32_t kCodeRingOffset = Pair::kXRingOffset + Pair::kStages * Pair::kXBytes, kBarrierOffset = kCodeRingOffset + kCodeStages * kCodeBytes;
-constexpr int kSmemBytes = kBarrierOffset + 1024 /*align*/ + 512 /*barriers*/;
-static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
-constexpr uint32_t kTileRows = 2 * Pair::kRows;
+
+// CTAS: 1 or 2 that work as an MMA unit on 128 weight rows each; TOKENS: rows of x in a stage of a CTA (a pair's CTAs hold half of a tile's each).
+template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGES>
+struct Form {
+  static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTileRows = CTAS * Pair::kRows;
+  static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = STAGES * Pair::kWBytes, kCodeRing = kXRing + STAGES * kXBytes;
+  static constexpr uint32_t kBarriers = kCodeRing + kCodeStages * kCodeBytes;
+  static constexpr int kSmemBytes = kBarriers + 1024 /*align*/ + 512 /*barriers*/;
+  static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
+};
+using Single64 = Form<1, 64, 4>;
+using Single128 = Form<1, 128, 3>;
+using Paired = Form<2, 128, 3>;
+constexpr uint32_t kSms = 2 * kPairs;
 constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to
 static_assert(Pair::kStageK == 128, "a stage is four pieces of 32 k");
 
@@ -47,22 +57,24 @@ struct Workspace {
 
 struct Plan {
   uint32_t tokens = 256, splits = 1, tiles_w = 0, tiles_x = 0, stages = 0;
+  uint32_t ctas = 2;  // of an MMA unit
 };
 
-// Rounds of the 74 pairs times what a round takes, in cycles: a stage takes the tensor cores two cycles a token column and the dequantising warps some 420
-// cycles, a tile's end some 3000; parts of k are written and read again.
+// Up to 128 tokens single CTAs, beyond them pairs. Tiles and parts of k so that the rounds of the units, times what a round takes, are least, in cycles: a
+// stage takes the tensor cores four cycles a token column and the dequantising warps some 450, a tile's end some 3000; parts of k are written and read again.
 Plan make_plan(uint32_t rows, uint32_t weight_rows, uint32_t k) {
   Plan best;
   double cost = 1e300;
-  const uint32_t stages = (k + Pair::kStageK - 1) / Pair::kStageK, tiles_w = (weight_rows + kTileRows - 1) / kTileRows;
+  const uint32_t ctas = rows <= Single128::kTokens ? 1 : 2, units = kSms / ctas;
+  const uint32_t stages = (k + Pair::kStageK - 1) / Pair::kStageK, tiles_w = (weight_rows + ctas * Pair::kRows - 1) / (ctas * Pair::kRows);
   const uint32_t most = std::min(256u, (rows + 31) / 32 * 32);
   for (uint32_t tokens = most; tokens >= std::min(most, 128u); tokens -= 32) {
     const uint32_t tiles_x = (rows + tokens - 1) / tokens;
-    for (uint32_t splits = 1; splits <= 8 && splits <= stages && (splits == 1 || (uint64_t)tiles_w * tiles_x <= 8 * kPairs); ++splits) {
-      const uint64_t jobs = (uint64_t)tiles_w * tiles_x * splits, rounds = (jobs + kPairs - 1) / kPairs;
-      double c = (double)rounds * ((stages + splits - 1) / splits * std::max(2.0 * tokens + 32.0, 420.0) + 3000.0);
+    for (uint32_t splits = 1; splits <= 8 && splits <= stages && (splits == 1 || (uint64_t)tiles_w * tiles_x <= 8 * units); ++splits) {
+      const uint64_t jobs = (uint64_t)tiles_w * tiles_x * splits, rounds = (jobs + units - 1) / units;
+      double c = (double)rounds * ((stages + splits - 1) / splits * std::max(4.0 * tokens, 450.0) + 3000.0);
       if (splits > 1) c += 4000.0 + (double)splits * rows * weight_rows * 8.0 / 2500.0;
-      if (c < cost) cost = c, best = {tokens, splits, tiles_w, tiles_x, stages};
+      if (c < cost) cost = c, best = {tokens, splits, tiles_w, tiles_x, stages, ctas};
     }
   }
   return best;
@@ -178,6 +190,9 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity
   }
   return false;
 }
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -204,33 +219,34 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
 // f32 accumulation, f16 x f16
 __device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
 
-template <bool GATED, bool ZEROS>
+template <typename F, bool GATED, bool ZEROS>
 __global__ void __launch_bounds__(kWarps * 32, 1)
-w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                const __grid_constant__ CUtensorMap map_up, const Workspace ws, const Plan plan, uint32_t *error) {
-  constexpr uint32_t kStages = Pair::kStages, kMatrices = GATED ? 2 : 1;
+  constexpr uint32_t kStages = F::kStages, kMatrices = GATED ? 2 : 1;
+  constexpr bool kPair = F::kCtas == 2;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
-  uint8_t *w_ring = smem, *x_ring = smem + Pair::kXRingOffset;
-  uint8_t *code_ring = smem + kCodeRingOffset;
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kBarrierOffset);
+  uint8_t *w_ring = smem, *x_ring = smem + F::kXRing;
+  uint8_t *code_ring = smem + F::kCodeRing;
+  uint64_t *full = reinterpret_cast<uint64_t *>(smem + F::kBarriers);
   uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2, *code_full = acc_empty + 2, *code_empty = code_full + kCodeStages;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + kCodeStages);
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = blockIdx.x & 1u, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t rank = blockIdx.x % F::kCtas, unit = blockIdx.x / F::kCtas, units = gridDim.x / F::kCtas;
   const bool leader = rank == 0;
   const uint32_t total = plan.tiles_w * plan.tiles_x * plan.splits, weight_rows = kMatrices * c.n;
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kStages; ++s) {
       // leader: the announcement of the tokens' bytes, its own weights, word of the peer's; peer: its weights
-      mbar_init(&full[s], leader ? 2 + kDequantWarps : kDequantWarps);
+      mbar_init(&full[s], !leader ? kDequantWarps : F::kCtas + kDequantWarps);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 2 * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
+      mbar_init(&acc_empty[b], F::kCtas * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
     }
     for (uint32_t s = 0; s < kCodeStages; ++s) {
       mbar_init(&code_full[s], 1);
@@ -239,18 +255,31 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     mbar_fence_init();
   }
   if (warp == 1) {
-    tmem_alloc_pair(tmem_slot, Pair::kTmemCols);
-    tmem_relinquish_pair();
+    if constexpr (kPair) {
+      tmem_alloc_pair(tmem_slot, Pair::kTmemCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, Pair::kTmemCols);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_arrive_release();  // the peer's barriers exist before anything of this CTA signals them
-  cluster_wait_acquire();
+  if constexpr (kPair) {
+    cluster_arrive_release();  // the peer's barriers exist before anything of this CTA signals them
+    cluster_wait_acquire();
+  }
   tc_fence_after();
   pdl_trigger();
   const uint32_t tmem_base = *tmem_slot;
   bool ok = true;
-  auto wait = [](uint64_t *bar, uint32_t parity) { return (bool)__all_sync(0xffffffffu, mbar_wait_cluster(bar, parity)); };  // one answer for a warp
+  auto wait = [](uint64_t *bar, uint32_t parity) {  // one answer for a warp
+    return (bool)__all_sync(0xffffffffu, kPair ? mbar_wait_cluster(bar, parity) : mbar_wait(bar, parity));
+  };
+  auto commit = [](uint64_t *bar) {  // on this barrier in all CTAs of the unit, once the MMAs issued so far have ended
+    if constexpr (kPair) umma_commit_both(bar);
+    else umma_commit(bar);
+  };
 
   // A job: weight rows w_row .. + 255 against tokens x_row .. + cols - 1, stages kb .. end - 1 of k. Splits of a tile are neighbours: they share tokens and
   // weights of L2.
@@ -260,27 +289,29 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
   auto job = [&](uint32_t id) {
     const TileXy t = raster(id / plan.splits, plan.tiles_w, plan.tiles_x);
     const uint32_t split = id % plan.splits, x_row = t.y * plan.tokens;
-    return Job{t.x * kTileRows, x_row, min(plan.tokens, (c.rows - x_row + 31) / 32 * 32), split * plan.stages / plan.splits, (split + 1) * plan.stages / plan.splits, split};
+    return Job{t.x * F::kTileRows, x_row, min(plan.tokens, (c.rows - x_row + 31) / 32 * 32), split * plan.stages / plan.splits, (split + 1) * plan.stages / plan.splits, split};
   };
 
   if (warp == 0) {
     // Tokens: this CTA's half of a tile's; the bytes of both CTAs are counted on the leader's barrier. Nothing is there beyond the last token and k: zeros.
     const bool elected = elect_one();
-    const uint32_t box = plan.tokens / 2;
+    const uint32_t box = plan.tokens / F::kCtas;
     uint32_t it = 0;
     pdl_wait();
-    for (uint32_t t = pair; ok && t < total; t += pairs) {
+    for (uint32_t t = unit; ok && t < total; t += units) {
       const Job j = job(t);
       for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
         const uint32_t s = it % kStages;
         if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
         if (elected) {
-          const uint32_t bar = mapa_u32(smem_u32(&full[s]), 0);
-          if (leader) mbar_arrive_expect_tx(&full[s], 2 * 2 * box * Pair::kSlabK * 2);
+          if (leader) mbar_arrive_expect_tx(&full[s], F::kCtas * 2 * box * Pair::kSlabK * 2);
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h)
-            tma_load_2d_pair(x_ring + s * Pair::kXBytes + h * Pair::kXSlab, &map_x, (int)(kb * Pair::kStageK + h * Pair::kSlabK),
-                             (int)(j.x_row + rank * (j.cols / 2)), bar);
+          for (uint32_t h = 0; h < 2; ++h) {
+            uint8_t *to = x_ring + s * F::kXBytes + h * F::kXSlab;
+            const int k = (int)(kb * Pair::kStageK + h * Pair::kSlabK), row = (int)(j.x_row + rank * (j.cols / F::kCtas));
+            if constexpr (kPair) tma_load_2d_pair(to, &map_x, k, row, mapa_u32(smem_u32(&full[s]), 0));
+            else tma_load_2d(to, &map_x, k, row, &full[s]);
+          }
         }
         __syncwarp();
       }
@@ -292,9 +323,9 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       const uint64_t w_desc = desc_k_sw128(smem_u32(w_ring)), x_desc = desc_k_sw128(smem_u32(x_ring));
       const bool elected = elect_one();
       uint32_t it = 0, turn = 0;
-      for (uint32_t t = pair; ok && t < total; t += pairs, ++turn) {
+      for (uint32_t t = unit; ok && t < total; t += units, ++turn) {
         const Job j = job(t);
-        const uint32_t id = idesc_f16(kTileRows, j.cols), buf = turn & 1, acc = tmem_base + buf * Pair::kMaxTokens;
+        const uint32_t id = idesc_f16(F::kTileRows, j.cols), buf = turn & 1, acc = tmem_base + buf * Pair::kMaxTokens;
         if (!wait(&acc_empty[buf], ((turn >> 1) & 1) ^ 1)) { ok = false; break; }
         tc_fence_after();
         for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
@@ -302,27 +333,32 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
           if (!wait(&full[s], (it / kStages) & 1)) { ok = false; break; }
           tc_fence_after();
           if (elected) {
-            const uint64_t a = w_desc + s * (Pair::kWBytes >> 4), b = x_desc + s * (Pair::kXBytes >> 4);
+            const uint64_t a = w_desc + s * (Pair::kWBytes >> 4), b = x_desc + s * (F::kXBytes >> 4);
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h)
 #pragma unroll
-              for (uint32_t k = 0; k < Pair::kSlabK / 16; ++k)
-                umma_bf16_pair(acc, a + ((h * Pair::kWSlab + k * 32) >> 4), b + ((h * Pair::kXSlab + k * 32) >> 4), id, (kb > j.kb || h > 0 || k > 0) ? 1u : 0u);
-            umma_commit_both(&empty[s]);
+              for (uint32_t k = 0; k < Pair::kSlabK / 16; ++k) {
+                const uint64_t a_at = a + ((h * Pair::kWSlab + k * 32) >> 4), b_at = b + ((h * F::kXSlab + k * 32) >> 4);
+                const uint32_t more = kb > j.kb || h > 0 || k > 0 ? 1u : 0u;
+                if constexpr (kPair) umma_bf16_pair(acc, a_at, b_at, id, more);
+                else umma_bf16(acc, a_at, b_at, id, more);
+              }
+            commit(&empty[s]);
           }
           __syncwarp();
         }
-        if (ok && elected) umma_commit_both(&acc_full[buf]);
+        if (ok && elected) commit(&acc_full[buf]);
       }
     } else {
-      // Hands word of this CTA's weights on to the leader. Were every dequantising warp to arrive there by itself, each would wait at every stage until its
-      // stores are visible to the cluster.
+      // Hands word of this CTA's weights on to the leader. They are stores to this SM's own shared memory, which this SM's tensor cores read; the barrier that
+      // is waited for here has ordered them, and the arrival needs no more than that. (Released to the cluster it waits some hundred cycles at every stage:
+      // gated 4096 x 4096 to 14336 in 785 us against 704.)
       uint32_t it = 0;
-      for (uint32_t t = pair; ok && t < total; t += pairs) {
+      for (uint32_t t = unit; ok && t < total; t += units) {
         const Job j = job(t);
         for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
           if (!wait(&full[it % kStages], (it / kStages) & 1)) { ok = false; break; }
-          if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&full[it % kStages]), 0));
+          if (lane == 0) mbar_arrive_remote(mapa_u32(smem_u32(&full[it % kStages]), 0));
           __syncwarp();
         }
       }
@@ -331,7 +367,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     // Codes, ahead of everything else: the weights were complete before the first kernel began, whose beginning this one's launch waited for.
     const bool elected = elect_one();
     uint32_t it = 0;
-    for (uint32_t t = pair; ok && t < total; t += pairs) {
+    for (uint32_t t = unit; ok && t < total; t += units) {
       const Job j = job(t);
       const int row = (int)((j.w_row + rank * Pair::kRows) / kMatrices);
       for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
@@ -363,7 +399,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     pdl_wait();
 
     // Jobs and stages, one stage ahead with scales and zero points; these stay as loaded: anything done to them ahead of time would wait for them
-    uint32_t load_t = pair, load_kb = 0, load_end = 0, row = 0, next_scale = 0, next_zero = 8;
+    uint32_t load_t = unit, load_kb = 0, load_end = 0, row = 0, next_scale = 0, next_zero = 8;
     int32_t load_raise = 0;  // what a row's scales are multiplied by, as an exponent
     auto aim = [&] {
       if (load_t >= total) return;
@@ -393,7 +429,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       const uint32_t low = (uint32_t)__half_as_ushort(h) * 0x10001u, high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
       const uint32_t eight = hmul2(low, 0x80088008u);                                                // -8 * 2^-24 * scale
       const uint32_t zero = next_zero * 0x10001u, zero_high = zero << 4;
-      if (++load_kb == load_end) load_t += pairs, aim();
+      if (++load_kb == load_end) load_t += units, aim();
       load();
       uint32_t v[4][4];
 #pragma unroll
@@ -422,7 +458,7 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     // columns each.
     pdl_wait();
     uint32_t turn = 0;
-    for (uint32_t t = pair; ok && t < total; t += pairs, ++turn) {
+    for (uint32_t t = unit; ok && t < total; t += units, ++turn) {
       const Job j = job(t);
       const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * Pair::kMaxTokens;
       const uint32_t r = j.w_row + rank * Pair::kRows + (warp & 3) * 32 + lane, row = GATED ? r >> 1 : r;
@@ -437,7 +473,9 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       auto release = [&] {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[buf]), 0));
+        if (lane != 0) return;
+        if constexpr (kPair) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[buf]), 0));
+        else mbar_arrive(&acc_empty[buf]);
       };
       if (mb >= j.cols) release();
 #pragma unroll 1
@@ -481,9 +519,14 @@ w4_pair_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
   tc_fence_before();
   __syncthreads();
   // Neither CTA leaves, nor frees the tensor memory the pair allocated together, while the other may still be read by an MMA or be reading its accumulator.
-  cluster_arrive_release();
-  cluster_wait_acquire();
-  if (warp == 1) tmem_dealloc_pair(tmem_base, Pair::kTmemCols);
+  if constexpr (kPair) {
+    cluster_arrive_release();
+    cluster_wait_acquire();
+  }
+  if (warp == 1) {
+    if constexpr (kPair) tmem_dealloc_pair(tmem_base, Pair::kTmemCols);
+    else tmem_dealloc(tmem_base, Pair::kTmemCols);
+  }
 }
 
 // ---- third kernel: the parts of k, in order --------------------------------------------------------
@@ -527,21 +570,21 @@ int matrix_map(CUtensorMap *map, CUtensorMapDataType type, uint32_t size, CUtens
   return ORION_OK;
 }
 
-template <bool GATED, bool ZEROS>
-int launch_pair(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
+template <typename F, bool GATED, bool ZEROS>
+int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
   static bool done[kMaxDeviceOrdinals] = {};
-  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_pair_kernel<GATED, ZEROS>, kSmemBytes, done));
+  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_tile_kernel<F, GATED, ZEROS>, F::kSmemBytes, done));
   const uint32_t matrices = GATED ? 2 : 1;
   CUtensorMap map_x, map_w, map_up;
-  ORION_TRY(matrix_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, ws.x, c.rows, c.k, Pair::kSlabK, plan.tokens / 2));
+  ORION_TRY(matrix_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, ws.x, c.rows, c.k, Pair::kSlabK, plan.tokens / F::kCtas));
   ORION_TRY(matrix_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_NONE, c.w.packed, c.n, c.k / 2, kCodeRow, Pair::kRows / matrices));
   map_up = map_w;
   if (GATED) ORION_TRY(matrix_map(&map_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_NONE, c.up.packed, c.n, c.k / 2, kCodeRow, Pair::kRows / 2));
   const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
   const uint32_t blocks = c.rows + (c.n * matrices + kPrepThreads - 1) / kPrepThreads;
   ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices));
-  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_pair_kernel<GATED, ZEROS>, dim3(2 * std::min(jobs, kPairs)), dim3(kWarps * 32), dim3(2, 1, 1),
-                                                       kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, error));
+  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(kWarps * 32),
+                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, error));
   count_launch();
   count_launch();
   if (plan.splits > 1) {
@@ -552,15 +595,22 @@ int launch_pair(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   return ORION_OK;
 }
 
+template <bool GATED, bool ZEROS>
+int launch_kind(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
+  if (plan.ctas == 2) return launch_form<Paired, GATED, ZEROS>(c, ws, plan, error, stream);
+  if (plan.tokens > Single64::kTokens) return launch_form<Single128, GATED, ZEROS>(c, ws, plan, error, stream);
+  return launch_form<Single64, GATED, ZEROS>(c, ws, plan, error, stream);
+}
+
 }  // namespace
 
-uint64_t w4_pair_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k) {
+uint64_t w4_tiles_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k) {
   uint64_t bytes = 0;
   workspace_at(nullptr, rows, weight_rows, k, make_plan(rows, weight_rows, k), &bytes);
   return bytes;
 }
 
-int launch_w4_pair(const W4Call &c, void *workspace, uint32_t *error, cudaStream_t stream) {
+int launch_w4_tiles(const W4Call &c, void *workspace, uint32_t *error, cudaStream_t stream) {
   const uint32_t weight_rows = c.up.packed ? 2 * c.n : c.n;
   const Plan plan = make_plan(c.rows, weight_rows, c.k);
   if ((uint64_t)plan.tiles_w * plan.tiles_x * plan.splits > 0x7fffffffull || c.rows > 0x3fffffffu)
@@ -568,8 +618,8 @@ int launch_w4_pair(const W4Call &c, void *workspace, uint32_t *error, cudaStream
   uint64_t bytes = 0;
   const Workspace ws = workspace_at(static_cast<uint8_t *>(workspace), c.rows, weight_rows, c.k, plan, &bytes);
   const bool zeros = c.w.zeros || c.up.zeros;
-  if (c.up.packed) return zeros ? launch_pair<true, true>(c, ws, plan, error, stream) : launch_pair<true, false>(c, ws, plan, error, stream);
-  return zeros ? launch_pair<false, true>(c, ws, plan, error, stream) : launch_pair<false, false>(c, ws, plan, error, stream);
+  if (c.up.packed) return zeros ? launch_kind<true, true>(c, ws, plan, error, stream) : launch_kind<true, false>(c, ws, plan, error, stream);
+  return zeros ? launch_kind<false, true>(c, ws, plan, error, stream) : launch_kind<false, false>(c, ws, plan, error, stream);
 }
 
 }  // namespace orion
