@@ -34,7 +34,7 @@ template <typename T>
 int launch_w4_few(const W4Call &c, cudaStream_t stream);
 
 // bf16 activations of many rows; `workspace` holds w4_tiles_workspace() bytes, `error` is the word that waits which run out set.
-uint64_t w4_tiles_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k);
+uint64_t w4_tiles_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k, uint32_t group);
 int launch_w4_tiles(const W4Call &c, void *workspace, uint32_t *error, cudaStream_t stream);
 
 template <typename T>

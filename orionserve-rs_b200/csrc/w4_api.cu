@@ -88,7 +88,7 @@ int launch(int device, int dtype, const W4Call &c, void *workspace, uint64_t wor
     ORION_CUDA_CHECK("set device", current.status);
     return dtype == ORION_DTYPE_F32 ? launch_w4_few<float>(c, stream) : launch_w4_few<bf16>(c, stream);
   }
-  const uint64_t need = w4_tiles_workspace(c.rows, c.up.packed ? 2 * c.n : c.n, c.k);
+  const uint64_t need = w4_tiles_workspace(c.rows, c.up.packed ? 2 * c.n : c.n, c.k, c.group);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return set_error(ORION_ERR_INVALID_REQUEST, "a workspace of %llu bytes on a 256-byte boundary is needed, got %llu", (unsigned long long)need,
                      (unsigned long long)(workspace ? workspace_bytes : 0));
@@ -135,7 +135,7 @@ int orion_cuda_w4_workspace(int dtype, uint64_t rows, const OrionW4Weight *weigh
   ORION_TRY(check_dtype(dtype));
   ORION_TRY(check_weight("weight", weight));
   if (rows > kMostRows) return set_error(ORION_ERR_INVALID_REQUEST, "%llu rows: at most 2^30 are possible", (unsigned long long)rows);
-  if (takes_tiles(dtype, rows, weight->in_features)) *bytes = w4_tiles_workspace((uint32_t)rows, (uint32_t)weight->out_features * (gated ? 2 : 1), (uint32_t)weight->in_features);
+  if (takes_tiles(dtype, rows, weight->in_features)) *bytes = w4_tiles_workspace((uint32_t)rows, (uint32_t)weight->out_features * (gated ? 2 : 1), (uint32_t)weight->in_features, weight->group);
   return ORION_OK;
 }
 

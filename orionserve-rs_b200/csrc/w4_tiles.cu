@@ -2,8 +2,8 @@
 // into shared memory.
 //
 // From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05. A pair of CTAs works as one MMA unit on 256 weight rows x
-// up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: a ring of codes is filled by TMA, four stages of 128
-// k ahead, and eight warps of each CTA write the operand tiles of its 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
+// up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: a ring of codes is filled by TMA, and teams of warps
+// write the operand tiles of a CTA's 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
 //
 // The operands are f16, not bf16. (code - zero) * scale has at most 11 significant bits with a zero of 8 and 12 with any other, f16 holds 11: products are
 // exact, or off by 2^-12 of a weight, where bf16 would round every weight by 2^-9. Range is no matter, since both sides are scaled by powers of two, every
@@ -14,8 +14,8 @@
 //
 // Where tiles are too few for 74 pairs, k is cut as well: the parts are stored in f32 and summed in order by a third kernel, so results do not vary.
 //
-// A CTA has 27 warps: 0 loads tokens, 1 of the leader issues the MMAs, 2-17 dequantise, 18-25 are the epilogue, which works under the next tile's main loop,
-// 26 loads codes. Every wait is bounded; one that runs out sets the projections' error word.
+// Warp 0 loads tokens, 1 of the leader issues the MMAs, then come the dequantising warps, eight of the epilogue, which works under the next tile's main loop,
+// and one that loads codes. Every wait is bounded; one that runs out sets the projections' error word.
 #include "gemm_pair.cuh"
 #include "w4.cuh"
 
@@ -27,17 +27,17 @@ namespace orion {
 namespace {
 
 using Pair = PairConfig;
-constexpr uint32_t kDequantWarps = 16, kFirstDequant = 2, kFirstEpilogue = kFirstDequant + kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
-constexpr uint32_t kWarps = kCodesWarp + 1;
-constexpr uint32_t kCodeStages = 4, kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;  // ring of codes: 64 bytes a row and stage
+constexpr uint32_t kDequantWarps = 4, kFirstDequant = 2;             // warps that make a stage's weights; as many such teams as the rings have stages
+constexpr uint32_t kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;  // a stage of codes: 64 bytes a row
 
 // CTAS: 1 or 2 that work as an MMA unit on 128 weight rows each; TOKENS: rows of x in a stage of a CTA (a pair's CTAs hold half of a tile's each).
 template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGES>
 struct Form {
   static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTileRows = CTAS * Pair::kRows;
   static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = STAGES * Pair::kWBytes, kCodeRing = kXRing + STAGES * kXBytes;
-  static constexpr uint32_t kBarriers = kCodeRing + kCodeStages * kCodeBytes;
+  static constexpr uint32_t kBarriers = kCodeRing + STAGES * kCodeBytes;
   static constexpr int kSmemBytes = kBarriers + 1024 /*align*/ + 512 /*barriers*/;
+  static constexpr uint32_t kFirstEpilogue = kFirstDequant + STAGES * kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps, kWarps = kCodesWarp + 1;
   static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
 };
 using Single64 = Form<1, 64, 4>;
@@ -51,7 +51,9 @@ static_assert(Pair::kStageK == 128, "a stage is four pieces of 32 k");
 struct Workspace {
   __half *x = nullptr;        // [rows][k], scaled
   float *x_unit = nullptr;    // [rows, rounded up to 32] what a token was divided by, but for 2^kTop
-  int32_t *w_exp = nullptr;   // [weight rows] exponent of the largest scale
+  // Weight rows as tiles hold them: with a gate its rows and the other matrix's in turn. Rounded up to whole tiles.
+  float *w_unit = nullptr;    // [weight rows] 2^exponent of the largest scale
+  uint32_t *params = nullptr; // [k / group][weight rows] scale, in f16 and with the largest at 2^kTop .. 2^(kTop + 1), | zero << 16
   float *parts = nullptr;     // [splits][rows][weight rows]
 };
 
@@ -80,17 +82,20 @@ Plan make_plan(uint32_t rows, uint32_t weight_rows, uint32_t k) {
   return best;
 }
 
+constexpr uint32_t kParamRows = 2 * Pair::kRows;
+uint64_t padded_rows(uint32_t weight_rows) { return ((uint64_t)weight_rows + kParamRows - 1) / kParamRows * kParamRows; }
 uint64_t place(uint64_t *at, uint64_t bytes) {
   const uint64_t here = *at;
   *at += (bytes + 255) / 256 * 256;
   return here;
 }
-Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint32_t k, const Plan &plan, uint64_t *bytes) {
+Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint32_t k, uint32_t group, const Plan &plan, uint64_t *bytes) {
   uint64_t at = 0;
   Workspace w;
   w.x = reinterpret_cast<__half *>(base + place(&at, (uint64_t)rows * k * 2));
   w.x_unit = reinterpret_cast<float *>(base + place(&at, ((uint64_t)rows + 31) / 32 * 32 * 4));
-  w.w_exp = reinterpret_cast<int32_t *>(base + place(&at, (uint64_t)weight_rows * 4));
+  w.w_unit = reinterpret_cast<float *>(base + place(&at, padded_rows(weight_rows) * 4));
+  w.params = reinterpret_cast<uint32_t *>(base + place(&at, padded_rows(weight_rows) * (k / group) * 4));
   w.parts = reinterpret_cast<float *>(base + place(&at, plan.splits > 1 ? (uint64_t)plan.splits * rows * weight_rows * 4 : 0));
   *bytes = at;
   return w;
@@ -101,21 +106,44 @@ Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint3
 constexpr uint32_t kPrepThreads = 256, kHeld = 8;
 
 __global__ void __launch_bounds__(kPrepThreads)
-w4_prepare_kernel(const W4Call c, const Workspace ws, uint32_t matrices) {
+w4_prepare_kernel(const W4Call c, const Workspace ws, uint32_t matrices, uint32_t param_rows) {
   pdl_wait();
   pdl_trigger();  // after the wait: what the next kernel reads ahead of its own wait was complete before this one began
   if (blockIdx.x >= c.rows) {
-    const uint32_t i = (blockIdx.x - c.rows) * kPrepThreads + threadIdx.x;
-    if (i >= c.n * matrices) return;
-    const uint32_t row = i % c.n, groups = c.k / c.group;
-    const uint16_t *s = reinterpret_cast<const uint16_t *>(i >= c.n ? c.up.scales : c.w.scales) + row;
-    uint32_t top = 0;
-#pragma unroll 8
-    for (uint32_t g = 0; g < groups; ++g) {
-      const uint32_t e = __ldg(s + (uint64_t)g * c.n) >> 7 & 255u;
+    // 32 weight rows, their groups dealt to eight warps
+    constexpr uint32_t kMine = 8;
+    __shared__ uint32_t tops[kPrepThreads / 32][32];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = (blockIdx.x - c.rows) * 32 + lane, row = r / matrices, groups = c.k / c.group;
+    const W4View &w = r % matrices ? c.up : c.w;
+    const bool there = row < c.n;
+    uint32_t held[kMine], top = 0;
+    auto scale_of = [&](uint32_t g) { return there && g < groups ? (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(w.scales) + (uint64_t)g * c.n + row) : 0u; };
+    auto larger = [&](uint32_t p) {
+      const uint32_t e = p >> 7 & 255u;
       top = max(top, e == 255u ? 0u : e);
-    }
-    ws.w_exp[i] = top ? (int32_t)top - 127 : 0;
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < kMine; ++j) held[j] = scale_of(warp + j * 8);
+#pragma unroll
+    for (uint32_t j = 0; j < kMine; ++j) larger(held[j]);
+    for (uint32_t g = warp + kMine * 8; g < groups; g += 8) larger(scale_of(g));
+    tops[warp][lane] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kPrepThreads / 32; ++i) top = max(top, tops[i][lane]);
+    const int32_t raise = top ? kTop + 127 - (int32_t)top : 0;
+    auto store = [&](uint32_t g, uint32_t p) {
+      if (g >= groups) return;
+      const uint32_t e = p >> 7 & 255u;
+      // infinities and NaN stay, what is far below the row's largest scale vanishes
+      const uint32_t f = e == 255u ? p << 16 : (int32_t)e + raise <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise << 23);
+      const uint32_t zero = there && w.zeros ? __ldg(w.zeros + (uint64_t)g * c.n + row) : 8u;
+      ws.params[(uint64_t)g * param_rows + r] = (uint32_t)__half_as_ushort(__float2half_rn(__uint_as_float(f))) | zero << 16;
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < kMine; ++j) store(warp + j * 8, held[j]);
+    for (uint32_t g = warp + kMine * 8; g < groups; g += 8) store(g, scale_of(g));
+    if (warp == 0) ws.w_unit[r] = top ? __uint_as_float(top << 23) : 1.f;
     return;
   }
   const uint32_t m = blockIdx.x, pieces = c.k / 8;
@@ -213,6 +241,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t ld_params(const uint32_t *p) {  // in program order, so that a later load does not wait for the stage's arithmetic
+  uint32_t v;
+  asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -220,9 +253,9 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
 __device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
 
 template <typename F, bool GATED, bool ZEROS>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+__global__ void __launch_bounds__(F::kWarps * 32, 1)
 w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-               const __grid_constant__ CUtensorMap map_up, const Workspace ws, const Plan plan, uint32_t *error) {
+               const __grid_constant__ CUtensorMap map_up, const Workspace ws, const Plan plan, const uint32_t param_rows, uint32_t *error) {
   constexpr uint32_t kStages = F::kStages, kMatrices = GATED ? 2 : 1;
   constexpr bool kPair = F::kCtas == 2;
   extern __shared__ uint8_t raw_smem[];
@@ -230,8 +263,8 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
   uint8_t *w_ring = smem, *x_ring = smem + F::kXRing;
   uint8_t *code_ring = smem + F::kCodeRing;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + F::kBarriers);
-  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2, *code_full = acc_empty + 2, *code_empty = code_full + kCodeStages;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + kCodeStages);
+  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2, *code_full = acc_empty + 2, *code_empty = code_full + kStages;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + kStages);
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blockIdx.x % F::kCtas, unit = blockIdx.x / F::kCtas, units = gridDim.x / F::kCtas;
@@ -243,14 +276,12 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       // leader: the announcement of the tokens' bytes, its own weights, word of the peer's; peer: its weights
       mbar_init(&full[s], !leader ? kDequantWarps : F::kCtas + kDequantWarps);
       mbar_init(&empty[s], 1);
+      mbar_init(&code_full[s], 1);
+      mbar_init(&code_empty[s], kDequantWarps);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], F::kCtas * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
-    }
-    for (uint32_t s = 0; s < kCodeStages; ++s) {
-      mbar_init(&code_full[s], 1);
-      mbar_init(&code_empty[s], kDequantWarps);
     }
     mbar_fence_init();
   }
@@ -363,7 +394,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         }
       }
     }
-  } else if (warp == kCodesWarp) {
+  } else if (warp == F::kCodesWarp) {
     // Codes, ahead of everything else: the weights were complete before the first kernel began, whose beginning this one's launch waited for.
     const bool elected = elect_one();
     uint32_t it = 0;
@@ -371,8 +402,8 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       const Job j = job(t);
       const int row = (int)((j.w_row + rank * Pair::kRows) / kMatrices);
       for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
-        const uint32_t s = it % kCodeStages;
-        if (it >= kCodeStages && !wait(&code_empty[s], ((it / kCodeStages) & 1) ^ 1)) { ok = false; break; }
+        const uint32_t s = it % kStages;
+        if (it >= kStages && !wait(&code_empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
         if (elected) {
           mbar_arrive_expect_tx(&code_full[s], kCodeBytes);
           tma_load_2d(code_ring + s * kCodeBytes, &map_w, (int)(kb * kCodeRow), row, &code_full[s]);
@@ -381,77 +412,76 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         __syncwarp();
       }
     }
-  } else if (warp < kFirstEpilogue) {
-    // Weights: eight rows of the CTA's 128 a warp, 32 k (piece) of a row a lane. With a gate every other row of a tile is the gate's and the next the other
-    // matrix's, so that a pair of lanes of the epilogue holds both; in the ring of codes the gate's 64 rows come first.
-    //
-    // The values are made before the place for them is free: what stands between the MMAs that leave a stage and those that take it next is four stores.
-    const uint32_t piece = lane & 3, q8 = lane >> 2;
-    const uint32_t in_tile = (warp - kFirstDequant) * 8 + (GATED ? 2 * (q8 & 3) + (q8 >> 2) : q8);
+  } else if (warp < F::kFirstEpilogue) {
+    // Weights: 32 rows of the CTA's 128 a warp, as four sets of eight; a lane has 32 k (piece) of a row of each. With a gate every other row of a tile is the
+    // gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds both; in the ring of codes the gate's 64 rows come first. What
+    // a stage costs a warp besides its weights counts less with few warps to a stage: each team of four makes the stages of one place in the rings. (With
+    // more teams than places one could wait for a barrier that is two phases behind, and two phases are one to a wait.)
+    const uint32_t piece = lane & 3, q8 = lane >> 2, team = (warp - kFirstDequant) / kDequantWarps;
+    const uint32_t in_tile = (warp - kFirstDequant) % kDequantWarps * 32 + (GATED ? 2 * (q8 & 3) + (q8 >> 2) : q8);
     const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile;
-    const uint32_t code_from = smem_u32(code_ring) + code_row * kCodeRow + piece * 16;
+    const uint32_t code_from = smem_u32(code_ring) + team * kCodeBytes + code_row * kCodeRow + piece * 16;
     // chunks of 16 bytes are permuted by row & 7; lanes of the upper 64 k take theirs in another order, so that eight lanes meet eight different banks
     constexpr uint32_t kTurn = GATED ? 1 : 2;
     const bool turned = piece >= 2;
-    const uint32_t to = smem_u32(w_ring) + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ (turned ? kTurn : 0) ^ (in_tile & 7)) * 16;
-    const uint32_t group_bits = 31 - __clz((int)c.group);
-    const W4View &w = GATED && (in_tile & 1) ? c.up : c.w;
+    const uint32_t to = smem_u32(w_ring) + team * Pair::kWBytes + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ (turned ? kTurn : 0) ^ (in_tile & 7)) * 16;
+    const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
     pdl_wait();
 
-    // Jobs and stages, one stage ahead with scales and zero points; these stay as loaded: anything done to them ahead of time would wait for them
-    uint32_t load_t = unit, load_kb = 0, load_end = 0, row = 0, next_scale = 0, next_zero = 8;
-    int32_t load_raise = 0;  // what a row's scales are multiplied by, as an exponent
+    // Jobs and stages; the next stage's scales and zero points stay as loaded: anything done to them ahead of time would wait for them
+    uint32_t load_t = unit, load_kb = 0, load_end = 0, load_row = 0, next[4];
     auto aim = [&] {
       if (load_t >= total) return;
       const Job j = job(load_t);
-      load_kb = j.kb, load_end = j.end, row = (j.w_row + rank * Pair::kRows + in_tile) / kMatrices;
-      load_raise = row < c.n ? kTop - ws.w_exp[(GATED && (in_tile & 1) ? c.n : 0) + row] : 0;
+      load_kb = j.kb, load_end = j.end, load_row = j.w_row + rank * Pair::kRows + in_tile;
+    };
+    auto advance = [&] {
+      if (load_t < total && ++load_kb == load_end) load_t += units, aim();
     };
     auto load = [&] {
-      const uint32_t k = load_kb * Pair::kStageK + piece * 32;
-      next_scale = 0, next_zero = 8;
-      if (load_t < total && row < c.n && k < c.k) {
-        const uint64_t at = (uint64_t)(k >> group_bits) * c.n + row;
-        next_scale = __ldg(reinterpret_cast<const uint16_t *>(w.scales) + at);
-        if (ZEROS && w.zeros) next_zero = __ldg(w.zeros + at);
-      }
+      if (load_t >= total) return;
+      // beyond the last k the codes meet zeros: any scale does
+      const uint32_t *p = ws.params + (uint64_t)min((load_kb * Pair::kStageK + piece * 32) >> group_bits, last_group) * param_rows + load_row;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) next[i] = ld_params(p + i * 8);
     };
     aim();
+    for (uint32_t i = 0; i < team; ++i) advance();
     load();
-    for (uint32_t it = 0; ok && load_t < total; ++it) {
-      const uint32_t s = it % kStages, cs = it % kCodeStages, p = next_scale, e = p >> 7 & 255u;
-      if (!wait(&code_full[cs], (it / kCodeStages) & 1)) { ok = false; break; }
-      const uint4 codes = lds128(code_from + cs * kCodeBytes);
-      const int32_t raised = (int32_t)e + load_raise;
-      // infinities and NaN stay, what is far below the row's largest scale vanishes
-      const uint32_t f = e == 255u ? p << 16 : raised <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)load_raise << 23);
-      const __half h = __float2half_rn(__uint_as_float(f));
-      const uint32_t low = (uint32_t)__half_as_ushort(h) * 0x10001u, high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
-      const uint32_t eight = hmul2(low, 0x80088008u);                                                // -8 * 2^-24 * scale
-      const uint32_t zero = next_zero * 0x10001u, zero_high = zero << 4;
-      if (++load_kb == load_end) load_t += units, aim();
-      load();
-      uint32_t v[4][4];
+    for (uint32_t round = 0; ok && load_t < total; ++round) {
+      uint32_t param[4];
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) {
-        const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
-        const uint32_t word = turned ? words[j ^ kTurn] : words[j], rest = word >> 8;
-        v[j][0] = word & 0x000f000fu, v[j][1] = word & 0x00f000f0u, v[j][2] = rest & 0x000f000fu, v[j][3] = rest & 0x00f000f0u;
+      for (uint32_t i = 0; i < 4; ++i) param[i] = next[i];
 #pragma unroll
-        for (uint32_t q = 0; q < 4; ++q) {
-          if (ZEROS) v[j][q] = hmul2(hsub2(v[j][q], q & 1 ? zero_high : zero), q & 1 ? high : low);
-          else v[j][q] = hfma2(v[j][q], q & 1 ? high : low, eight);
+      for (uint32_t i = 0; i < kStages; ++i) advance();
+      if (!wait(&code_full[team], round & 1)) { ok = false; break; }
+      if (round > 0 && !wait(&empty[team], (round & 1) ^ 1)) { ok = false; break; }
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint4 codes = lds128(code_from + i * (GATED ? 4 : 8) * kCodeRow);
+        const uint32_t low = __byte_perm(param[i], 0, 0x1010), high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
+        const uint32_t eight = hmul2(low, 0x80088008u);                                        // -8 * 2^-24 * scale
+        const uint32_t zero = __byte_perm(param[i], 0, 0x3232), zero_high = zero << 4;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+          const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+          const uint32_t word = turned ? words[j ^ kTurn] : words[j], rest = word >> 8;
+          uint32_t v[4] = {word & 0x000f000fu, word & 0x00f000f0u, rest & 0x000f000fu, rest & 0x00f000f0u};
+#pragma unroll
+          for (uint32_t q = 0; q < 4; ++q) {
+            if (ZEROS) v[q] = hmul2(hsub2(v[q], q & 1 ? zero_high : zero), q & 1 ? high : low);
+            else v[q] = hfma2(v[q], q & 1 ? high : low, eight);
+          }
+          sts128(to + i * 8 * 128 + (chunk ^ (j * 16)), v[0], v[1], v[2], v[3]);
         }
       }
-      if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
-#pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) sts128(to + s * Pair::kWBytes + (chunk ^ (j * 16)), v[j][0], v[j][1], v[j][2], v[j][3]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&full[s]);
-        mbar_arrive(&code_empty[cs]);
+        mbar_arrive(&full[team]);
+        mbar_arrive(&code_empty[team]);
       }
+      load();
     }
   } else {
     // Epilogue: warp w reads tensor-memory lanes 32 * (w % 4) .. + 31 (lane = weight row, column = token); the two warps of the same lanes take turns, 16
@@ -463,13 +493,12 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * Pair::kMaxTokens;
       const uint32_t r = j.w_row + rank * Pair::kRows + (warp & 3) * 32 + lane, row = GATED ? r >> 1 : r;
       const bool inside = row < c.n;
-      // 2^exponent, and 2^-4 left of the powers that scales (2^14), codes (2^-24) and tokens (2^14) were brought to
-      const float unit = inside ? __uint_as_float((uint32_t)(ws.w_exp[(GATED && (r & 1) ? c.n : 0) + row] + 127) << 23) : 0.f;
+      const float row_unit = ws.w_unit[r];
       const float bias = !GATED && inside && c.bias && plan.splits == 1 ? c.bias[row] : 0.f;
       if (!wait(&acc_full[buf], (turn >> 1) & 1)) { ok = false; break; }
       tc_fence_after();
       constexpr uint32_t kStep = 16 * (Pair::kEpilogueWarps / 4);
-      uint32_t mb = 16 * ((warp - kFirstEpilogue) / 4);
+      uint32_t mb = 16 * ((warp - F::kFirstEpilogue) / 4);
       auto release = [&] {
         tc_fence_before();
         __syncwarp();
@@ -485,12 +514,12 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         tmem_ld_wait();
         if (mb + kStep >= j.cols) release();
         const uint32_t token = j.x_row + mb;
-        float v[16];
+        float v[16];  // 2^-4 is left of the powers that scales (2^14), codes (2^-24) and tokens (2^14) were brought to
 #pragma unroll
         for (uint32_t q = 0; q < 4; ++q) {
           const float4 f = *reinterpret_cast<const float4 *>(ws.x_unit + token + 4 * q);
-          v[4 * q] = __uint_as_float(rr[4 * q]) * 0.0625f * unit * f.x, v[4 * q + 1] = __uint_as_float(rr[4 * q + 1]) * 0.0625f * unit * f.y;
-          v[4 * q + 2] = __uint_as_float(rr[4 * q + 2]) * 0.0625f * unit * f.z, v[4 * q + 3] = __uint_as_float(rr[4 * q + 3]) * 0.0625f * unit * f.w;
+          v[4 * q] = __uint_as_float(rr[4 * q]) * 0.0625f * row_unit * f.x, v[4 * q + 1] = __uint_as_float(rr[4 * q + 1]) * 0.0625f * row_unit * f.y;
+          v[4 * q + 2] = __uint_as_float(rr[4 * q + 2]) * 0.0625f * row_unit * f.z, v[4 * q + 3] = __uint_as_float(rr[4 * q + 3]) * 0.0625f * row_unit * f.w;
         }
         if (plan.splits > 1) {
           float *p = ws.parts + ((uint64_t)j.split * c.rows + token) * weight_rows + r;
@@ -515,7 +544,12 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       }
     }
   }
-  if (!ok) atomicOr(error, 1u);
+  if (!ok) {  // copies that are on their way land in a few microseconds: they find this CTA's memory still there
+    atomicOr(error, 1u);
+    const uint64_t start = global_timer_ns();
+    for (uint32_t i = 0; i < (1u << 20) && global_timer_ns() - start < 200000u; ++i) {
+    }
+  }
   tc_fence_before();
   __syncthreads();
   // Neither CTA leaves, nor frees the tensor memory the pair allocated together, while the other may still be read by an MMA or be reading its accumulator.
@@ -581,10 +615,10 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   map_up = map_w;
   if (GATED) ORION_TRY(matrix_map(&map_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_NONE, c.up.packed, c.n, c.k / 2, kCodeRow, Pair::kRows / 2));
   const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
-  const uint32_t blocks = c.rows + (c.n * matrices + kPrepThreads - 1) / kPrepThreads;
-  ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices));
-  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(kWarps * 32),
-                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, error));
+  const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), blocks = c.rows + param_rows / 32;
+  ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices, param_rows));
+  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(F::kWarps * 32),
+                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, param_rows, error));
   count_launch();
   count_launch();
   if (plan.splits > 1) {
@@ -604,9 +638,9 @@ int launch_kind(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
 
 }  // namespace
 
-uint64_t w4_tiles_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k) {
+uint64_t w4_tiles_workspace(uint32_t rows, uint32_t weight_rows, uint32_t k, uint32_t group) {
   uint64_t bytes = 0;
-  workspace_at(nullptr, rows, weight_rows, k, make_plan(rows, weight_rows, k), &bytes);
+  workspace_at(nullptr, rows, weight_rows, k, group, make_plan(rows, weight_rows, k), &bytes);
   return bytes;
 }
 
@@ -616,7 +650,7 @@ int launch_w4_tiles(const W4Call &c, void *workspace, uint32_t *error, cudaStrea
   if ((uint64_t)plan.tiles_w * plan.tiles_x * plan.splits > 0x7fffffffull || c.rows > 0x3fffffffu)
     return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
   uint64_t bytes = 0;
-  const Workspace ws = workspace_at(static_cast<uint8_t *>(workspace), c.rows, weight_rows, c.k, plan, &bytes);
+  const Workspace ws = workspace_at(static_cast<uint8_t *>(workspace), c.rows, weight_rows, c.k, c.group, plan, &bytes);
   const bool zeros = c.w.zeros || c.up.zeros;
   if (c.up.packed) return zeros ? launch_kind<true, true>(c, ws, plan, error, stream) : launch_kind<true, false>(c, ws, plan, error, stream);
   return zeros ? launch_kind<false, true>(c, ws, plan, error, stream) : launch_kind<false, false>(c, ws, plan, error, stream);

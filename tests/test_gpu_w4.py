@@ -76,6 +76,20 @@ def test_gated(pkg, backend, rows, dtype, act):
         plain.check(host(got), *plain.gated(act, x, gate.w, up.w, gate.step(rows, dtype), up.step(rows, dtype)), dtype, f"{rows} x {k} to {n}, groups of {group}")
 
 
+@pytest.mark.parametrize("rows, n, k", [(3, 38000, 160), (14, 39001, 128), (30, 38001, 288), (100, 39000, 256), (129, 20001, 384), (1100, 6001, 512), (520, 20000, 160)])
+def test_more_tiles_than_the_device_takes_at_once(pkg, backend, rows, n, k):
+    """Resident CTAs go from tile to tile, their rings running on."""
+    rng = np.random.default_rng([rows, n])
+    w = Weight(pkg, rng, n, k, 32, zeros=rows % 2 == 0)
+    x = values(rng, (rows, k), "bf16")
+    plain.check(host(pkg.linear_w4(backend, device(x, "bf16"), w.handle)), *plain.product(x, w.w, w.step(rows, "bf16")), "bf16")
+    half = n // 2
+    top, low = (pkg.W4Weight(w.handle.packed[i:i + half].clone(), w.handle.scales[:, i:i + half].contiguous(),
+                             None if w.zeros is None else w.handle.zeros[:, i:i + half].contiguous(), 32) for i in (0, half))
+    step = w.step(rows, "bf16")
+    plain.check(host(pkg.gated_w4(backend, device(x, "bf16"), top, low)), *plain.gated("silu", x, w.w[:half], w.w[half:2 * half], step, step), "bf16")
+
+
 @pytest.mark.parametrize("with_zeros", [False, True])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("n, k, group", [(1, 32, 32), (3, 128, 128), (31, 96, 32), (33, 64, 64), (70, 1120, 32), (257, 4096, 128), (513, 2112, 64)])
