@@ -2,8 +2,8 @@
 // into shared memory.
 //
 // From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05. A pair of CTAs works as one MMA unit on 256 weight rows x
-// up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: a ring of codes is filled by TMA, and teams of warps
-// write the operand tiles of a CTA's 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
+// up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: teams of warps read them into
+// registers, a round of stages ahead, and write the operand tiles of a CTA's 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
 //
 // The operands are f16, not bf16. (code - zero) * scale has at most 11 significant bits with a zero of 8 and 12 with any other, f16 holds 11: products are
 // exact, or off by 2^-12 of a weight, where bf16 would round every weight by 2^-9. Range is no matter, since both sides are scaled by powers of two, every
@@ -14,8 +14,8 @@
 //
 // Where tiles are too few for 74 pairs, k is cut as well: the parts are stored in f32 and summed in order by a third kernel, so results do not vary.
 //
-// Warp 0 loads tokens, 1 of the leader issues the MMAs, then come the dequantising warps, eight of the epilogue, which works under the next tile's main loop,
-// and one that loads codes. Every wait is bounded; one that runs out sets the projections' error word.
+// Warp 0 loads tokens, 1 of the leader issues the MMAs, then come the dequantising warps, eight of the epilogue, which works under the next tile's main loop.
+// Every wait is bounded; one that runs out sets the projections' error word.
 #include "gemm_pair.cuh"
 #include "w4.cuh"
 
@@ -28,16 +28,14 @@ namespace {
 
 using Pair = PairConfig;
 constexpr uint32_t kDequantWarps = 4, kFirstDequant = 2;             // warps that make a stage's weights; as many such teams as the rings have stages
-constexpr uint32_t kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;  // a stage of codes: 64 bytes a row
 
 // CTAS: 1 or 2 that work as an MMA unit on 128 weight rows each; TOKENS: rows of x in a stage of a CTA (a pair's CTAs hold half of a tile's each).
 template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGES>
 struct Form {
   static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTileRows = CTAS * Pair::kRows;
-  static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = STAGES * Pair::kWBytes, kCodeRing = kXRing + STAGES * kXBytes;
-  static constexpr uint32_t kBarriers = kCodeRing + STAGES * kCodeBytes;
+  static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = STAGES * Pair::kWBytes, kBarriers = kXRing + STAGES * kXBytes;
   static constexpr int kSmemBytes = kBarriers + 1024 /*align*/ + 512 /*barriers*/;
-  static constexpr uint32_t kFirstEpilogue = kFirstDequant + STAGES * kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps, kWarps = kCodesWarp + 1;
+  static constexpr uint32_t kFirstEpilogue = kFirstDequant + STAGES * kDequantWarps, kWarps = kFirstEpilogue + Pair::kEpilogueWarps;
   static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
 };
 using Single64 = Form<1, 64, 4>;
@@ -236,9 +234,9 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+__device__ __forceinline__ uint4 ld_codes(const uint8_t *p) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
 __device__ __forceinline__ uint32_t ld_params(const uint32_t *p) {  // in program order, so that a later load does not wait for the stage's arithmetic
@@ -254,17 +252,15 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) 
 
 template <typename F, bool GATED, bool ZEROS>
 __global__ void __launch_bounds__(F::kWarps * 32, 1)
-w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-               const __grid_constant__ CUtensorMap map_up, const Workspace ws, const Plan plan, const uint32_t param_rows, uint32_t *error) {
+w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const Workspace ws, const Plan plan, const uint32_t param_rows, uint32_t *error) {
   constexpr uint32_t kStages = F::kStages, kMatrices = GATED ? 2 : 1;
   constexpr bool kPair = F::kCtas == 2;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint8_t *w_ring = smem, *x_ring = smem + F::kXRing;
-  uint8_t *code_ring = smem + F::kCodeRing;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + F::kBarriers);
-  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2, *code_full = acc_empty + 2, *code_empty = code_full + kStages;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + kStages);
+  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blockIdx.x % F::kCtas, unit = blockIdx.x / F::kCtas, units = gridDim.x / F::kCtas;
@@ -276,8 +272,6 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       // leader: the announcement of the tokens' bytes, its own weights, word of the peer's; peer: its weights
       mbar_init(&full[s], !leader ? kDequantWarps : F::kCtas + kDequantWarps);
       mbar_init(&empty[s], 1);
-      mbar_init(&code_full[s], 1);
-      mbar_init(&code_empty[s], kDequantWarps);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
@@ -394,77 +388,70 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         }
       }
     }
-  } else if (warp == F::kCodesWarp) {
-    // Codes, ahead of everything else: the weights were complete before the first kernel began, whose beginning this one's launch waited for.
-    const bool elected = elect_one();
-    uint32_t it = 0;
-    for (uint32_t t = unit; ok && t < total; t += units) {
-      const Job j = job(t);
-      const int row = (int)((j.w_row + rank * Pair::kRows) / kMatrices);
-      for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
-        const uint32_t s = it % kStages;
-        if (it >= kStages && !wait(&code_empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
-        if (elected) {
-          mbar_arrive_expect_tx(&code_full[s], kCodeBytes);
-          tma_load_2d(code_ring + s * kCodeBytes, &map_w, (int)(kb * kCodeRow), row, &code_full[s]);
-          if (GATED) tma_load_2d(code_ring + s * kCodeBytes + kCodeBytes / 2, &map_up, (int)(kb * kCodeRow), row, &code_full[s]);
-        }
-        __syncwarp();
-      }
-    }
   } else if (warp < F::kFirstEpilogue) {
     // Weights: 32 rows of the CTA's 128 a warp, as four sets of eight; a lane has 32 k (piece) of a row of each. With a gate every other row of a tile is the
-    // gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds both; in the ring of codes the gate's 64 rows come first. What
+    // gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds both. What
     // a stage costs a warp besides its weights counts less with few warps to a stage: each team of four makes the stages of one place in the rings. (With
     // more teams than places one could wait for a barrier that is two phases behind, and two phases are one to a wait.)
     const uint32_t piece = lane & 3, q8 = lane >> 2, team = (warp - kFirstDequant) / kDequantWarps;
     const uint32_t in_tile = (warp - kFirstDequant) % kDequantWarps * 32 + (GATED ? 2 * (q8 & 3) + (q8 >> 2) : q8);
-    const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile;
-    const uint32_t code_from = smem_u32(code_ring) + team * kCodeBytes + code_row * kCodeRow + piece * 16;
     // chunks of 16 bytes are permuted by row & 7; lanes of the upper 64 k take theirs in another order, so that eight lanes meet eight different banks
     constexpr uint32_t kTurn = GATED ? 1 : 2;
     const bool turned = piece >= 2;
     const uint32_t to = smem_u32(w_ring) + team * Pair::kWBytes + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ (turned ? kTurn : 0) ^ (in_tile & 7)) * 16;
     const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
-    pdl_wait();
+    const uint8_t *packed = reinterpret_cast<const uint8_t *>(GATED && (in_tile & 1) ? c.up.packed : c.w.packed);
+    const uint64_t set_step = (uint64_t)c.k / 2 * (8 / kMatrices);
 
-    // Jobs and stages; the next stage's scales and zero points stay as loaded: anything done to them ahead of time would wait for them
+    // Jobs and stages. The next stage of the team's, codes, scales and zero points, is on its way while this one is made; it stays as loaded, since anything
+    // done to it ahead of time would wait for it.
     uint32_t load_t = unit, load_kb = 0, load_end = 0, load_row = 0, next[4];
+    uint4 next_codes[4];
     auto aim = [&] {
       if (load_t >= total) return;
       const Job j = job(load_t);
       load_kb = j.kb, load_end = j.end, load_row = j.w_row + rank * Pair::kRows + in_tile;
+    };
+    auto load_codes = [&] {
+      if (load_t >= total) return;
+      // beyond the last k the codes meet zeros: any do
+      const uint32_t row = load_row / kMatrices, at = min(load_kb * (Pair::kStageK / 2) + piece * 16, c.k / 2 - 16);
+      const uint8_t *p = packed + (uint64_t)row * (c.k / 2) + at;
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) next_codes[i] = row + i * (8 / kMatrices) < c.n ? ld_codes(p + i * set_step) : make_uint4(0, 0, 0, 0);
     };
     auto advance = [&] {
       if (load_t < total && ++load_kb == load_end) load_t += units, aim();
     };
     auto load = [&] {
       if (load_t >= total) return;
-      // beyond the last k the codes meet zeros: any scale does
       const uint32_t *p = ws.params + (uint64_t)min((load_kb * Pair::kStageK + piece * 32) >> group_bits, last_group) * param_rows + load_row;
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) next[i] = ld_params(p + i * 8);
     };
     aim();
     for (uint32_t i = 0; i < team; ++i) advance();
+    load_codes();  // ahead of everything else: the weights were complete before the first kernel began, whose beginning this one's launch waited for
+    pdl_wait();
     load();
     for (uint32_t round = 0; ok && load_t < total; ++round) {
       uint32_t param[4];
+      uint4 codes[4];
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) param[i] = next[i];
+      for (uint32_t i = 0; i < 4; ++i) param[i] = next[i], codes[i] = next_codes[i];
 #pragma unroll
       for (uint32_t i = 0; i < kStages; ++i) advance();
-      if (!wait(&code_full[team], round & 1)) { ok = false; break; }
+      load_codes();
+      load();
       if (round > 0 && !wait(&empty[team], (round & 1) ^ 1)) { ok = false; break; }
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
-        const uint4 codes = lds128(code_from + i * (GATED ? 4 : 8) * kCodeRow);
         const uint32_t low = __byte_perm(param[i], 0, 0x1010), high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
         const uint32_t eight = hmul2(low, 0x80088008u);                                        // -8 * 2^-24 * scale
         const uint32_t zero = __byte_perm(param[i], 0, 0x3232), zero_high = zero << 4;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-          const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+          const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
           const uint32_t word = turned ? words[j ^ kTurn] : words[j], rest = word >> 8;
           uint32_t v[4] = {word & 0x000f000fu, word & 0x00f000f0u, rest & 0x000f000fu, rest & 0x00f000f0u};
 #pragma unroll
@@ -477,11 +464,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&full[team]);
-        mbar_arrive(&code_empty[team]);
-      }
-      load();
+      if (lane == 0) mbar_arrive(&full[team]);
     }
   } else {
     // Epilogue: warp w reads tensor-memory lanes 32 * (w % 4) .. + 31 (lane = weight row, column = token); the two warps of the same lanes take turns, 16
@@ -590,17 +573,15 @@ __global__ void __launch_bounds__(256) w4_sum_kernel(const W4Call c, const float
   static_cast<bf16 *>(c.out)[(uint64_t)m * c.ldo + n] = __float2bfloat16_rn(y);
 }
 
-// [rows][cols] matrix of 16-bit or 8-bit elements, without gaps; boxes of box_cols x box_rows.
-int matrix_map(CUtensorMap *map, CUtensorMapDataType type, uint32_t size, CUtensorMapSwizzle swizzle, const void *base, uint64_t rows, uint64_t cols,
-               uint32_t box_cols, uint32_t box_rows) {
+// [rows][k] f16 matrix without gaps; boxes of 64 k x box_rows.
+int token_map(CUtensorMap *map, const __half *x, uint32_t rows, uint32_t k, uint32_t box_rows) {
   EncodeFn fn = encode_fn();
   if (!fn) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: driver entry point missing");
-  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * size};
-  const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
-  const CUresult r = fn(map, type, 2, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS)
-    return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: encode returned %d (%llu x %llu)", (int)r, (unsigned long long)rows, (unsigned long long)cols);
+  const cuuint64_t dims[2] = {k, rows}, strides[1] = {(cuuint64_t)k * 2};
+  const cuuint32_t box[2] = {Pair::kSlabK, box_rows}, one[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half *>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: encode returned %d (rows %u k %u)", (int)r, rows, k);
   return ORION_OK;
 }
 
@@ -609,16 +590,13 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   static bool done[kMaxDeviceOrdinals] = {};
   ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_tile_kernel<F, GATED, ZEROS>, F::kSmemBytes, done));
   const uint32_t matrices = GATED ? 2 : 1;
-  CUtensorMap map_x, map_w, map_up;
-  ORION_TRY(matrix_map(&map_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, ws.x, c.rows, c.k, Pair::kSlabK, plan.tokens / F::kCtas));
-  ORION_TRY(matrix_map(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_NONE, c.w.packed, c.n, c.k / 2, kCodeRow, Pair::kRows / matrices));
-  map_up = map_w;
-  if (GATED) ORION_TRY(matrix_map(&map_up, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_NONE, c.up.packed, c.n, c.k / 2, kCodeRow, Pair::kRows / 2));
+  CUtensorMap map;
+  ORION_TRY(token_map(&map, ws.x, c.rows, c.k, plan.tokens / F::kCtas));
   const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
   const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), blocks = c.rows + param_rows / 32;
   ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices, param_rows));
   ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(F::kWarps * 32),
-                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, param_rows, error));
+                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map, ws, plan, param_rows, error));
   count_launch();
   count_launch();
   if (plan.splits > 1) {
