@@ -30,16 +30,25 @@ using Pair = PairConfig;
 constexpr uint32_t kDequantWarps = 4, kFirstDequant = 2;             // warps that make a stage's weights; as many such teams as the rings have stages
 
 // CTAS: 1 or 2 that work as an MMA unit on 128 weight rows each; TOKENS: rows of x in a stage of a CTA (a pair's CTAs hold half of a tile's each).
+//
+// Where the accumulators leave room (single CTAs), the weights of a stage go to tensor memory, 64 columns of it: through shared memory they would cost it 64
+// KiB of traffic a stage, 512 cycles, where HBM brings the codes in some 360. Shared memory then holds codes instead, two stages for each team.
 template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGES>
 struct Form {
-  static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTileRows = CTAS * Pair::kRows;
-  static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = STAGES * Pair::kWBytes, kBarriers = kXRing + STAGES * kXBytes;
+  static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTileRows = CTAS * Pair::kRows, kAccCols = CTAS * TOKENS;
+  static constexpr bool kWeightsInTmem = CTAS == 1;
+  static constexpr uint32_t kTmemStage = Pair::kStageK / 2, kTmemWeights = 2 * kAccCols;  // columns
+  static constexpr uint32_t kCodeStages = kWeightsInTmem ? 2 * STAGES : 0, kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;
+  static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = kWeightsInTmem ? 0 : STAGES * Pair::kWBytes;
+  static constexpr uint32_t kCodeRing = kXRing + STAGES * kXBytes, kBarriers = kCodeRing + kCodeStages * kCodeBytes;
   static constexpr int kSmemBytes = kBarriers + 1024 /*align*/ + 512 /*barriers*/;
-  static constexpr uint32_t kFirstEpilogue = kFirstDequant + STAGES * kDequantWarps, kWarps = kFirstEpilogue + Pair::kEpilogueWarps;
+  static constexpr uint32_t kFirstEpilogue = kFirstDequant + STAGES * kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
+  static constexpr uint32_t kWarps = kCodesWarp + (kWeightsInTmem ? 1 : 0);
   static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
+  static_assert(kTmemWeights + (kWeightsInTmem ? STAGES * kTmemStage : 0) <= Pair::kTmemCols, "weights and accumulators exceed tensor memory");
 };
 using Single64 = Form<1, 64, 4>;
-using Single128 = Form<1, 128, 3>;
+using Single128 = Form<1, 128, 4>;
 using Paired = Form<2, 128, 3>;
 constexpr uint32_t kSms = 2 * kPairs;
 constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to
@@ -234,6 +243,38 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
   asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+// A from tensor memory (128 rows, 16 k in eight columns), B from shared memory
+__device__ __forceinline__ void umma_tmem_a(uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 codes of a row, all of one group, as sixteen pairs in f16: (code - zero) * scale * 2^-24
+template <bool ZEROS>
+__device__ __forceinline__ void dequant_piece(uint4 codes, uint32_t param, uint32_t *v) {
+  const uint32_t low = __byte_perm(param, 0, 0x1010), high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
+  const uint32_t eight = hmul2(low, 0x80088008u);                                     // -8 * 2^-24 * scale
+  const uint32_t zero = __byte_perm(param, 0, 0x3232), zero_high = zero << 4;
+  const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    const uint32_t rest = words[j] >> 8;
+    const uint32_t pairs[4] = {words[j] & 0x000f000fu, words[j] & 0x00f000f0u, rest & 0x000f000fu, rest & 0x00f000f0u};
+#pragma unroll
+    for (uint32_t q = 0; q < 4; ++q) {
+      if (ZEROS) v[4 * j + q] = hmul2(hsub2(pairs[q], q & 1 ? zero_high : zero), q & 1 ? high : low);
+      else v[4 * j + q] = hfma2(pairs[q], q & 1 ? high : low, eight);
+    }
+  }
+}
 __device__ __forceinline__ uint4 ld_codes(const uint8_t *p) {
   uint4 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
@@ -252,15 +293,16 @@ __device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) 
 
 template <typename F, bool GATED, bool ZEROS>
 __global__ void __launch_bounds__(F::kWarps * 32, 1)
-w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const Workspace ws, const Plan plan, const uint32_t param_rows, uint32_t *error) {
+w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+               const __grid_constant__ CUtensorMap map_up, const Workspace ws, const Plan plan, const uint32_t param_rows, uint32_t *error) {
   constexpr uint32_t kStages = F::kStages, kMatrices = GATED ? 2 : 1;
   constexpr bool kPair = F::kCtas == 2;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
   uint8_t *w_ring = smem, *x_ring = smem + F::kXRing;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + F::kBarriers);
-  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+  uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2, *code_full = acc_empty + 2, *code_empty = code_full + F::kCodeStages;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + F::kCodeStages);
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blockIdx.x % F::kCtas, unit = blockIdx.x / F::kCtas, units = gridDim.x / F::kCtas;
@@ -276,6 +318,10 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], F::kCtas * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
+    }
+    for (uint32_t s = 0; s < F::kCodeStages; ++s) {
+      mbar_init(&code_full[s], 1);
+      mbar_init(&code_empty[s], kDequantWarps);
     }
     mbar_fence_init();
   }
@@ -350,7 +396,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       uint32_t it = 0, turn = 0;
       for (uint32_t t = unit; ok && t < total; t += units, ++turn) {
         const Job j = job(t);
-        const uint32_t id = idesc_f16(F::kTileRows, j.cols), buf = turn & 1, acc = tmem_base + buf * Pair::kMaxTokens;
+        const uint32_t id = idesc_f16(F::kTileRows, j.cols), buf = turn & 1, acc = tmem_base + buf * F::kAccCols;
         if (!wait(&acc_empty[buf], ((turn >> 1) & 1) ^ 1)) { ok = false; break; }
         tc_fence_after();
         for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
@@ -366,7 +412,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
                 const uint64_t a_at = a + ((h * Pair::kWSlab + k * 32) >> 4), b_at = b + ((h * F::kXSlab + k * 32) >> 4);
                 const uint32_t more = kb > j.kb || h > 0 || k > 0 ? 1u : 0u;
                 if constexpr (kPair) umma_bf16_pair(acc, a_at, b_at, id, more);
-                else umma_bf16(acc, a_at, b_at, id, more);
+                else umma_tmem_a(acc, tmem_base + F::kTmemWeights + s * F::kTmemStage + (h * (Pair::kSlabK / 16) + k) * 8, b_at, id, more);
               }
             commit(&empty[s]);
           }
@@ -388,11 +434,90 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         }
       }
     }
-  } else if (warp < F::kFirstEpilogue) {
-    // Weights: 32 rows of the CTA's 128 a warp, as four sets of eight; a lane has 32 k (piece) of a row of each. With a gate every other row of a tile is the
-    // gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds both. What
-    // a stage costs a warp besides its weights counts less with few warps to a stage: each team of four makes the stages of one place in the rings. (With
-    // more teams than places one could wait for a barrier that is two phases behind, and two phases are one to a wait.)
+  } else if (F::kWeightsInTmem && warp == F::kCodesWarp) {
+    // Codes, ahead of everything else: the weights were complete before the first kernel began, whose beginning this one's launch waited for. With a gate the
+    // 64 rows of the gate's come first, then those of the other matrix.
+    if constexpr (F::kWeightsInTmem) {
+      const bool elected = elect_one();
+      uint32_t it = 0;
+      for (uint32_t t = unit; ok && t < total; t += units) {
+        const Job j = job(t);
+        for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
+          const uint32_t s = it % F::kCodeStages;
+          if (it >= F::kCodeStages && !wait(&code_empty[s], ((it / F::kCodeStages) & 1) ^ 1)) { ok = false; break; }
+          if (elected) {
+            uint8_t *to = smem + F::kCodeRing + s * F::kCodeBytes;
+            mbar_arrive_expect_tx(&code_full[s], F::kCodeBytes);
+            tma_load_2d(to, &map_w, (int)(kb * F::kCodeRow), (int)(j.w_row / kMatrices), &code_full[s]);
+            if (GATED) tma_load_2d(to + F::kCodeBytes / 2, &map_up, (int)(kb * F::kCodeRow), (int)(j.w_row / kMatrices), &code_full[s]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else if (F::kWeightsInTmem && warp < F::kFirstEpilogue) {
+    // Weights to tensor memory: a lane is a row of the tile, a warp the 32 rows whose lanes of tensor memory it may write; it makes the 128 k of a stage for
+    // each in two halves. With a gate every other row of a tile is the gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds
+    // both. What a stage costs a warp besides its weights counts less with few warps to a stage: each team of four makes the stages of one place in the rings.
+    // (With more teams than places one could wait for a barrier that is two phases behind, and two phases are one to a wait.)
+    const uint32_t team = (warp - kFirstDequant) / kDequantWarps, in_tile = (warp & 3) * 32 + lane;
+    const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile, code_turn = (code_row >> 1) & 3;  // how TMA permutes rows of 64 bytes
+    const uint32_t code_from = smem_u32(smem + F::kCodeRing) + team * F::kCodeBytes + code_row * F::kCodeRow;
+    const uint32_t to = tmem_base + (((warp & 3) * 32u) << 16) + F::kTmemWeights + team * F::kTmemStage;
+    const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
+    pdl_wait();
+
+    // Jobs and stages. The scales and zero points of the team's next stage are on their way while this one is made; they stay as loaded, since anything done
+    // to them ahead of time would wait for them.
+    uint32_t load_t = unit, load_kb = 0, load_end = 0, load_row = 0, next[4];
+    auto aim = [&] {
+      if (load_t >= total) return;
+      const Job j = job(load_t);
+      load_kb = j.kb, load_end = j.end, load_row = j.w_row + in_tile;
+    };
+    auto advance = [&] {
+      if (load_t < total && ++load_kb == load_end) load_t += units, aim();
+    };
+    auto load = [&] {
+      if (load_t >= total) return;
+      // beyond the last k the codes meet zeros: any scale does
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i)
+        if (i == 0 || group_bits < 7 - (i & 1 ? 1 : 0))  // one, two or four groups in 128 k
+          next[i] = ld_params(ws.params + (uint64_t)min((load_kb * Pair::kStageK + i * 32) >> group_bits, last_group) * param_rows + load_row);
+    };
+    aim();
+    for (uint32_t i = 0; i < team; ++i) advance();
+    load();
+    for (uint32_t round = 0; ok && load_t < total; ++round) {
+      uint32_t param[4];
+      param[0] = next[0], param[2] = group_bits < 7 ? next[2] : param[0], param[1] = group_bits < 6 ? next[1] : param[0], param[3] = group_bits < 6 ? next[3] : param[2];
+#pragma unroll
+      for (uint32_t i = 0; i < kStages; ++i) advance();
+      const uint32_t slot = round & 1;  // of the team's two in the ring of codes
+      if (!wait(&code_full[team + slot * kStages], (round >> 1) & 1)) { ok = false; break; }
+      uint4 codes[4];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) codes[i] = lds128(code_from + slot * kStages * F::kCodeBytes + ((i ^ code_turn) * 16));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&code_empty[team + slot * kStages]);
+      load();
+      if (round > 0 && !wait(&empty[team], (round & 1) ^ 1)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (uint32_t half = 0; half < 2; ++half) {
+        uint32_t v[32];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) dequant_piece<ZEROS>(codes[half * 2 + i], param[half * 2 + i], &v[i * 16]);
+        tmem_st32(to + half * 32, v);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[team]);
+    }
+  } else if (!F::kWeightsInTmem && warp < F::kFirstEpilogue) {
+    // Weights to shared memory: 32 rows of the CTA's 128 a warp, as four sets of eight; a lane has 32 k (piece) of a row of each. Rows and teams as above.
     const uint32_t piece = lane & 3, q8 = lane >> 2, team = (warp - kFirstDequant) / kDequantWarps;
     const uint32_t in_tile = (warp - kFirstDequant) % kDequantWarps * 32 + (GATED ? 2 * (q8 & 3) + (q8 >> 2) : q8);
     // chunks of 16 bytes are permuted by row & 7; lanes of the upper 64 k take theirs in another order, so that eight lanes meet eight different banks
@@ -446,21 +571,11 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       if (round > 0 && !wait(&empty[team], (round & 1) ^ 1)) { ok = false; break; }
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
-        const uint32_t low = __byte_perm(param[i], 0, 0x1010), high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
-        const uint32_t eight = hmul2(low, 0x80088008u);                                        // -8 * 2^-24 * scale
-        const uint32_t zero = __byte_perm(param[i], 0, 0x3232), zero_high = zero << 4;
+        uint32_t v[16];
+        const uint4 w = codes[i];
+        dequant_piece<ZEROS>(!turned ? w : kTurn == 1 ? make_uint4(w.y, w.x, w.w, w.z) : make_uint4(w.z, w.w, w.x, w.y), param[i], v);
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-          const uint32_t words[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
-          const uint32_t word = turned ? words[j ^ kTurn] : words[j], rest = word >> 8;
-          uint32_t v[4] = {word & 0x000f000fu, word & 0x00f000f0u, rest & 0x000f000fu, rest & 0x00f000f0u};
-#pragma unroll
-          for (uint32_t q = 0; q < 4; ++q) {
-            if (ZEROS) v[q] = hmul2(hsub2(v[q], q & 1 ? zero_high : zero), q & 1 ? high : low);
-            else v[q] = hfma2(v[q], q & 1 ? high : low, eight);
-          }
-          sts128(to + i * 8 * 128 + (chunk ^ (j * 16)), v[0], v[1], v[2], v[3]);
-        }
+        for (uint32_t j = 0; j < 4; ++j) sts128(to + i * 8 * 128 + (chunk ^ (j * 16)), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -473,7 +588,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     uint32_t turn = 0;
     for (uint32_t t = unit; ok && t < total; t += units, ++turn) {
       const Job j = job(t);
-      const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * Pair::kMaxTokens;
+      const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * F::kAccCols;
       const uint32_t r = j.w_row + rank * Pair::kRows + (warp & 3) * 32 + lane, row = GATED ? r >> 1 : r;
       const bool inside = row < c.n;
       const float row_unit = ws.w_unit[r];
@@ -573,15 +688,16 @@ __global__ void __launch_bounds__(256) w4_sum_kernel(const W4Call c, const float
   static_cast<bf16 *>(c.out)[(uint64_t)m * c.ldo + n] = __float2bfloat16_rn(y);
 }
 
-// [rows][k] f16 matrix without gaps; boxes of 64 k x box_rows.
-int token_map(CUtensorMap *map, const __half *x, uint32_t rows, uint32_t k, uint32_t box_rows) {
+// [rows][cols] matrix of f16 values or of bytes, without gaps; boxes of box_cols x box_rows.
+int matrix_map(CUtensorMap *map, bool bytes, CUtensorMapSwizzle swizzle, const void *base, uint64_t rows, uint64_t cols, uint32_t box_cols, uint32_t box_rows) {
   EncodeFn fn = encode_fn();
   if (!fn) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: driver entry point missing");
-  const cuuint64_t dims[2] = {k, rows}, strides[1] = {(cuuint64_t)k * 2};
-  const cuuint32_t box[2] = {Pair::kSlabK, box_rows}, one[2] = {1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<__half *>(x), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: encode returned %d (rows %u k %u)", (int)r, rows, k);
+  const cuuint64_t dims[2] = {cols, rows}, strides[1] = {cols * (bytes ? 1 : 2)};
+  const cuuint32_t box[2] = {box_cols, box_rows}, one[2] = {1, 1};
+  const CUresult r = fn(map, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(base), dims, strides, box, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return set_error(ORION_ERR_BACKEND, "backend cuda failed at tensor map: encode returned %d (%llu x %llu)", (int)r, (unsigned long long)rows, (unsigned long long)cols);
   return ORION_OK;
 }
 
@@ -590,13 +706,18 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   static bool done[kMaxDeviceOrdinals] = {};
   ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_tile_kernel<F, GATED, ZEROS>, F::kSmemBytes, done));
   const uint32_t matrices = GATED ? 2 : 1;
-  CUtensorMap map;
-  ORION_TRY(token_map(&map, ws.x, c.rows, c.k, plan.tokens / F::kCtas));
+  CUtensorMap map_x, map_w, map_up;
+  ORION_TRY(matrix_map(&map_x, false, CU_TENSOR_MAP_SWIZZLE_128B, ws.x, c.rows, c.k, Pair::kSlabK, plan.tokens / F::kCtas));
+  map_w = map_up = map_x;
+  if (F::kWeightsInTmem) {
+    ORION_TRY(matrix_map(&map_w, true, CU_TENSOR_MAP_SWIZZLE_64B, c.w.packed, c.n, c.k / 2, F::kCodeRow, Pair::kRows / matrices));
+    if (GATED) ORION_TRY(matrix_map(&map_up, true, CU_TENSOR_MAP_SWIZZLE_64B, c.up.packed, c.n, c.k / 2, F::kCodeRow, Pair::kRows / 2));
+  }
   const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
   const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), blocks = c.rows + param_rows / 32;
   ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices, param_rows));
   ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(F::kWarps * 32),
-                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map, ws, plan, param_rows, error));
+                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, param_rows, error));
   count_launch();
   count_launch();
   if (plan.splits > 1) {
