@@ -33,23 +33,24 @@ constexpr uint32_t kDequantWarps = 4, kFirstDequant = 2;             // warps th
 //
 // Where the accumulators leave room (single CTAs), the weights of a stage go to tensor memory, 64 columns of it: through shared memory they would cost it 64
 // KiB of traffic a stage, 512 cycles, where HBM brings the codes in some 360. Shared memory then holds codes instead, two stages for each team.
-template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGES>
+template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGES, uint32_t TEAMS>
 struct Form {
-  static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTileRows = CTAS * Pair::kRows, kAccCols = CTAS * TOKENS;
+  static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTeams = TEAMS, kTileRows = CTAS * Pair::kRows, kAccCols = CTAS * TOKENS;
   static constexpr bool kWeightsInTmem = CTAS == 1;
   static constexpr uint32_t kTmemStage = Pair::kStageK / 2, kTmemWeights = 2 * kAccCols;  // columns
-  static constexpr uint32_t kCodeStages = kWeightsInTmem ? 2 * STAGES : 0, kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;
+  static constexpr uint32_t kCodeStages = kWeightsInTmem ? 2 * TEAMS : 0, kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;
   static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = kWeightsInTmem ? 0 : STAGES * Pair::kWBytes;
   static constexpr uint32_t kCodeRing = kXRing + STAGES * kXBytes, kBarriers = kCodeRing + kCodeStages * kCodeBytes;
   static constexpr int kSmemBytes = kBarriers + 1024 /*align*/ + 512 /*barriers*/;
-  static constexpr uint32_t kFirstEpilogue = kFirstDequant + STAGES * kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
+  static constexpr uint32_t kFirstEpilogue = kFirstDequant + TEAMS * kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
   static constexpr uint32_t kWarps = kCodesWarp + (kWeightsInTmem ? 1 : 0);
+  static_assert(TEAMS <= STAGES, "a team could wait for a barrier that is two phases behind, and two phases are one to a wait");
   static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
   static_assert(kTmemWeights + (kWeightsInTmem ? STAGES * kTmemStage : 0) <= Pair::kTmemCols, "weights and accumulators exceed tensor memory");
 };
-using Single64 = Form<1, 64, 4>;
-using Single128 = Form<1, 128, 4>;
-using Paired = Form<2, 128, 3>;
+using Single64 = Form<1, 64, 6, 4>;
+using Single128 = Form<1, 128, 4, 4>;
+using Paired = Form<2, 128, 3, 3>;
 constexpr uint32_t kSms = 2 * kPairs;
 constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to
 static_assert(Pair::kStageK == 128, "a stage is four pieces of 32 k");
@@ -319,7 +320,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], F::kCtas * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
     }
-    for (uint32_t s = 0; s < F::kCodeStages; ++s) {
+    for (uint32_t s = 0; F::kWeightsInTmem && s < F::kCodeStages; ++s) {
       mbar_init(&code_full[s], 1);
       mbar_init(&code_empty[s], kDequantWarps);
     }
@@ -458,12 +459,11 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
   } else if (F::kWeightsInTmem && warp < F::kFirstEpilogue) {
     // Weights to tensor memory: a lane is a row of the tile, a warp the 32 rows whose lanes of tensor memory it may write; it makes the 128 k of a stage for
     // each in two halves. With a gate every other row of a tile is the gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds
-    // both. What a stage costs a warp besides its weights counts less with few warps to a stage: each team of four makes the stages of one place in the rings.
-    // (With more teams than places one could wait for a barrier that is two phases behind, and two phases are one to a wait.)
+    // both. What a stage costs a warp besides its weights counts less with few warps to a stage: teams of four take turns.
     const uint32_t team = (warp - kFirstDequant) / kDequantWarps, in_tile = (warp & 3) * 32 + lane;
     const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile, code_turn = (code_row >> 1) & 3;  // how TMA permutes rows of 64 bytes
-    const uint32_t code_from = smem_u32(smem + F::kCodeRing) + team * F::kCodeBytes + code_row * F::kCodeRow;
-    const uint32_t to = tmem_base + (((warp & 3) * 32u) << 16) + F::kTmemWeights + team * F::kTmemStage;
+    const uint32_t code_from = smem_u32(smem + F::kCodeRing) + code_row * F::kCodeRow;
+    const uint32_t to = tmem_base + (((warp & 3) * 32u) << 16) + F::kTmemWeights;
     const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
     pdl_wait();
 
@@ -493,28 +493,28 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       uint32_t param[4];
       param[0] = next[0], param[2] = group_bits < 7 ? next[2] : param[0], param[1] = group_bits < 6 ? next[1] : param[0], param[3] = group_bits < 6 ? next[3] : param[2];
 #pragma unroll
-      for (uint32_t i = 0; i < kStages; ++i) advance();
-      const uint32_t slot = round & 1;  // of the team's two in the ring of codes
-      if (!wait(&code_full[team + slot * kStages], (round >> 1) & 1)) { ok = false; break; }
+      for (uint32_t i = 0; i < F::kTeams; ++i) advance();
+      const uint32_t it = team + round * F::kTeams, s = it % kStages, cs = it % F::kCodeStages;
+      if (!wait(&code_full[cs], (it / F::kCodeStages) & 1)) { ok = false; break; }
       uint4 codes[4];
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) codes[i] = lds128(code_from + slot * kStages * F::kCodeBytes + ((i ^ code_turn) * 16));
+      for (uint32_t i = 0; i < 4; ++i) codes[i] = lds128(code_from + cs * F::kCodeBytes + ((i ^ code_turn) * 16));
       __syncwarp();
-      if (lane == 0) mbar_arrive(&code_empty[team + slot * kStages]);
+      if (lane == 0) mbar_arrive(&code_empty[cs]);
       load();
-      if (round > 0 && !wait(&empty[team], (round & 1) ^ 1)) { ok = false; break; }
+      if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
       tc_fence_after();
 #pragma unroll
       for (uint32_t half = 0; half < 2; ++half) {
         uint32_t v[32];
 #pragma unroll
         for (uint32_t i = 0; i < 2; ++i) dequant_piece<ZEROS>(codes[half * 2 + i], param[half * 2 + i], &v[i * 16]);
-        tmem_st32(to + half * 32, v);
+        tmem_st32(to + s * F::kTmemStage + half * 32, v);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[team]);
+      if (lane == 0) mbar_arrive(&full[s]);
     }
   } else if (!F::kWeightsInTmem && warp < F::kFirstEpilogue) {
     // Weights to shared memory: 32 rows of the CTA's 128 a warp, as four sets of eight; a lane has 32 k (piece) of a row of each. Rows and teams as above.
@@ -523,7 +523,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     // chunks of 16 bytes are permuted by row & 7; lanes of the upper 64 k take theirs in another order, so that eight lanes meet eight different banks
     constexpr uint32_t kTurn = GATED ? 1 : 2;
     const bool turned = piece >= 2;
-    const uint32_t to = smem_u32(w_ring) + team * Pair::kWBytes + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ (turned ? kTurn : 0) ^ (in_tile & 7)) * 16;
+    const uint32_t to = smem_u32(w_ring) + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ (turned ? kTurn : 0) ^ (in_tile & 7)) * 16;
     const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
     const uint8_t *packed = reinterpret_cast<const uint8_t *>(GATED && (in_tile & 1) ? c.up.packed : c.w.packed);
     const uint64_t set_step = (uint64_t)c.k / 2 * (8 / kMatrices);
@@ -565,21 +565,22 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) param[i] = next[i], codes[i] = next_codes[i];
 #pragma unroll
-      for (uint32_t i = 0; i < kStages; ++i) advance();
+      for (uint32_t i = 0; i < F::kTeams; ++i) advance();
       load_codes();
       load();
-      if (round > 0 && !wait(&empty[team], (round & 1) ^ 1)) { ok = false; break; }
+      const uint32_t it = team + round * F::kTeams, s = it % kStages;
+      if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
         uint32_t v[16];
         const uint4 w = codes[i];
         dequant_piece<ZEROS>(!turned ? w : kTurn == 1 ? make_uint4(w.y, w.x, w.w, w.z) : make_uint4(w.z, w.w, w.x, w.y), param[i], v);
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) sts128(to + i * 8 * 128 + (chunk ^ (j * 16)), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        for (uint32_t j = 0; j < 4; ++j) sts128(to + s * Pair::kWBytes + i * 8 * 128 + (chunk ^ (j * 16)), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&full[team]);
+      if (lane == 0) mbar_arrive(&full[s]);
     }
   } else {
     // Epilogue: warp w reads tensor-memory lanes 32 * (w % 4) .. + 31 (lane = weight row, column = token); the two warps of the same lanes take turns, 16
