@@ -111,96 +111,118 @@ Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint3
 
 // ---- first kernel: tokens to f16, exponents of tokens and of weight rows ------------------------
 
-constexpr uint32_t kPrepThreads = 256, kHeld = 8;
+constexpr uint32_t kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
 
-__global__ void __launch_bounds__(kPrepThreads)
-w4_prepare_kernel(const W4Call c, const Workspace ws, uint32_t matrices, uint32_t param_rows) {
-  pdl_wait();
-  pdl_trigger();  // after the wait: what the next kernel reads ahead of its own wait was complete before this one began
-  if (blockIdx.x >= c.rows) {
-    // 32 weight rows, their groups dealt to eight warps
-    constexpr uint32_t kMine = 8;
-    __shared__ uint32_t tops[kPrepThreads / 32][32];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = (blockIdx.x - c.rows) * 32 + lane, row = r / matrices, groups = c.k / c.group;
-    const W4View &w = r % matrices ? c.up : c.w;
-    const bool there = row < c.n;
-    uint32_t held[kMine], top = 0;
-    auto scale_of = [&](uint32_t g) { return there && g < groups ? (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(w.scales) + (uint64_t)g * c.n + row) : 0u; };
-    auto larger = [&](uint32_t p) {
-      const uint32_t e = p >> 7 & 255u;
-      top = max(top, e == 255u ? 0u : e);
-    };
+// 32 weight rows, their groups dealt to eight warps; sixteen groups of a thread's are on their way together.
+__device__ __forceinline__ void prepare_weights(const W4Call &c, const Workspace &ws, uint32_t matrices, uint32_t param_rows, uint32_t block) {
+  constexpr uint32_t kAtOnce = 16;
+  __shared__ uint32_t tops[kPrepWarps][32];
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = block * 32 + lane, row = r / matrices, groups = c.k / c.group;
+  const W4View &w = r % matrices ? c.up : c.w;
+  const bool there = row < c.n, zeros = there && w.zeros;
+  uint32_t scale[kAtOnce], zero[kAtOnce], top = 0;
+  auto load = [&](uint32_t first) {
 #pragma unroll
-    for (uint32_t j = 0; j < kMine; ++j) held[j] = scale_of(warp + j * 8);
-#pragma unroll
-    for (uint32_t j = 0; j < kMine; ++j) larger(held[j]);
-    for (uint32_t g = warp + kMine * 8; g < groups; g += 8) larger(scale_of(g));
-    tops[warp][lane] = top;
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < kPrepThreads / 32; ++i) top = max(top, tops[i][lane]);
-    const int32_t raise = top ? kTop + 127 - (int32_t)top : 0;
-    auto store = [&](uint32_t g, uint32_t p) {
-      if (g >= groups) return;
-      const uint32_t e = p >> 7 & 255u;
-      // infinities and NaN stay, what is far below the row's largest scale vanishes
-      const uint32_t f = e == 255u ? p << 16 : (int32_t)e + raise <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise << 23);
-      const uint32_t zero = there && w.zeros ? __ldg(w.zeros + (uint64_t)g * c.n + row) : 8u;
-      ws.params[(uint64_t)g * param_rows + r] = (uint32_t)__half_as_ushort(__float2half_rn(__uint_as_float(f))) | zero << 16;
-    };
-#pragma unroll
-    for (uint32_t j = 0; j < kMine; ++j) store(warp + j * 8, held[j]);
-    for (uint32_t g = warp + kMine * 8; g < groups; g += 8) store(g, scale_of(g));
-    if (warp == 0) ws.w_unit[r] = top ? __uint_as_float(top << 23) : 1.f;
-    return;
-  }
-  const uint32_t m = blockIdx.x, pieces = c.k / 8;
-  const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const bf16 *>(c.x) + (uint64_t)m * c.ldx);
-  uint4 held[kHeld];
-  uint32_t top = 0;  // the largest finite magnitude's bits
-  auto largest = [&](const uint4 &v) {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t lo = u[i] & 0x7fffu, hi = u[i] >> 16 & 0x7fffu;
-      top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+    for (uint32_t j = 0; j < kAtOnce; ++j) {
+      const uint32_t g = first + j * kPrepWarps;
+      const uint64_t at = (uint64_t)g * c.n + row;
+      scale[j] = there && g < groups ? (uint32_t)__ldg(reinterpret_cast<const uint16_t *>(w.scales) + at) : 0u;
+      zero[j] = 8;
+      if (zeros && g < groups) zero[j] = __ldg(w.zeros + at);
     }
   };
+  for (uint32_t first = warp; first < groups; first += kAtOnce * kPrepWarps) {
+    load(first);
 #pragma unroll
-  for (uint32_t j = 0; j < kHeld; ++j) {
-    const uint32_t i = threadIdx.x + j * kPrepThreads;
-    held[j] = i < pieces ? __ldg(x + i) : make_uint4(0, 0, 0, 0);
+    for (uint32_t j = 0; j < kAtOnce; ++j) {
+      const uint32_t e = scale[j] >> 7 & 255u;
+      top = max(top, e == 255u ? 0u : e);
+    }
   }
-#pragma unroll
-  for (uint32_t j = 0; j < kHeld; ++j) largest(held[j]);
-  for (uint32_t i = threadIdx.x + kHeld * kPrepThreads; i < pieces; i += kPrepThreads) largest(__ldg(x + i));
-  __shared__ uint32_t tops[kPrepThreads / 32];
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  tops[warp][lane] = top;
   __syncthreads();
 #pragma unroll
-  for (uint32_t i = 0; i < kPrepThreads / 32; ++i) top = max(top, tops[i]);
+  for (uint32_t i = 0; i < kPrepWarps; ++i) top = max(top, tops[i][lane]);
+  const int32_t raise = top ? kTop + 127 - (int32_t)top : 0;
+  for (uint32_t first = warp; first < groups; first += kAtOnce * kPrepWarps) {
+    if (groups > kAtOnce * kPrepWarps) load(first);  // else they are still there
+#pragma unroll
+    for (uint32_t j = 0; j < kAtOnce; ++j) {
+      const uint32_t g = first + j * kPrepWarps, p = scale[j], e = p >> 7 & 255u;
+      // infinities and NaN stay, what is far below the row's largest scale vanishes
+      const uint32_t f = e == 255u ? p << 16 : (int32_t)e + raise <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise << 23);
+      if (g < groups) ws.params[(uint64_t)g * param_rows + r] = (uint32_t)__half_as_ushort(__float2half_rn(__uint_as_float(f))) | zero[j] << 16;
+    }
+  }
+  if (warp == 0) ws.w_unit[r] = top ? __uint_as_float(top << 23) : 1.f;
+}
+
+// A token, by THREADS threads (a block or a warp), HELD pieces of eight values each in registers.
+template <uint32_t THREADS, uint32_t HELD>
+__device__ __forceinline__ void prepare_token(const W4Call &c, const Workspace &ws, uint32_t m) {
+  const uint32_t thread = threadIdx.x % THREADS, pieces = c.k / 8;
+  const uint4 *x = reinterpret_cast<const uint4 *>(static_cast<const bf16 *>(c.x) + (uint64_t)m * c.ldx);
+  uint4 held[HELD];
+  uint32_t top = 0;  // the largest finite magnitude's bits
+  auto load = [&](uint32_t first) {
+#pragma unroll
+    for (uint32_t j = 0; j < HELD; ++j) held[j] = first + j * THREADS < pieces ? __ldg(x + first + j * THREADS) : make_uint4(0, 0, 0, 0);
+  };
+  for (uint32_t first = thread; first < pieces; first += HELD * THREADS) {
+    load(first);
+#pragma unroll
+    for (uint32_t j = 0; j < HELD; ++j) {
+      const uint32_t u[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t lo = u[i] & 0x7fffu, hi = u[i] >> 16 & 0x7fffu;
+        top = max(top, max(lo < 0x7f80u ? lo : 0u, hi < 0x7f80u ? hi : 0u));
+      }
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (THREADS > 32) {
+    __shared__ uint32_t tops[kPrepWarps];
+    if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kPrepWarps; ++i) top = max(top, tops[i]);
+  }
   const int e = top == 0 ? 0 : top >= 0x80u ? (int)(top >> 7) - 127 : 31 - __clz((int)top) - 133, up = kTop - e, half = up / 2;
   // two factors: one alone would not be finite where the token's values are the smallest there are
   const float f0 = __uint_as_float((uint32_t)(half + 127) << 23), f1 = __uint_as_float((uint32_t)(up - half + 127) << 23);
   uint4 *out = reinterpret_cast<uint4 *>(ws.x + (uint64_t)m * c.k);
-  auto convert = [&](const uint4 &v) {
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-    uint32_t r[4];
+  for (uint32_t first = thread; first < pieces; first += HELD * THREADS) {
+    if (pieces > HELD * THREADS) load(first);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(__uint_as_float(u[i] << 16) * f0 * f1, __uint_as_float(u[i] & 0xffff0000u) * f0 * f1);
-      r[i] = *reinterpret_cast<const uint32_t *>(&h);
+    for (uint32_t j = 0; j < HELD; ++j) {
+      const uint32_t u[4] = {held[j].x, held[j].y, held[j].z, held[j].w};
+      uint32_t r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __half2 h = __floats2half2_rn(__uint_as_float(u[i] << 16) * f0 * f1, __uint_as_float(u[i] & 0xffff0000u) * f0 * f1);
+        r[i] = *reinterpret_cast<const uint32_t *>(&h);
+      }
+      if (first + j * THREADS < pieces) out[first + j * THREADS] = make_uint4(r[0], r[1], r[2], r[3]);
     }
-    return make_uint4(r[0], r[1], r[2], r[3]);
-  };
-#pragma unroll
-  for (uint32_t j = 0; j < kHeld; ++j) {
-    const uint32_t i = threadIdx.x + j * kPrepThreads;
-    if (i < pieces) out[i] = convert(held[j]);
   }
-  for (uint32_t i = threadIdx.x + kHeld * kPrepThreads; i < pieces; i += kPrepThreads) out[i] = convert(__ldg(x + i));
-  if (threadIdx.x == 0) ws.x_unit[m] = ldexpf(1.f, e);
+  if (thread == 0) ws.x_unit[m] = ldexpf(1.f, e);
+}
+
+// Blocks 0 .. token_blocks - 1 make tokens, one each or, of many tokens, one a warp: a block to a row is there sooner, a warp to a row needs no barrier and
+// keeps twice as much on the way (2048 x 4096 with the weights of 4096 outputs: 14 us with blocks). The others make weight rows.
+__global__ void __launch_bounds__(kPrepThreads)
+w4_prepare_kernel(const W4Call c, const Workspace ws, uint32_t matrices, uint32_t param_rows, uint32_t token_blocks) {
+  pdl_wait();
+  pdl_trigger();  // after the wait: what the next kernel reads ahead of its own wait was complete before this one began
+  if (blockIdx.x >= token_blocks) {
+    prepare_weights(c, ws, matrices, param_rows, blockIdx.x - token_blocks);
+  } else if (token_blocks == c.rows) {
+    prepare_token<kPrepThreads, 8>(c, ws, blockIdx.x);
+  } else {
+    const uint32_t m = blockIdx.x * kPrepWarps + threadIdx.x / 32;
+    if (m < c.rows) prepare_token<32, 16>(c, ws, m);
+  }
 }
 
 // ---- second kernel: the products ------------------------------------------------------------------
@@ -216,13 +238,18 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
-// mbar_wait for barriers that threads of the other CTA arrive at
-__device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
-  if (mbar_try_wait_cluster(bar, parity)) return true;
-  const uint64_t start = global_timer_ns();
+// As mbar_wait, but the clock is not read before the sixty-fourth poll: a stage has several hand-overs, and reading it takes longer than one. REMOTE: for
+// barriers that threads of the other CTA arrive at.
+template <bool REMOTE>
+__device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity) {
+  uint64_t start = 0;
   for (uint32_t i = 0; i < (1u << 30); ++i) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if ((i & 63u) == 63u && global_timer_ns() - start > 2000000000ull) return false;
+    if (REMOTE ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 63u) {
+      const uint64_t now = global_timer_ns();
+      if (start == 0) start = now;
+      else if (now - start > 2000000000ull) return false;
+    }
   }
   return false;
 }
@@ -320,7 +347,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], F::kCtas * Pair::kEpilogueWarps);  // both CTAs' epilogues (used in the leader)
     }
-    for (uint32_t s = 0; F::kWeightsInTmem && s < F::kCodeStages; ++s) {
+    for (uint32_t s = 0; s < F::kCodeStages; ++s) {
       mbar_init(&code_full[s], 1);
       mbar_init(&code_empty[s], kDequantWarps);
     }
@@ -346,7 +373,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
   const uint32_t tmem_base = *tmem_slot;
   bool ok = true;
   auto wait = [](uint64_t *bar, uint32_t parity) {  // one answer for a warp
-    return (bool)__all_sync(0xffffffffu, kPair ? mbar_wait_cluster(bar, parity) : mbar_wait(bar, parity));
+    return (bool)__all_sync(0xffffffffu, wait_for<kPair>(bar, parity));
   };
   auto commit = [](uint64_t *bar) {  // on this barrier in all CTAs of the unit, once the MMAs issued so far have ended
     if constexpr (kPair) umma_commit_both(bar);
@@ -715,8 +742,8 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
     if (GATED) ORION_TRY(matrix_map(&map_up, true, CU_TENSOR_MAP_SWIZZLE_64B, c.up.packed, c.n, c.k / 2, F::kCodeRow, Pair::kRows / 2));
   }
   const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
-  const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), blocks = c.rows + param_rows / 32;
-  ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(blocks), dim3(kPrepThreads), 0, stream, c, ws, matrices, param_rows));
+  const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), token_blocks = c.rows > 512 ? (c.rows + kPrepWarps - 1) / kPrepWarps : c.rows;
+  ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(token_blocks + param_rows / 32), dim3(kPrepThreads), 0, stream, c, ws, matrices, param_rows, token_blocks));
   ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(F::kWarps * 32),
                                                        dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, param_rows, error));
   count_launch();
