@@ -68,7 +68,7 @@ int check_product(int dtype, const void *x, uint64_t rows, uint64_t x_stride, co
 
 // The tiles of tcgen05 take bf16 products of more rows than this, and of at least a stage of k.
 constexpr uint64_t kFewRows = 16;
-bool takes_tiles(int dtype, uint64_t rows, uint64_t k) { return dtype == ORION_DTYPE_BF16 && rows > kFewRows && k >= 128; }
+bool takes_tiles(int dtype, uint64_t rows, uint64_t k) { return dtype == ORION_DTYPE_BF16 && rows > kFewRows && k >= 256; }
 
 // Address of the projections' error word, looked up once per device.
 int error_word(int device, uint32_t **word) {

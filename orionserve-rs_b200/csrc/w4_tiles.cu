@@ -33,27 +33,28 @@ constexpr uint32_t kDequantWarps = 4, kFirstDequant = 2;             // warps th
 //
 // Where the accumulators leave room (single CTAs), the weights of a stage go to tensor memory, 64 columns of it: through shared memory they would cost it 64
 // KiB of traffic a stage, 512 cycles, where HBM brings the codes in some 360. Shared memory then holds codes instead, two stages for each team.
-template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGES, uint32_t TEAMS>
+template <uint32_t CTAS, uint32_t TOKENS, uint32_t STAGE_K, uint32_t STAGES>
 struct Form {
-  static constexpr uint32_t kCtas = CTAS, kTokens = TOKENS, kStages = STAGES, kTeams = TEAMS, kTileRows = CTAS * Pair::kRows, kAccCols = CTAS * TOKENS;
+  static constexpr uint32_t kCtas = CTAS, kStages = STAGES, kTeams = STAGES, kStageK = STAGE_K, kTileRows = CTAS * Pair::kRows, kAccCols = CTAS * TOKENS;
   static constexpr bool kWeightsInTmem = CTAS == 1;
-  static constexpr uint32_t kTmemStage = Pair::kStageK / 2, kTmemWeights = 2 * kAccCols;  // columns
-  static constexpr uint32_t kCodeStages = kWeightsInTmem ? 2 * TEAMS : 0, kCodeRow = Pair::kStageK / 2, kCodeBytes = Pair::kRows * kCodeRow;
-  static constexpr uint32_t kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = 2 * kXSlab, kXRing = kWeightsInTmem ? 0 : STAGES * Pair::kWBytes;
+  static constexpr uint32_t kTmemStage = STAGE_K / 2, kTmemWeights = 2 * kAccCols;  // columns
+  static constexpr uint32_t kCodeStages = kWeightsInTmem ? 2 * STAGES : 1, kCodeRow = STAGE_K / 2, kCodeBytes = kWeightsInTmem ? Pair::kRows * kCodeRow : 0;
+  static constexpr uint32_t kSlabs = STAGE_K / Pair::kSlabK, kXSlab = TOKENS * Pair::kSlabK * 2, kXBytes = kSlabs * kXSlab, kXRing = kWeightsInTmem ? 0 : STAGES * Pair::kWBytes;
   static constexpr uint32_t kCodeRing = kXRing + STAGES * kXBytes, kBarriers = kCodeRing + kCodeStages * kCodeBytes;
   static constexpr int kSmemBytes = kBarriers + 1024 /*align*/ + 512 /*barriers*/;
-  static constexpr uint32_t kFirstEpilogue = kFirstDequant + TEAMS * kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
+  static constexpr uint32_t kFirstEpilogue = kFirstDequant + STAGES * kDequantWarps, kCodesWarp = kFirstEpilogue + Pair::kEpilogueWarps;
   static constexpr uint32_t kWarps = kCodesWarp + (kWeightsInTmem ? 1 : 0);
-  static_assert(TEAMS <= STAGES, "a team could wait for a barrier that is two phases behind, and two phases are one to a wait");
+  static_assert(kTeams <= STAGES, "a team could wait for a barrier that is two phases behind, and two phases are one to a wait");
+  static_assert(STAGE_K == 128 || kWeightsInTmem, "the pairs' stages of weights");
   static_assert(kSmemBytes <= 232448, "rings exceed the shared memory of an SM");
   static_assert(kTmemWeights + (kWeightsInTmem ? STAGES * kTmemStage : 0) <= Pair::kTmemCols, "weights and accumulators exceed tensor memory");
 };
-using Single64 = Form<1, 64, 6, 4>;
-using Single128 = Form<1, 128, 4, 4>;
-using Paired = Form<2, 128, 3, 3>;
+// Up to 64 tokens a stage's MMAs take a quarter of what its hand-overs do, and it holds 256 k (64 rows of k 14336 to 18944 outputs: 53 us with 128 k).
+using Single64 = Form<1, 64, 256, 3>;
+using Single128 = Form<1, 128, 128, 4>;
+using Paired = Form<2, 128, 128, 3>;
 constexpr uint32_t kSms = 2 * kPairs;
 constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to
-static_assert(Pair::kStageK == 128, "a stage is four pieces of 32 k");
 
 // What the first kernel leaves for the second, and the parts of k that the third one sums.
 struct Workspace {
@@ -75,14 +76,15 @@ struct Plan {
 Plan make_plan(uint32_t rows, uint32_t weight_rows, uint32_t k) {
   Plan best;
   double cost = 1e300;
-  const uint32_t ctas = rows <= Single128::kTokens ? 1 : 2, units = kSms / ctas;
-  const uint32_t stages = (k + Pair::kStageK - 1) / Pair::kStageK, tiles_w = (weight_rows + ctas * Pair::kRows - 1) / (ctas * Pair::kRows);
+  const uint32_t ctas = rows <= Single128::kAccCols ? 1 : 2, units = kSms / ctas;
+  const uint32_t stage_k = rows <= Single64::kAccCols ? Single64::kStageK : ctas == 1 ? Single128::kStageK : Paired::kStageK;
+  const uint32_t stages = (k + stage_k - 1) / stage_k, tiles_w = (weight_rows + ctas * Pair::kRows - 1) / (ctas * Pair::kRows);
   const uint32_t most = std::min(256u, (rows + 31) / 32 * 32);
   for (uint32_t tokens = most; tokens >= std::min(most, 128u); tokens -= 32) {
     const uint32_t tiles_x = (rows + tokens - 1) / tokens;
     for (uint32_t splits = 1; splits <= 8 && splits <= stages && (splits == 1 || (uint64_t)tiles_w * tiles_x <= 8 * units); ++splits) {
       const uint64_t jobs = (uint64_t)tiles_w * tiles_x * splits, rounds = (jobs + units - 1) / units;
-      double c = (double)rounds * ((stages + splits - 1) / splits * std::max(4.0 * tokens, 450.0) + 3000.0);
+      double c = (double)rounds * ((stages + splits - 1) / splits * std::max(4.0 * tokens, 450.0) * (stage_k / 128) + 3000.0);
       if (splits > 1) c += 4000.0 + (double)splits * rows * weight_rows * 8.0 / 2500.0;
       if (c < cost) cost = c, best = {tokens, splits, tiles_w, tiles_x, stages, ctas};
     }
@@ -113,9 +115,9 @@ Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint3
 
 constexpr uint32_t kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
 
-// 32 weight rows, their groups dealt to eight warps; sixteen groups of a thread's are on their way together.
+// 32 weight rows, their groups dealt to eight warps; eight groups of a thread's are on their way together.
 __device__ __forceinline__ void prepare_weights(const W4Call &c, const Workspace &ws, uint32_t matrices, uint32_t param_rows, uint32_t block) {
-  constexpr uint32_t kAtOnce = 16;
+  constexpr uint32_t kAtOnce = 8;
   __shared__ uint32_t tops[kPrepWarps][32];
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = block * 32 + lane, row = r / matrices, groups = c.k / c.group;
   const W4View &w = r % matrices ? c.up : c.w;
@@ -209,9 +211,9 @@ __device__ __forceinline__ void prepare_token(const W4Call &c, const Workspace &
   if (thread == 0) ws.x_unit[m] = ldexpf(1.f, e);
 }
 
-// Blocks 0 .. token_blocks - 1 make tokens, one each or, of many tokens, one a warp: a block to a row is there sooner, a warp to a row needs no barrier and
-// keeps twice as much on the way (2048 x 4096 with the weights of 4096 outputs: 14 us with blocks). The others make weight rows.
-__global__ void __launch_bounds__(kPrepThreads)
+// Blocks 0 .. token_blocks - 1 make tokens, one each or, of many tokens, one a warp: a block to a row is there sooner, a warp to a row needs no barrier so that more
+// of them are at work (2048 x 4096 with the weights of 4096 outputs: 14 us with blocks). The others make weight rows.
+__global__ void __launch_bounds__(kPrepThreads, 4)
 w4_prepare_kernel(const W4Call c, const Workspace ws, uint32_t matrices, uint32_t param_rows, uint32_t token_blocks) {
   pdl_wait();
   pdl_trigger();  // after the wait: what the next kernel reads ahead of its own wait was complete before this one began
@@ -221,7 +223,7 @@ w4_prepare_kernel(const W4Call c, const Workspace ws, uint32_t matrices, uint32_
     prepare_token<kPrepThreads, 8>(c, ws, blockIdx.x);
   } else {
     const uint32_t m = blockIdx.x * kPrepWarps + threadIdx.x / 32;
-    if (m < c.rows) prepare_token<32, 16>(c, ws, m);
+    if (m < c.rows) prepare_token<32, 8>(c, ws, m);
   }
 }
 
@@ -403,11 +405,11 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         const uint32_t s = it % kStages;
         if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
         if (elected) {
-          if (leader) mbar_arrive_expect_tx(&full[s], F::kCtas * 2 * box * Pair::kSlabK * 2);
+          if (leader) mbar_arrive_expect_tx(&full[s], F::kCtas * F::kSlabs * box * Pair::kSlabK * 2);
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) {
+          for (uint32_t h = 0; h < F::kSlabs; ++h) {
             uint8_t *to = x_ring + s * F::kXBytes + h * F::kXSlab;
-            const int k = (int)(kb * Pair::kStageK + h * Pair::kSlabK), row = (int)(j.x_row + rank * (j.cols / F::kCtas));
+            const int k = (int)(kb * F::kStageK + h * Pair::kSlabK), row = (int)(j.x_row + rank * (j.cols / F::kCtas));
             if constexpr (kPair) tma_load_2d_pair(to, &map_x, k, row, mapa_u32(smem_u32(&full[s]), 0));
             else tma_load_2d(to, &map_x, k, row, &full[s]);
           }
@@ -434,7 +436,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
           if (elected) {
             const uint64_t a = w_desc + s * (Pair::kWBytes >> 4), b = x_desc + s * (F::kXBytes >> 4);
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h)
+            for (uint32_t h = 0; h < F::kSlabs; ++h)
 #pragma unroll
               for (uint32_t k = 0; k < Pair::kSlabK / 16; ++k) {
                 const uint64_t a_at = a + ((h * Pair::kWSlab + k * 32) >> 4), b_at = b + ((h * F::kXSlab + k * 32) >> 4);
@@ -484,11 +486,12 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       }
     }
   } else if (F::kWeightsInTmem && warp < F::kFirstEpilogue) {
-    // Weights to tensor memory: a lane is a row of the tile, a warp the 32 rows whose lanes of tensor memory it may write; it makes the 128 k of a stage for
-    // each in two halves. With a gate every other row of a tile is the gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds
+    // Weights to tensor memory: a lane is a row of the tile, a warp the 32 rows whose lanes of tensor memory it may write; it makes the k of a stage for
+    // each, 64 at a time. With a gate every other row of a tile is the gate's and the next the other matrix's, so that a pair of lanes of the epilogue holds
     // both. What a stage costs a warp besides its weights counts less with few warps to a stage: teams of four take turns.
+    constexpr uint32_t kPieces = F::kStageK / 32;
     const uint32_t team = (warp - kFirstDequant) / kDequantWarps, in_tile = (warp & 3) * 32 + lane;
-    const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile, code_turn = (code_row >> 1) & 3;  // how TMA permutes rows of 64 bytes
+    const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile, code_turn = F::kCodeRow == 128 ? code_row & 7 : (code_row >> 1) & 3;  // how TMA permutes rows of 128 and of 64 bytes
     const uint32_t code_from = smem_u32(smem + F::kCodeRing) + code_row * F::kCodeRow;
     const uint32_t to = tmem_base + (((warp & 3) * 32u) << 16) + F::kTmemWeights;
     const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
@@ -496,7 +499,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
 
     // Jobs and stages. The scales and zero points of the team's next stage are on their way while this one is made; they stay as loaded, since anything done
     // to them ahead of time would wait for them.
-    uint32_t load_t = unit, load_kb = 0, load_end = 0, load_row = 0, next[4];
+    uint32_t load_t = unit, load_kb = 0, load_end = 0, load_row = 0, next[kPieces];
     auto aim = [&] {
       if (load_t >= total) return;
       const Job j = job(load_t);
@@ -509,35 +512,42 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       if (load_t >= total) return;
       // beyond the last k the codes meet zeros: any scale does
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i)
-        if (i == 0 || group_bits < 7 - (i & 1 ? 1 : 0))  // one, two or four groups in 128 k
-          next[i] = ld_params(ws.params + (uint64_t)min((load_kb * Pair::kStageK + i * 32) >> group_bits, last_group) * param_rows + load_row);
+      for (uint32_t i = 0; i < kPieces; ++i)
+        if (i % 4 == 0 || group_bits < 7 - (i & 1 ? 1 : 0))  // one, two or four groups in 128 k
+          next[i] = ld_params(ws.params + (uint64_t)min((load_kb * F::kStageK + i * 32) >> group_bits, last_group) * param_rows + load_row);
     };
     aim();
     for (uint32_t i = 0; i < team; ++i) advance();
     load();
     for (uint32_t round = 0; ok && load_t < total; ++round) {
-      uint32_t param[4];
-      param[0] = next[0], param[2] = group_bits < 7 ? next[2] : param[0], param[1] = group_bits < 6 ? next[1] : param[0], param[3] = group_bits < 6 ? next[3] : param[2];
+      uint32_t param[kPieces];
+#pragma unroll
+      for (uint32_t i = 0; i < kPieces; i += 4) {
+        param[i] = next[i], param[i + 2] = group_bits < 7 ? next[i + 2] : param[i];
+        param[i + 1] = group_bits < 6 ? next[i + 1] : param[i], param[i + 3] = group_bits < 6 ? next[i + 3] : param[i + 2];
+      }
 #pragma unroll
       for (uint32_t i = 0; i < F::kTeams; ++i) advance();
       const uint32_t it = team + round * F::kTeams, s = it % kStages, cs = it % F::kCodeStages;
       if (!wait(&code_full[cs], (it / F::kCodeStages) & 1)) { ok = false; break; }
-      uint4 codes[4];
-#pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) codes[i] = lds128(code_from + cs * F::kCodeBytes + ((i ^ code_turn) * 16));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&code_empty[cs]);
       load();
       if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
       tc_fence_after();
 #pragma unroll
-      for (uint32_t half = 0; half < 2; ++half) {
-        uint32_t v[32];
+      for (uint32_t i0 = 0; i0 < kPieces; i0 += 4) {
+        uint4 codes[4];
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) dequant_piece<ZEROS>(codes[half * 2 + i], param[half * 2 + i], &v[i * 16]);
-        tmem_st32(to + s * F::kTmemStage + half * 32, v);
+        for (uint32_t i = 0; i < 4; ++i) codes[i] = lds128(code_from + cs * F::kCodeBytes + (((i0 + i) ^ code_turn) * 16));
+#pragma unroll
+        for (uint32_t half = 0; half < 2; ++half) {
+          uint32_t v[32];
+#pragma unroll
+          for (uint32_t i = 0; i < 2; ++i) dequant_piece<ZEROS>(codes[half * 2 + i], param[i0 + half * 2 + i], &v[i * 16]);
+          tmem_st32(to + s * F::kTmemStage + (i0 + half * 2) * 16, v);
+        }
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&code_empty[cs]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -737,9 +747,10 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   CUtensorMap map_x, map_w, map_up;
   ORION_TRY(matrix_map(&map_x, false, CU_TENSOR_MAP_SWIZZLE_128B, ws.x, c.rows, c.k, Pair::kSlabK, plan.tokens / F::kCtas));
   map_w = map_up = map_x;
+  constexpr CUtensorMapSwizzle code_swizzle = F::kCodeRow == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   if (F::kWeightsInTmem) {
-    ORION_TRY(matrix_map(&map_w, true, CU_TENSOR_MAP_SWIZZLE_64B, c.w.packed, c.n, c.k / 2, F::kCodeRow, Pair::kRows / matrices));
-    if (GATED) ORION_TRY(matrix_map(&map_up, true, CU_TENSOR_MAP_SWIZZLE_64B, c.up.packed, c.n, c.k / 2, F::kCodeRow, Pair::kRows / 2));
+    ORION_TRY(matrix_map(&map_w, true, code_swizzle, c.w.packed, c.n, c.k / 2, F::kCodeRow, Pair::kRows / matrices));
+    if (GATED) ORION_TRY(matrix_map(&map_up, true, code_swizzle, c.up.packed, c.n, c.k / 2, F::kCodeRow, Pair::kRows / 2));
   }
   const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
   const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), token_blocks = c.rows > 512 ? (c.rows + kPrepWarps - 1) / kPrepWarps : c.rows;
@@ -759,7 +770,7 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
 template <bool GATED, bool ZEROS>
 int launch_kind(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
   if (plan.ctas == 2) return launch_form<Paired, GATED, ZEROS>(c, ws, plan, error, stream);
-  if (plan.tokens > Single64::kTokens) return launch_form<Single128, GATED, ZEROS>(c, ws, plan, error, stream);
+  if (plan.tokens > Single64::kAccCols) return launch_form<Single128, GATED, ZEROS>(c, ws, plan, error, stream);
   return launch_form<Single64, GATED, ZEROS>(c, ws, plan, error, stream);
 }
 
