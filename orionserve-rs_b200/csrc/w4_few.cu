@@ -26,18 +26,15 @@ namespace {
 constexpr uint32_t kThreads = 256, kWarps = 8;
 constexpr float kUnit = 8192.f;        // dequantised codes are multiples of 1 / kUnit
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool some) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(some ? 16u : 0u) : "memory");
-}
-__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void *src, bool some) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(dst), "l"(src), "r"((uint32_t)some) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void sts128_zero(uint32_t addr) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0u) : "memory"); }
 __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((uint16_t)v) : "memory"); }
 __device__ __forceinline__ void sts8(uint32_t addr, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src, uint32_t bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -51,6 +48,12 @@ __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
+}
+template <uint32_t N>
+__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[N]) {
+  if constexpr (N == 1) w[0] = lds32(addr);
+  if constexpr (N == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+  if constexpr (N == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   uint16_t v;
@@ -160,27 +163,42 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
     }
     held_at = 0;
   };
-  auto load_params = [&](uint32_t s_at, uint32_t slab, uint32_t n0) {
+  constexpr uint32_t kScaleTurns = (kRowsOfParams * kScaleWords + WR * 32 - 1) / (WR * 32), kZeroTurns = (kRowsOfParams * kZeroWords + WR * 32 - 1) / (WR * 32);
+  const uint64_t slab_step = (uint64_t)units * kPerSlab * c.n;  // scales from one slab to the next
+  const bf16 *load_s[kScaleTurns];
+  const uint8_t *load_z[kZeroTurns];
+  auto aim_params = [&](uint32_t n0) {
+#pragma unroll
+    for (uint32_t j = 0; j < kScaleTurns; ++j) {
+      const uint32_t i = in_kg + j * WR * 32, row = i / kScaleWords;
+      load_s[j] = (row >= kPerSlab ? c.up.scales : c.w.scales) + (uint64_t)(unit * kPerSlab + row % kPerSlab) * c.n + n0 + i % kScaleWords * 2;
+    }
+#pragma unroll
+    for (uint32_t j = 0; ZEROS && j < kZeroTurns; ++j) {
+      const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords;
+      const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
+      load_z[j] = p ? p + (uint64_t)(unit * kPerSlab + row % kPerSlab) * c.n + n0 + i % kZeroWords * 4 : nullptr;
+    }
+  };
+  auto load_params = [&](uint32_t s_at, uint32_t slab, uint32_t n0, bool whole) {
     if (words) {
 #pragma unroll
-      for (uint32_t j = 0; j < (kRowsOfParams * kScaleWords + WR * 32 - 1) / (WR * 32); ++j) {
-        const uint32_t i = in_kg + j * WR * 32, row = i / kScaleWords, col = i % kScaleWords * 2, group = slab * kPerSlab + row % kPerSlab;
+      for (uint32_t j = 0; j < kScaleTurns; ++j) {
+        const uint32_t i = in_kg + j * WR * 32, row = i / kScaleWords, col = i % kScaleWords * 2;
         if (row < kRowsOfParams) {
-          const bf16 *p = row >= kPerSlab ? c.up.scales : c.w.scales;
-          const bool some = group < groups && n0 + col < c.n;
-          cp_async4(s_at + row * Cfg::kScaleRow + col * 2, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
+          if (whole || (slab * kPerSlab + row % kPerSlab < groups && n0 + col < c.n)) cp_async4(s_at + row * Cfg::kScaleRow + col * 2, load_s[j]);
+          else sts32(s_at + row * Cfg::kScaleRow + col * 2, 0);
         }
+        load_s[j] += slab_step;
       }
 #pragma unroll
-      for (uint32_t j = 0; ZEROS && j < (kRowsOfParams * kZeroWords + WR * 32 - 1) / (WR * 32); ++j) {
-        const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords, col = i % kZeroWords * 4, group = slab * kPerSlab + row % kPerSlab;
-        const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
-        if (row < kRowsOfParams && !p) {
-          sts32(s_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, 0x08080808u);
-        } else if (row < kRowsOfParams) {
-          const bool some = group < groups && n0 + col < c.n;
-          cp_async4(s_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col, some ? p + (uint64_t)group * c.n + n0 + col : p, some ? 4 : 0);
+      for (uint32_t j = 0; ZEROS && j < kZeroTurns; ++j) {
+        const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords, col = i % kZeroWords * 4, at = s_at + kRowsOfParams * Cfg::kScaleRow + row * Cfg::kZeroRow + col;
+        if (row < kRowsOfParams) {
+          if (load_z[j] && (whole || (slab * kPerSlab + row % kPerSlab < groups && n0 + col < c.n))) cp_async4(at, load_z[j]);
+          else sts32(at, 0x08080808u);
         }
+        if (load_z[j]) load_z[j] += slab_step;
       }
     } else {
       held_at = s_at;
@@ -208,9 +226,19 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   static_assert(kXStep % 2 == 0, "rows of a lane's turns are permuted alike");
   constexpr uint32_t kWPieces = kSlab / 32, kWStep = 32 / kWPieces, kWTurns = kTilesPerMatrix * 16 / kWStep;  // rows from one turn to the next, turns per matrix
   const uint32_t w_row = lane / kWPieces, w_piece = lane % kWPieces;
-  // a piece goes to the place at ^ (row & 7) of rows of 128 bytes, at ^ ((row / 2) & 3) of rows of 64; of the former every other turn has row & 4 set
-  const uint32_t w_to = wr * RT * 16 * kWRow + w_row * kWRow + (w_piece ^ (kWPieces == 8 ? w_row : (w_row >> 1) & 3)) * 16;
-  const uint32_t x_row = in_kg / kPieces, x_piece = in_kg % kPieces, x_to = Cfg::kWStage + x_row * Cfg::kXRow + (x_piece ^ ((x_row & 1) << 2)) * 16;
+  // Where a piece goes within its row, so that the rows that are read together lie in different banks: eight of them 4 bytes a lane (f32, groups of 32),
+  // four 8 bytes (64), two 16 bytes (128). Of rows of 128 bytes every other turn has row & 4 set.
+  constexpr uint32_t kWide = kF32 ? 1 : GROUP / 32, kBlock = 32 * kWide;  // words of a row that a lane takes together, k of the four lanes of a row
+  auto w_place = [](uint32_t piece, uint32_t row) {
+    if (kWPieces == 8) return piece ^ (kWide == 1 ? row & 7 : kWide == 2 ? (row & 3) << 1 : (row & 1) << 2);
+    return piece ^ (kWide == 1 ? (row >> 1) & 3 : kWide == 2 ? row & 2 : 0);
+  };
+  const uint32_t w_to = wr * RT * 16 * kWRow + w_row * kWRow;
+  const uint32_t w_to_places[2] = {w_to + w_place(w_piece, w_row) * 16, w_to + w_place(w_piece, w_row + kWStep) * 16};
+  auto x_place = [](uint32_t piece, uint32_t row) {  // likewise: lanes read pieces kWide apart, of two rows together
+    return piece ^ (kWide == 1 ? (row & 1) << 2 : row & 1) ^ (kWide == 4 ? (piece >> 3 & 1) << 1 : 0);
+  };
+  const uint32_t x_row = in_kg / kPieces, x_piece = in_kg % kPieces, x_to = Cfg::kWStage + x_row * Cfg::kXRow + x_place(x_piece, x_row) * 16;
   const uint64_t w_step = (uint64_t)c.k / 2 * kWStep, x_step = kXStep * c.ldx * sizeof(T);  // bytes
   uint32_t load_tile = blockIdx.x, load_index = 0, load_slot = 0, load_n0 = 0, load_tokens = 0, load_rows = 0;
   const uint8_t *load_w[Cfg::kMatrices] = {}, *load_x = nullptr;
@@ -221,6 +249,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
         load_n0 = load_tile / tiles_m * Cfg::kOutputs;
         const uint32_t m0 = load_tile % tiles_m * Cfg::kTokens, row = load_n0 + wr * kTilesPerMatrix * 16 + w_row;
         load_tokens = min(Cfg::kTokens, c.rows - m0);
+        aim_params(load_n0);
         load_rows = row < c.n ? (c.n - row + kWStep - 1) / kWStep : 0;  // of this lane's, per matrix
         const uint64_t at = ((uint64_t)row * (c.k / 8) + unit * (kSlab / 8) + w_piece * 4) * 4;
         load_w[0] = reinterpret_cast<const uint8_t *>(c.w.packed) + at;
@@ -228,11 +257,16 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
         load_x = static_cast<const uint8_t *>(c.x) + ((uint64_t)(m0 + x_row) * c.ldx + unit * kSlab + x_piece * kPer) * sizeof(T);
       }
       const uint32_t slab = unit + load_index * units, k0 = slab * kSlab, base = ring + load_slot * kStageBytes;
-      const uint32_t rows = k0 + w_piece * 32 < c.k ? load_rows : 0;
+      const uint32_t to[2] = {base + w_to_places[0], base + w_to_places[1]};
+      const bool whole = load_n0 + Cfg::kOutputs <= c.n && k0 + kSlab <= c.k;
+      if (whole) {
 #pragma unroll
-      for (uint32_t i = 0; i < Cfg::kMatrices * kWTurns; ++i) {
-        const uint32_t m = i / kWTurns, r = i % kWTurns, to = base + (kWPieces == 8 && r % 2 ? w_to ^ 64 : w_to);
-        cp_async16_if(to + i * kWStep * kWRow, load_w[m] + r * w_step, r < rows);
+        for (uint32_t i = 0; i < Cfg::kMatrices * kWTurns; ++i) cp_async16(to[i % 2] + i * kWStep * kWRow, load_w[i / kWTurns] + i % kWTurns * w_step);
+      } else {
+        const uint32_t rows = k0 + w_piece * 32 < c.k ? load_rows : 0;
+#pragma unroll
+        for (uint32_t i = 0; i < Cfg::kMatrices * kWTurns; ++i)
+          if (i % kWTurns < rows) cp_async16(to[i % 2] + i * kWStep * kWRow, load_w[i / kWTurns] + i % kWTurns * w_step);
       }
 #pragma unroll
       for (uint32_t m = 0; m < Cfg::kMatrices; ++m) load_w[m] += units * kWRow;
@@ -240,13 +274,11 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
 #pragma unroll
       for (uint32_t j = 0; j < kXTurns; ++j) {
         const uint32_t row = x_row + j * kXStep;
-        if (row < stored_tokens) {
-          const bool some = row < load_tokens && x_inside;
-          cp_async16(base + x_to + j * kXStep * Cfg::kXRow, some ? load_x + j * x_step : static_cast<const uint8_t *>(c.x), some);
-        }
+        if (row < load_tokens && x_inside) cp_async16(base + x_to + j * kXStep * Cfg::kXRow, load_x + j * x_step);
+        else if (row < stored_tokens) sts128_zero(base + x_to + j * kXStep * Cfg::kXRow);
       }
       load_x += (uint64_t)units * kSlab * sizeof(T);
-      load_params(base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow, slab, load_n0);
+      load_params(base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow, slab, load_n0, whole);
       if (++load_index == mine) load_index = 0, load_tile += gridDim.x;
       load_slot = load_slot + 1 == kStages ? 0 : load_slot + 1;
     }
@@ -258,13 +290,11 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
 #pragma unroll
   for (uint32_t s = 0; s + 1 < kStages; ++s) load();
 
-  // Offsets of this lane's words in a stage: piece q of its weight rows, and its 16 (bf16) or 32 bytes of the tokens' 32 k, the latter for even and odd q
-  uint32_t w_from[kSlab / 32], x_from[2];
+  // Offsets in a stage of this lane's words of a block of its weight rows
+  uint32_t w_from[kSlab / kBlock];
 #pragma unroll
-  for (uint32_t q = 0; q < kSlab / 32; ++q) w_from[q] = (wr * RT * 16 + g) * kWRow + (q ^ (kWPieces == 8 ? g : (g >> 1) & 3)) * 16 + t * 4;
-#pragma unroll
-  for (uint32_t q = 0; q < 2; ++q)
-    x_from[q] = Cfg::kWStage + g * Cfg::kXRow + (kF32 ? (2 * t ^ ((g & 1) << 2)) * 16 : (q ^ (g & 1)) * 64 + t * 16);
+  for (uint32_t i = 0; i < kSlab / kBlock; ++i)
+    w_from[i] = (wr * RT * 16 + g) * kWRow + w_place(i * kWide + t * kWide / 4, g) * 16 + t * kWide % 4 * 4;
 
   uint32_t slot = 0, turn = 0;
   for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= Cfg::kSets - 1) {
@@ -288,9 +318,9 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
       const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
       slot = slot + 1 == kStages ? 0 : slot + 1;
       float part[RT][NT][4];
-      uint32_t minus_zero[RT][2];
+      uint32_t minus_zero[RT][2], words[RT][2][kWide];
 #pragma unroll
-      for (uint32_t q = 0; q < kSlab / 32; ++q) {  // 32 k: one 16-byte piece of a weight row
+      for (uint32_t q = 0; q < kSlab / 32; ++q) {  // a word of the lane's, 32 k of the four lanes of a row
         const bool begins = q * 32 % GROUP == 0, ends = (q + 1) * 32 % GROUP == 0;
         if (begins) {
 #pragma unroll
@@ -305,11 +335,17 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
               }
             }
         }
+        if (q % kWide == 0) {
+#pragma unroll
+          for (uint32_t rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) lds_words<kWide>(base + w_from[q / kWide] + (rt * 16 + h * 8) * kWRow, words[rt][h]);
+        }
         uint32_t a[RT][2][4];  // [rows 0-7 / 8-15][pair]
 #pragma unroll
         for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) dequant(lds32(base + w_from[q] + (rt * 16 + h * 8) * kWRow), minus_zero[rt][h], a[rt][h]);
+          for (uint32_t h = 0; h < 2; ++h) dequant(words[rt][h][q % kWide], minus_zero[rt][h], a[rt][h]);
 #pragma unroll
         for (uint32_t nt = 0; nt < NT; ++nt) {
           auto multiply = [&](const uint32_t (&b)[4], bool first) {
@@ -322,10 +358,11 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
                 else mma_bf16_16816(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
               }
           };
-          const uint32_t x_at = base + x_from[q & 1] + nt * 8 * Cfg::kXRow;
+          // the piece that goes with the word: its 8 k, of which a piece holds 16 / sizeof(T)
+          const uint32_t x_piece_at = (q / kWide * kBlock + t * 8 * kWide + q % kWide * 8) / kPer;
+          const uint32_t x_at = base + Cfg::kWStage + (nt * 8 + g) * Cfg::kXRow + x_place(x_piece_at, g) * 16;
           if constexpr (kF32) {
-            const uint32_t at = base + x_from[0] + nt * 8 * Cfg::kXRow + q * 128;
-            const uint4 lo = lds128(at), hi = lds128(at + 16);
+            const uint4 lo = lds128(x_at), hi = lds128(x_at + 16);
             float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
                           __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
 #pragma unroll
@@ -340,7 +377,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
               multiply(b, begins && term == 0);
             }
           } else {
-            const uint4 r = lds128(x_at + (q >> 1) * 128);
+            const uint4 r = lds128(x_at);
             const uint32_t b[4] = {r.x, r.y, r.z, r.w};
             multiply(b, begins);
           }
