@@ -464,8 +464,10 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
     if (cost < best) best = cost, ranks = r;
   }
   const uint32_t ctas = (uint32_t)std::min<uint64_t>(tiles, resident / ranks);
-  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(kernel, dim3(ctas, 1, ranks), dim3(kThreads), dim3(1, 1, ranks), smem, stream, c, (uint32_t)tiles, tiles_m,
-                                                       stored));
+  if (ranks == 1)
+    ORION_CUDA_CHECK("4-bit product", launch_pdl(kernel, dim3(ctas), dim3(kThreads), smem, stream, c, (uint32_t)tiles, tiles_m, stored));
+  else
+    ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(kernel, dim3(ctas, 1, ranks), dim3(kThreads), dim3(1, 1, ranks), smem, stream, c, (uint32_t)tiles, tiles_m, stored));
   count_launch();
   return ORION_OK;
 }

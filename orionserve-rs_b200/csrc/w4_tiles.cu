@@ -12,7 +12,8 @@
 // 9 instructions for eight weights: the masked pairs, read as f16, are code * 2^-24 or code * 2^-20 (subnormal numbers and the first binade count in steps of
 // 2^-24), and one fused multiply-add each subtracts 8 and multiplies by the scale; zero points are subtracted first, which is exact.
 //
-// Where tiles are too few for 74 pairs, k is cut as well: the parts are stored in f32 and summed in order by a third kernel, so results do not vary.
+// Where tiles are too few for the device, k is cut as well: the parts are summed in order, of single CTAs over the distributed shared memory of a cluster, of
+// pairs by a third kernel, so results do not vary.
 //
 // Warp 0 loads tokens, 1 of the leader issues the MMAs, then come the dequantising warps, eight of the epilogue, which works under the next tile's main loop.
 // Every wait is bounded; one that runs out sets the projections' error word.
@@ -72,8 +73,12 @@ struct Plan {
 };
 
 // Up to 128 tokens single CTAs, beyond them pairs. Tiles and parts of k so that the rounds of the units, times what a round takes, are least, in cycles: a
-// stage takes the tensor cores four cycles a token column and the dequantising warps some 450, a tile's end some 3000; parts of k are written and read again.
+// stage takes the tensor cores four cycles a token column and the dequantising warps some 450, a tile's end some 3000. Parts of k: of single CTAs they meet in a
+// cluster, all parts of a launch at once; of pairs they are written and read again.
 Plan make_plan(uint32_t rows, uint32_t weight_rows, uint32_t k) {
+  // CTAs of one to an SM that are at work together in clusters of so many, with the SMs of a GPC that are left over (36 clusters of four took two turns, 22 us
+  // instead of 12 for 32 of them)
+  constexpr uint32_t kClustered[9] = {0, 148, 144, 132, 128, 120, 126, 112, 112};
   Plan best;
   double cost = 1e300;
   const uint32_t ctas = rows <= Single128::kAccCols ? 1 : 2, units = kSms / ctas;
@@ -82,10 +87,12 @@ Plan make_plan(uint32_t rows, uint32_t weight_rows, uint32_t k) {
   const uint32_t most = std::min(256u, (rows + 31) / 32 * 32);
   for (uint32_t tokens = most; tokens >= std::min(most, 128u); tokens -= 32) {
     const uint32_t tiles_x = (rows + tokens - 1) / tokens;
-    for (uint32_t splits = 1; splits <= 8 && splits <= stages && (splits == 1 || (uint64_t)tiles_w * tiles_x <= 8 * units); ++splits) {
+    for (uint32_t splits = 1; splits <= 8 && splits <= stages; ++splits) {
+      const uint64_t tiles = (uint64_t)tiles_w * tiles_x;
+      if (splits > 1 && (ctas == 1 ? tiles * splits > kClustered[splits] : tiles > 8 * units)) continue;
       const uint64_t jobs = (uint64_t)tiles_w * tiles_x * splits, rounds = (jobs + units - 1) / units;
       double c = (double)rounds * ((stages + splits - 1) / splits * std::max(4.0 * tokens, 450.0) * (stage_k / 128) + 3000.0);
-      if (splits > 1) c += 4000.0 + (double)splits * rows * weight_rows * 8.0 / 2500.0;
+      if (splits > 1) c += ctas == 1 ? 2000.0 : 4000.0 + (double)splits * rows * weight_rows * 8.0 / 2500.0;
       if (c < cost) cost = c, best = {tokens, splits, tiles_w, tiles_x, stages, ctas};
     }
   }
@@ -106,7 +113,7 @@ Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint3
   w.x_unit = reinterpret_cast<float *>(base + place(&at, ((uint64_t)rows + 31) / 32 * 32 * 4));
   w.w_unit = reinterpret_cast<float *>(base + place(&at, padded_rows(weight_rows) * 4));
   w.params = reinterpret_cast<uint32_t *>(base + place(&at, padded_rows(weight_rows) * (k / group) * 4));
-  w.parts = reinterpret_cast<float *>(base + place(&at, plan.splits > 1 ? (uint64_t)plan.splits * rows * weight_rows * 4 : 0));
+  w.parts = reinterpret_cast<float *>(base + place(&at, plan.ctas == 2 && plan.splits > 1 ? (uint64_t)plan.splits * rows * weight_rows * 4 : 0));
   *bytes = at;
   return w;
 }
@@ -257,6 +264,11 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity) {
 }
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
@@ -657,7 +669,11 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
           v[4 * q] = __uint_as_float(rr[4 * q]) * 0.0625f * row_unit * f.x, v[4 * q + 1] = __uint_as_float(rr[4 * q + 1]) * 0.0625f * row_unit * f.y;
           v[4 * q + 2] = __uint_as_float(rr[4 * q + 2]) * 0.0625f * row_unit * f.z, v[4 * q + 3] = __uint_as_float(rr[4 * q + 3]) * 0.0625f * row_unit * f.w;
         }
-        if (plan.splits > 1) {
+        if (!kPair && plan.splits > 1) {  // over the tokens, which nothing reads any more
+          float *p = reinterpret_cast<float *>(smem) + mb * Pair::kRows + (warp & 3) * 32 + lane;
+#pragma unroll
+          for (uint32_t q = 0; q < 16; ++q) p[q * Pair::kRows] = v[q];
+        } else if (plan.splits > 1) {
           float *p = ws.parts + ((uint64_t)j.split * c.rows + token) * weight_rows + r;
 #pragma unroll
           for (uint32_t q = 0; q < 16; ++q)
@@ -688,6 +704,29 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (!kPair) {
+    if (plan.splits > 1) {
+      // The parts of a tile's k, in the CTAs of a cluster, each of which sums every splits-th token, in the order of k.
+      cluster_arrive_release();
+      cluster_wait_acquire();
+      const Job j = job(unit);
+      const uint32_t part = smem_u32(smem), tokens = min(j.cols, c.rows - j.x_row), outputs = Pair::kRows / kMatrices;
+      for (uint32_t i = threadIdx.x; i < (tokens + plan.splits - 1) / plan.splits * outputs; i += F::kWarps * 32) {
+        const uint32_t token = i / outputs * plan.splits + j.split, col = i % outputs, row = j.w_row / kMatrices + col;
+        if (token >= tokens || row >= c.n) continue;
+        float y[kMatrices];
+#pragma unroll
+        for (uint32_t m = 0; m < kMatrices; ++m) {
+          y[m] = 0.f;
+          for (uint32_t s = 0; s < plan.splits; ++s) y[m] += ld_cluster_f32(mapa_u32(part + (token * Pair::kRows + col * kMatrices + m) * 4, s));
+        }
+        const float out = GATED ? gated<bf16>(GatedAct{c.act, 0.f}, y[0], y[kMatrices - 1]) : y[0] + (c.bias ? c.bias[row] : 0.f);
+        static_cast<bf16 *>(c.out)[(uint64_t)(j.x_row + token) * c.ldo + row] = __float2bfloat16_rn(out);
+      }
+      cluster_arrive_release();  // nobody leaves while its parts are being read
+      cluster_wait_acquire();
+    }
+  }
   // Neither CTA leaves, nor frees the tensor memory the pair allocated together, while the other may still be read by an MMA or be reading its accumulator.
   if constexpr (kPair) {
     cluster_arrive_release();
@@ -756,10 +795,10 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), token_blocks = c.rows > 512 ? (c.rows + kPrepWarps - 1) / kPrepWarps : c.rows;
   ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(token_blocks + param_rows / 32), dim3(kPrepThreads), 0, stream, c, ws, matrices, param_rows, token_blocks));
   ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(F::kWarps * 32),
-                                                       dim3(F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, param_rows, error));
+                                                       dim3(F::kCtas == 1 ? plan.splits : F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, param_rows, error));
   count_launch();
   count_launch();
-  if (plan.splits > 1) {
+  if (F::kCtas == 2 && plan.splits > 1) {
     ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_sum_kernel<GATED>, dim3((c.n + 255) / 256 * c.rows), dim3(256), 0, stream, c, (const float *)ws.parts, plan.splits,
                                                  (c.n + 255) / 256));
     count_launch();

@@ -19,18 +19,18 @@ GROUPS = (32, 64, 128)
 _ACTIVATIONS = {"silu": _ffi.GATE_SILU, "gelu_tanh": _ffi.GATE_GELU_TANH}
 _torch = None
 _dtypes = {}  # torch dtype -> OrionDType
-_linear = _gated = None  # entry points of the library
+_empty = _linear = _gated = _quantize = None  # torch.empty_strided, the fastest of its kind, and entry points of the library
 
 
 def _load():
     """torch and the library, at the first call: the rest of the package does without torch."""
-    global _torch, _linear, _gated, _stream
+    global _torch, _empty, _linear, _gated, _quantize, _stream
     import torch
 
     lib = _ffi.lib()
-    _linear, _gated = lib.orion_cuda_w4_linear, lib.orion_cuda_w4_gated
+    _linear, _gated, _quantize = lib.orion_cuda_w4_linear, lib.orion_cuda_w4_gated, lib.orion_cuda_w4_quantize
     _dtypes.update({torch.float32: 0, torch.bfloat16: 2})
-    _torch = torch
+    _torch, _empty = torch, torch.empty_strided
     _stream = _raw_stream()
 
 
@@ -51,7 +51,7 @@ class W4Weight:
     ``packed`` is int32 ``[out, in / 8]``, ``scales`` bf16 ``[in / group, out]``, ``zeros`` uint8 like ``scales`` with values of at most 15, or None:
     8 everywhere. The tensors are kept and must not be resized; their values may be written."""
 
-    __slots__ = ("packed", "scales", "zeros", "group", "out_features", "in_features", "device_index", "_desc", "_address")
+    __slots__ = ("packed", "scales", "zeros", "group", "out_features", "in_features", "device_index", "_desc", "_address", "_spaces")
 
     def __init__(self, packed, scales, zeros=None, group: int = 128):
         if _torch is None:
@@ -71,10 +71,14 @@ class W4Weight:
             raise InvalidRequest("packed, scales and zeros are on different devices")
         if packed.data_ptr() % 16:
             raise InvalidRequest("packed: must start on a 16-byte boundary")
+        self._hold(packed, scales, zeros, group, n, k, packed.device.index)
+
+    def _hold(self, packed, scales, zeros, group, n, k, device_index):
         self.packed, self.scales, self.zeros, self.group = packed, scales, zeros, group
-        self.out_features, self.in_features, self.device_index = n, k, packed.device.index
+        self.out_features, self.in_features, self.device_index = n, k, device_index
         self._desc = _ffi.OrionW4Weight(packed.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), n, k, group)
         self._address = C.addressof(self._desc)
+        self._spaces = {}
 
     @classmethod
     def from_codes(cls, codes, scales, zeros=None, group: int = 128) -> "W4Weight":
@@ -111,7 +115,7 @@ def _rows(backend: CudaBackend, x, weight: W4Weight):
 
 def _output(x, out, rows, n):
     if out is None:
-        return x.new_empty((rows, n)), n
+        return _empty((rows, n), (n, 1), dtype=x.dtype, device=x.device), n
     if not isinstance(out, _torch.Tensor) or out.dtype != x.dtype or out.device != x.device or tuple(out.shape) != (rows, n) or (n > 1 and out.stride(1) != 1):
         raise InvalidRequest(f"out: a {x.dtype} tensor of shape [{rows}, {n}] on {x.device} is needed, its rows' values neighbours")
     if out.requires_grad and _torch.is_grad_enabled():
@@ -129,15 +133,20 @@ def _raw_stream():
 
 
 def _workspace(x, dtype, rows, weight, gated):
-    """(tensor or None, address, bytes) of what a call needs beside its arguments, from torch's allocator: its own until later work of the stream."""
-    if rows == 0 or dtype == 0:
+    """(tensor or None, address, bytes) of what a call needs beside its arguments, from torch's allocator: its own until later work of the stream. The sizes
+    are kept with the weight."""
+    key = rows << 3 | dtype << 1 | gated
+    need = weight._spaces.get(key)
+    if need is None:
+        size = C.c_uint64()
+        check(_ffi.lib().orion_cuda_w4_workspace(dtype, rows, weight._address, gated, C.byref(size)))
+        if len(weight._spaces) >= 256:
+            weight._spaces.clear()
+        need = weight._spaces[key] = size.value
+    if need == 0:
         return None, None, 0
-    need = C.c_uint64()
-    check(_ffi.lib().orion_cuda_w4_workspace(dtype, rows, weight._address, gated, C.byref(need)))
-    if need.value == 0:
-        return None, None, 0
-    t = x.new_empty(need.value, dtype=_torch.uint8)
-    return t, t.data_ptr(), need.value
+    t = _empty((need,), (1,), dtype=_torch.uint8, device=x.device)
+    return t, t.data_ptr(), need
 
 
 def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
@@ -193,9 +202,11 @@ def quantize_w4(backend: CudaBackend, weight, group: int = 128, zeros: bool = Fa
         raise InvalidRequest(f"a matrix of {n} x {k} has no whole groups of {group} (32, 64 or 128)")
     if weight.stride(1) != 1:
         raise InvalidRequest("weight: the values of a row must be neighbours")
-    packed = weight.new_empty((n, k // 8), dtype=_torch.int32)
-    scales = weight.new_empty((k // group, n), dtype=_torch.bfloat16)
-    zero = weight.new_empty((k // group, n), dtype=_torch.uint8) if zeros else None
-    check(_ffi.lib().orion_cuda_w4_quantize(backend._ordinal, _dtypes[weight.dtype], weight.data_ptr(), n, k, weight.stride(0), group, packed.data_ptr(),
-                                            scales.data_ptr(), None if zero is None else zero.data_ptr(), _stream(backend._ordinal)))
-    return W4Weight(packed, scales, zero, group)
+    w = W4Weight.__new__(W4Weight)
+    groups, device = k // group, weight.device
+    w._hold(_empty((n, k // 8), (k // 8, 1), dtype=_torch.int32, device=device), _empty((groups, n), (n, 1), dtype=_torch.bfloat16, device=device),
+            _empty((groups, n), (n, 1), dtype=_torch.uint8, device=device) if zeros else None, group, n, k, backend._ordinal)
+    d = w._desc
+    check(_quantize(backend._ordinal, _dtypes[weight.dtype], weight.data_ptr(), n, k, weight.stride(0), group, d.packed, d.scales, d.zeros,
+                    _stream(backend._ordinal)))
+    return w
