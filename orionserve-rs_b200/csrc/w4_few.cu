@@ -11,8 +11,8 @@
 //
 // A CTA of eight warps: WR of them side by side over weight rows, 8 / WR groups of them over k. Few tokens: WR = 1, every warp streams k slabs of its own
 // and only reads the tokens' values it needs; more tokens: warps share the tokens' slab, so that L2 delivers it less often. Each k group has a ring of
-// slabs of 128 or 256 k, weights, tokens and scales, filled by cp.async (no waits on barriers). CTAs stay and go from tile to tile, with the ring running ahead
-// across tiles. Sums of k groups meet in shared memory, and where the rows of weights give too few CTAs the k of a tile is dealt to the CTAs of a cluster, whose sums meet over
+// slabs of 128 or 256 k, weights, tokens and scales, filled by cp.async (no waits on barriers). A CTA has one tile: CTAs that went from tile to tile, the
+// rings running ahead, left more of the device idle at the end (8 rows of k 4096 to 128256 outputs: 68 us against 62). Sums of k groups meet in shared memory, and where the rows of weights give too few CTAs the k of a tile is dealt to the CTAs of a cluster, whose sums meet over
 // distributed shared memory: in both places in a fixed order, so results do not vary from run to run, and no workspace is needed.
 #include "kernels.h"
 #include "mma.cuh"
@@ -115,15 +115,15 @@ struct FewConfig {
   static constexpr uint32_t kPerSlab = kSlab / GROUP;                       // groups in a slab
   static constexpr uint32_t kScaleRow = kOutputs * 2, kZeroRow = kOutputs;  // scales, and zero points, of a group and matrix
   static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + (ZEROS ? kZeroRow : 0));
-  static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows;         // floats of the sums that meet in shared memory
-  // Slabs in the ring, and sets of sums: with few tokens two CTAs share an SM, with many one takes what there is.
-  static constexpr uint32_t kStages = kSlab == 256 ? 2 : NT <= 2 || sizeof(T) == 4 ? 3 : 4, kSets = NT <= 2 ? 2 : 1;
-  static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kSmem = kKGroups * kStages * kStage + kSets * kSums * 4;
+  static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows * 4;     // bytes of the sums that meet in shared memory, over the rings
+  // Slabs in the ring: with few tokens two CTAs share an SM, with many one takes what there is.
+  static constexpr uint32_t kStages = kSlab == 256 ? 2 : NT <= 2 || sizeof(T) == 4 ? 3 : 4;
+  static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kRings = kKGroups * kStages * kStage, kSmem = kRings > kSums ? kRings : kSums;
 };
 
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
 __global__ void __launch_bounds__(kThreads, NT == 1 || (NT == 2 && sizeof(T) == 2) ? 2 : 1)
-w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, const uint32_t stored_tokens) {
+w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   using Cfg = FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   constexpr bool kF32 = sizeof(T) == 4;
   constexpr uint32_t kPerSlab = Cfg::kPerSlab, kStages = Cfg::kStages, kStageBytes = Cfg::kStage, kSlab = Cfg::kSlab, kWRow = Cfg::kWRow;
@@ -137,7 +137,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   const uint32_t mine = unit < slabs ? (slabs - unit + units - 1) / units : 0;  // slabs of a tile that this k group takes
   const uint32_t groups = c.k / GROUP;
   const uint32_t ring = smem_u32(smem) + kg * kStages * kStageBytes;
-  float *const sums = reinterpret_cast<float *>(smem + Cfg::kKGroups * kStages * kStageBytes);
+  const uint32_t n0 = blockIdx.x / tiles_m * Cfg::kOutputs, m0 = blockIdx.x % tiles_m * Cfg::kTokens, tokens = min(Cfg::kTokens, c.rows - m0);
 
   // First output of a tile of 16 rows within the CTA's; with a gate the first half of a warp's tiles are the gate's.
   constexpr uint32_t kTilesPerMatrix = RT / Cfg::kMatrices;
@@ -167,20 +167,18 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   const uint64_t slab_step = (uint64_t)units * kPerSlab * c.n;  // scales from one slab to the next
   const bf16 *load_s[kScaleTurns];
   const uint8_t *load_z[kZeroTurns];
-  auto aim_params = [&](uint32_t n0) {
 #pragma unroll
-    for (uint32_t j = 0; j < kScaleTurns; ++j) {
-      const uint32_t i = in_kg + j * WR * 32, row = i / kScaleWords;
-      load_s[j] = (row >= kPerSlab ? c.up.scales : c.w.scales) + (uint64_t)(unit * kPerSlab + row % kPerSlab) * c.n + n0 + i % kScaleWords * 2;
-    }
+  for (uint32_t j = 0; j < kScaleTurns; ++j) {
+    const uint32_t i = in_kg + j * WR * 32, row = i / kScaleWords;
+    load_s[j] = (row >= kPerSlab ? c.up.scales : c.w.scales) + (uint64_t)(unit * kPerSlab + row % kPerSlab) * c.n + n0 + i % kScaleWords * 2;
+  }
 #pragma unroll
-    for (uint32_t j = 0; ZEROS && j < kZeroTurns; ++j) {
-      const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords;
-      const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
-      load_z[j] = p ? p + (uint64_t)(unit * kPerSlab + row % kPerSlab) * c.n + n0 + i % kZeroWords * 4 : nullptr;
-    }
-  };
-  auto load_params = [&](uint32_t s_at, uint32_t slab, uint32_t n0, bool whole) {
+  for (uint32_t j = 0; ZEROS && j < kZeroTurns; ++j) {
+    const uint32_t i = in_kg + j * WR * 32, row = i / kZeroWords;
+    const uint8_t *p = row >= kPerSlab ? c.up.zeros : c.w.zeros;
+    load_z[j] = p ? p + (uint64_t)(unit * kPerSlab + row % kPerSlab) * c.n + n0 + i % kZeroWords * 4 : nullptr;
+  }
+  auto load_params = [&](uint32_t s_at, uint32_t slab, bool whole) {
     if (words) {
 #pragma unroll
       for (uint32_t j = 0; j < kScaleTurns; ++j) {
@@ -216,8 +214,6 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
     }
   };
 
-  // What is loaded next: a slab of a tile. The loads run ahead of the products across tiles, so that the ring never drains.
-  //
   // Weight rows of 64 or 128 bytes, their 16-byte pieces permuted so that the eight rows of a fragment lie in different banks; a lane copies one piece of
   // every fourth or eighth row of its warp's tiles. Rows beyond the last are left as they are: nothing of them is stored. Token rows: every other one with its
   // halves of 64 bytes exchanged, zeros beyond the last k.
@@ -240,30 +236,25 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   };
   const uint32_t x_row = in_kg / kPieces, x_piece = in_kg % kPieces, x_to = Cfg::kWStage + x_row * Cfg::kXRow + x_place(x_piece, x_row) * 16;
   const uint64_t w_step = (uint64_t)c.k / 2 * kWStep, x_step = kXStep * c.ldx * sizeof(T);  // bytes
-  uint32_t load_tile = blockIdx.x, load_index = 0, load_slot = 0, load_n0 = 0, load_tokens = 0, load_rows = 0;
-  const uint8_t *load_w[Cfg::kMatrices] = {}, *load_x = nullptr;
-  auto load = [&] {
+  const uint32_t first_row = n0 + wr * kTilesPerMatrix * 16 + w_row, rows_there = first_row < c.n ? (c.n - first_row + kWStep - 1) / kWStep : 0;  // per matrix
+  const uint64_t first_at = ((uint64_t)first_row * (c.k / 8) + unit * (kSlab / 8) + w_piece * 4) * 4;
+  const uint8_t *load_w[Cfg::kMatrices];
+  load_w[0] = reinterpret_cast<const uint8_t *>(c.w.packed) + first_at;
+  if (GATED) load_w[Cfg::kMatrices - 1] = reinterpret_cast<const uint8_t *>(c.up.packed) + first_at;
+  const uint8_t *load_x = static_cast<const uint8_t *>(c.x) + ((uint64_t)(m0 + x_row) * c.ldx + unit * kSlab + x_piece * kPer) * sizeof(T);
+  const bool whole_rows = n0 + Cfg::kOutputs <= c.n;
+  uint32_t load_index = 0, load_slot = 0;
+  auto load = [&] {  // the next slab of this k group
     store_held();
-    if (load_tile < tiles && mine > 0) {
-      if (load_index == 0) {
-        load_n0 = load_tile / tiles_m * Cfg::kOutputs;
-        const uint32_t m0 = load_tile % tiles_m * Cfg::kTokens, row = load_n0 + wr * kTilesPerMatrix * 16 + w_row;
-        load_tokens = min(Cfg::kTokens, c.rows - m0);
-        aim_params(load_n0);
-        load_rows = row < c.n ? (c.n - row + kWStep - 1) / kWStep : 0;  // of this lane's, per matrix
-        const uint64_t at = ((uint64_t)row * (c.k / 8) + unit * (kSlab / 8) + w_piece * 4) * 4;
-        load_w[0] = reinterpret_cast<const uint8_t *>(c.w.packed) + at;
-        if (GATED) load_w[Cfg::kMatrices - 1] = reinterpret_cast<const uint8_t *>(c.up.packed) + at;
-        load_x = static_cast<const uint8_t *>(c.x) + ((uint64_t)(m0 + x_row) * c.ldx + unit * kSlab + x_piece * kPer) * sizeof(T);
-      }
+    if (load_index < mine) {
       const uint32_t slab = unit + load_index * units, k0 = slab * kSlab, base = ring + load_slot * kStageBytes;
       const uint32_t to[2] = {base + w_to_places[0], base + w_to_places[1]};
-      const bool whole = load_n0 + Cfg::kOutputs <= c.n && k0 + kSlab <= c.k;
+      const bool whole = whole_rows && k0 + kSlab <= c.k;
       if (whole) {
 #pragma unroll
         for (uint32_t i = 0; i < Cfg::kMatrices * kWTurns; ++i) cp_async16(to[i % 2] + i * kWStep * kWRow, load_w[i / kWTurns] + i % kWTurns * w_step);
       } else {
-        const uint32_t rows = k0 + w_piece * 32 < c.k ? load_rows : 0;
+        const uint32_t rows = k0 + w_piece * 32 < c.k ? rows_there : 0;
 #pragma unroll
         for (uint32_t i = 0; i < Cfg::kMatrices * kWTurns; ++i)
           if (i % kWTurns < rows) cp_async16(to[i % 2] + i * kWStep * kWRow, load_w[i / kWTurns] + i % kWTurns * w_step);
@@ -274,19 +265,19 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
 #pragma unroll
       for (uint32_t j = 0; j < kXTurns; ++j) {
         const uint32_t row = x_row + j * kXStep;
-        if (row < load_tokens && x_inside) cp_async16(base + x_to + j * kXStep * Cfg::kXRow, load_x + j * x_step);
-        else if (row < stored_tokens) sts128_zero(base + x_to + j * kXStep * Cfg::kXRow);
+        if (row < tokens && x_inside) cp_async16(base + x_to + j * kXStep * Cfg::kXRow, load_x + j * x_step);
+        else if (row < tokens) sts128_zero(base + x_to + j * kXStep * Cfg::kXRow);
       }
       load_x += (uint64_t)units * kSlab * sizeof(T);
-      load_params(base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow, slab, load_n0, whole);
-      if (++load_index == mine) load_index = 0, load_tile += gridDim.x;
+      load_params(base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow, slab, whole);
+      ++load_index;
       load_slot = load_slot + 1 == kStages ? 0 : load_slot + 1;
     }
     cp_async_commit();
   };
   // token rows that nothing is loaded to
   for (uint32_t s = 0; s < kStages; ++s)
-    for (uint32_t i = stored_tokens * kPieces + in_kg; i < Cfg::kTokens * kPieces; i += WR * 32) sts128_zero(ring + s * kStageBytes + Cfg::kWStage + i * 16);
+    for (uint32_t i = tokens * kPieces + in_kg; i < Cfg::kTokens * kPieces; i += WR * 32) sts128_zero(ring + s * kStageBytes + Cfg::kWStage + i * 16);
 #pragma unroll
   for (uint32_t s = 0; s + 1 < kStages; ++s) load();
 
@@ -296,151 +287,145 @@ w4_few_kernel(const W4Call c, const uint32_t tiles, const uint32_t tiles_m, cons
   for (uint32_t i = 0; i < kSlab / kBlock; ++i)
     w_from[i] = (wr * RT * 16 + g) * kWRow + w_place(i * kWide + t * kWide / 4, g) * 16 + t * kWide % 4 * 4;
 
-  uint32_t slot = 0, turn = 0;
-  for (uint32_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= Cfg::kSets - 1) {
-    const uint32_t n0 = tile / tiles_m * Cfg::kOutputs, m0 = tile % tiles_m * Cfg::kTokens, tokens = min(Cfg::kTokens, c.rows - m0);
-    float sum[RT][NT][4];
+  float sum[RT][NT][4];
 #pragma unroll
-    for (uint32_t rt = 0; rt < RT; ++rt)
+  for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (uint32_t nt = 0; nt < NT; ++nt)
+    for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) sum[rt][nt][i] = 0.f;
+      for (uint32_t i = 0; i < 4; ++i) sum[rt][nt][i] = 0.f;
 
-    for (uint32_t index = 0; index < mine; ++index) {
-      cp_async_wait<kStages - 2>();
-      if constexpr (WR == 1) __syncwarp();
-      else if constexpr (WR == kWarps) __syncthreads();
-      else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(WR * 32) : "memory");
-      load();
+  uint32_t slot = 0;
+  for (uint32_t index = 0; index < mine; ++index) {
+    cp_async_wait<kStages - 2>();
+    if constexpr (WR == 1) __syncwarp();
+    else if constexpr (WR == kWarps) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(WR * 32) : "memory");
+    load();
 
-      const uint32_t base = ring + slot * kStageBytes, s_at = base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow;
-      const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
-      slot = slot + 1 == kStages ? 0 : slot + 1;
-      float part[RT][NT][4];
-      uint32_t minus_zero[RT][2], words[RT][2][kWide];
+    const uint32_t base = ring + slot * kStageBytes, s_at = base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow;
+    const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
+    slot = slot + 1 == kStages ? 0 : slot + 1;
+    float part[RT][NT][4];
+    uint32_t minus_zero[RT][2], words[RT][2][kWide];
 #pragma unroll
-      for (uint32_t q = 0; q < kSlab / 32; ++q) {  // a word of the lane's, 32 k of the four lanes of a row
-        const bool begins = q * 32 % GROUP == 0, ends = (q + 1) * 32 % GROUP == 0;
-        if (begins) {
-#pragma unroll
-          for (uint32_t rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-              minus_zero[rt][h] = 0xba80ba80u;  // -8 / kUnit
-              if (ZEROS) {
-                const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
-                // as the codes: at most eight bits, so exact
-                minus_zero[rt][h] = fma_bf16x2(lds8(z_at + row * Cfg::kZeroRow + col_of(rt) + h * 8 + g) * 0x10001u, 0xfb80fb80u, 0x80008000u);
-              }
-            }
-        }
-        if (q % kWide == 0) {
-#pragma unroll
-          for (uint32_t rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) lds_words<kWide>(base + w_from[q / kWide] + (rt * 16 + h * 8) * kWRow, words[rt][h]);
-        }
-        uint32_t a[RT][2][4];  // [rows 0-7 / 8-15][pair]
+    for (uint32_t q = 0; q < kSlab / 32; ++q) {  // a word of the lane's, 32 k of the four lanes of a row
+      const bool begins = q * 32 % GROUP == 0, ends = (q + 1) * 32 % GROUP == 0;
+      if (begins) {
 #pragma unroll
         for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (uint32_t h = 0; h < 2; ++h) dequant(words[rt][h][q % kWide], minus_zero[rt][h], a[rt][h]);
-#pragma unroll
-        for (uint32_t nt = 0; nt < NT; ++nt) {
-          auto multiply = [&](const uint32_t (&b)[4], bool first) {
-#pragma unroll
-            for (uint32_t rt = 0; rt < RT; ++rt)
-#pragma unroll
-              for (uint32_t half = 0; half < 2; ++half) {
-                const uint32_t frag[4] = {a[rt][0][2 * half], a[rt][1][2 * half], a[rt][0][2 * half + 1], a[rt][1][2 * half + 1]};
-                if (first && half == 0) mma_first(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
-                else mma_bf16_16816(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
-              }
-          };
-          // the piece that goes with the word: its 8 k, of which a piece holds 16 / sizeof(T)
-          const uint32_t x_piece_at = (q / kWide * kBlock + t * 8 * kWide + q % kWide * 8) / kPer;
-          const uint32_t x_at = base + Cfg::kWStage + (nt * 8 + g) * Cfg::kXRow + x_place(x_piece_at, g) * 16;
-          if constexpr (kF32) {
-            const uint4 lo = lds128(x_at), hi = lds128(x_at + 16);
-            float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
-                          __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
-#pragma unroll
-            for (uint32_t term = 0; term < 3; ++term) {
-              uint32_t b[4];
-#pragma unroll
-              for (uint32_t i = 0; i < 4; ++i) {
-                b[i] = upper_halves(v[2 * i], v[2 * i + 1]);
-                v[2 * i] = beyond(v[2 * i], first_bits(v[2 * i]));
-                v[2 * i + 1] = beyond(v[2 * i + 1], first_bits(v[2 * i + 1]));
-              }
-              multiply(b, begins && term == 0);
+          for (uint32_t h = 0; h < 2; ++h) {
+            minus_zero[rt][h] = 0xba80ba80u;  // -8 / kUnit
+            if (ZEROS) {
+              const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
+              // as the codes: at most eight bits, so exact
+              minus_zero[rt][h] = fma_bf16x2(lds8(z_at + row * Cfg::kZeroRow + col_of(rt) + h * 8 + g) * 0x10001u, 0xfb80fb80u, 0x80008000u);
             }
-          } else {
-            const uint4 r = lds128(x_at);
-            const uint32_t b[4] = {r.x, r.y, r.z, r.w};
-            multiply(b, begins);
           }
-        }
-        if (ends) {
+      }
+      if (q % kWide == 0) {
+#pragma unroll
+        for (uint32_t rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (uint32_t h = 0; h < 2; ++h) lds_words<kWide>(base + w_from[q / kWide] + (rt * 16 + h * 8) * kWRow, words[rt][h]);
+      }
+      uint32_t a[RT][2][4];  // [rows 0-7 / 8-15][pair]
+#pragma unroll
+      for (uint32_t rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) dequant(words[rt][h][q % kWide], minus_zero[rt][h], a[rt][h]);
+#pragma unroll
+      for (uint32_t nt = 0; nt < NT; ++nt) {
+        auto multiply = [&](const uint32_t (&b)[4], bool first) {
 #pragma unroll
           for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
-              const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
-              const float scale = __uint_as_float(lds16(s_at + row * Cfg::kScaleRow + (col_of(rt) + h * 8 + g) * 2) << 16);
-#pragma unroll
-              for (uint32_t nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (uint32_t i = 2 * h; i < 2 * h + 2; ++i) sum[rt][nt][i] = fmaf(part[rt][nt][i], scale, sum[rt][nt][i]);
+            for (uint32_t half = 0; half < 2; ++half) {
+              const uint32_t frag[4] = {a[rt][0][2 * half], a[rt][1][2 * half], a[rt][0][2 * half + 1], a[rt][1][2 * half + 1]};
+              if (first && half == 0) mma_first(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
+              else mma_bf16_16816(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
             }
+        };
+        // the piece that goes with the word: its 8 k, of which a piece holds 16 / sizeof(T)
+        const uint32_t x_piece_at = (q / kWide * kBlock + t * 8 * kWide + q % kWide * 8) / kPer;
+        const uint32_t x_at = base + Cfg::kWStage + (nt * 8 + g) * Cfg::kXRow + x_place(x_piece_at, g) * 16;
+        if constexpr (kF32) {
+          const uint4 lo = lds128(x_at), hi = lds128(x_at + 16);
+          float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
+                        __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
+#pragma unroll
+          for (uint32_t term = 0; term < 3; ++term) {
+            uint32_t b[4];
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+              b[i] = upper_halves(v[2 * i], v[2 * i + 1]);
+              v[2 * i] = beyond(v[2 * i], first_bits(v[2 * i]));
+              v[2 * i + 1] = beyond(v[2 * i + 1], first_bits(v[2 * i + 1]));
+            }
+            multiply(b, begins && term == 0);
+          }
+        } else {
+          const uint4 r = lds128(x_at);
+          const uint32_t b[4] = {r.x, r.y, r.z, r.w};
+          multiply(b, begins);
         }
       }
-    }
-
-    // The k groups' sums, [k group][token][row]. Where two sets take turns one barrier a tile is enough.
-    if (Cfg::kSets == 1 && tile != blockIdx.x) {
-      if (ranks > 1) cluster_barrier();
-      else __syncthreads();
-    }
-    float *const mine_at = sums + turn * Cfg::kSums;
+      if (ends) {
 #pragma unroll
-    for (uint32_t rt = 0; rt < RT; ++rt)
+        for (uint32_t rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (uint32_t nt = 0; nt < NT; ++nt)
+          for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
+            const float scale = __uint_as_float(lds16(s_at + row * Cfg::kScaleRow + (col_of(rt) + h * 8 + g) * 2) << 16);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const uint32_t token = nt * 8 + t * 2 + (i & 1);
-          if (token < stored_tokens) mine_at[(kg * Cfg::kTokens + token) * Cfg::kTileRows + (wr * RT + rt) * 16 + (i >> 1) * 8 + g] = sum[rt][nt][i] * kUnit;
-        }
-    if (ranks > 1) cluster_barrier();
-    else __syncthreads();
-    auto total = [&](uint32_t token, uint32_t row) {
-      float v = 0.f;
-      for (uint32_t r = 0; r < ranks; ++r) {
+            for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (uint32_t j = 0; j < Cfg::kKGroups; ++j) {
-          const float *p = mine_at + (j * Cfg::kTokens + token) * Cfg::kTileRows + row;
-          v += ranks == 1 ? *p : ld_cluster_f32(smem_u32(p), r);
-        }
+              for (uint32_t i = 2 * h; i < 2 * h + 2; ++i) sum[rt][nt][i] = fmaf(part[rt][nt][i], scale, sum[rt][nt][i]);
+          }
       }
-      return v;
-    };
-    for (uint32_t i = rank * kThreads + threadIdx.x; i < tokens * Cfg::kOutputs; i += ranks * kThreads) {
-      const uint32_t token = i / Cfg::kOutputs, col = i % Cfg::kOutputs;
-      if (n0 + col >= c.n) continue;
-      float y;
-      if constexpr (GATED) {
-        constexpr uint32_t kHalf = kTilesPerMatrix * 16;
-        const uint32_t at = col / kHalf * (2 * kHalf) + col % kHalf;
-        y = gated<T>(GatedAct{c.act, 0.f}, total(token, at), total(token, at + kHalf));
-      } else {
-        y = total(token, col) + (c.bias ? c.bias[n0 + col] : 0.f);
-      }
-      static_cast<T *>(c.out)[(uint64_t)(m0 + token) * c.ldo + n0 + col] = from_f32<T>(y);
     }
   }
+
+  // The k groups' sums, [k group][token][row], over the rings
   cp_async_wait<0>();
+  __syncthreads();
+  float *const sums = reinterpret_cast<float *>(smem);
+#pragma unroll
+  for (uint32_t rt = 0; rt < RT; ++rt)
+#pragma unroll
+    for (uint32_t nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t token = nt * 8 + t * 2 + (i & 1);
+        if (token < tokens) sums[(kg * Cfg::kTokens + token) * Cfg::kTileRows + (wr * RT + rt) * 16 + (i >> 1) * 8 + g] = sum[rt][nt][i] * kUnit;
+      }
+  if (ranks > 1) cluster_barrier();
+  else __syncthreads();
+  auto total = [&](uint32_t token, uint32_t row) {
+    float v = 0.f;
+    for (uint32_t r = 0; r < ranks; ++r) {
+#pragma unroll
+      for (uint32_t j = 0; j < Cfg::kKGroups; ++j) {
+        const float *p = sums + (j * Cfg::kTokens + token) * Cfg::kTileRows + row;
+        v += ranks == 1 ? *p : ld_cluster_f32(smem_u32(p), r);
+      }
+    }
+    return v;
+  };
+  for (uint32_t i = rank * kThreads + threadIdx.x; i < tokens * Cfg::kOutputs; i += ranks * kThreads) {
+    const uint32_t token = i / Cfg::kOutputs, col = i % Cfg::kOutputs;
+    if (n0 + col >= c.n) continue;
+    float y;
+    if constexpr (GATED) {
+      constexpr uint32_t kHalf = kTilesPerMatrix * 16;
+      const uint32_t at = col / kHalf * (2 * kHalf) + col % kHalf;
+      y = gated<T>(GatedAct{c.act, 0.f}, total(token, at), total(token, at + kHalf));
+    } else {
+      y = total(token, col) + (c.bias ? c.bias[n0 + col] : 0.f);
+    }
+    static_cast<T *>(c.out)[(uint64_t)(m0 + token) * c.ldo + n0 + col] = from_f32<T>(y);
+  }
   if (ranks > 1) cluster_barrier();  // nobody leaves while its sums are being read
 }
 
@@ -451,23 +436,18 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
   const auto kernel = w4_few_kernel<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(kernel, (int)Cfg::kSmem, done));
   const uint32_t tiles_n = (c.n + Cfg::kOutputs - 1) / Cfg::kOutputs, tiles_m = (c.rows + Cfg::kTokens - 1) / Cfg::kTokens;
-  const uint32_t stored = std::min(c.rows, Cfg::kTokens), smem = Cfg::kSmem;
   const uint64_t tiles = (uint64_t)tiles_n * tiles_m;
   if (tiles > 0x7fffffffull) return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
-  // k over a cluster of `ranks` CTAs: as many as make the rounds of tiles shortest, a tile's end counted as two slabs
-  const uint32_t resident = 148 * (NT <= 2 && smem + 1024 <= 114 * 1024 ? 2 : 1), slabs = (c.k + Cfg::kSlab - 1) / Cfg::kSlab;
+  // k over a cluster of up to eight CTAs where there are few tiles, as long as every k group has a slab. A cluster starts when it has room for all of its
+  // CTAs, so it is not for launches that fill the device anyway: 1 row of k 14336 to 4096 outputs (32 tiles) takes 33 us with one CTA a tile, 15 with
+  // four, 11 with eight, of k 4096 to 28672 (224 tiles) 18, 30 and 45.
+  const uint32_t slabs = (c.k + Cfg::kSlab - 1) / Cfg::kSlab;
   uint32_t ranks = 1;
-  uint64_t best = ~0ull;
-  for (uint32_t r = 1; r <= 8; ++r) {
-    const uint64_t at_once = std::max(1u, resident / r), rounds = (tiles + at_once - 1) / at_once;
-    const uint64_t cost = rounds * ((slabs + Cfg::kKGroups * r - 1) / (Cfg::kKGroups * r) + 2);
-    if (cost < best) best = cost, ranks = r;
-  }
-  const uint32_t ctas = (uint32_t)std::min<uint64_t>(tiles, resident / ranks);
+  while (ranks < 8 && tiles * ranks * 2 <= 256 && slabs >= Cfg::kKGroups * ranks * 2) ranks *= 2;
   if (ranks == 1)
-    ORION_CUDA_CHECK("4-bit product", launch_pdl(kernel, dim3(ctas), dim3(kThreads), smem, stream, c, (uint32_t)tiles, tiles_m, stored));
+    ORION_CUDA_CHECK("4-bit product", launch_pdl(kernel, dim3((uint32_t)tiles), dim3(kThreads), Cfg::kSmem, stream, c, tiles_m));
   else
-    ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(kernel, dim3(ctas, 1, ranks), dim3(kThreads), dim3(1, 1, ranks), smem, stream, c, (uint32_t)tiles, tiles_m, stored));
+    ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(kernel, dim3((uint32_t)tiles, 1, ranks), dim3(kThreads), dim3(1, 1, ranks), Cfg::kSmem, stream, c, tiles_m));
   count_launch();
   return ORION_OK;
 }
