@@ -8,6 +8,7 @@
 // fma(pair, 2^120 or 2^116, -zero * 2^-13) = (code - zero) * 2^-13, exactly.
 //
 // f32 activations go through the same instructions as three bf16 terms of eight bits each (hi + mid + lo = x exactly), so f32 results have f32 accuracy.
+// The warps that share a slab of tokens make its terms together (211 rows of k 2048 to 5504 outputs: 98 us with each warp making its own).
 //
 // A CTA of eight warps: WR of them side by side over weight rows, 8 / WR groups of them over k. Few tokens: WR = 1, every warp streams k slabs of its own
 // and only reads the tokens' values it needs; more tokens: warps share the tokens' slab, so that L2 delivers it less often. Each k group has a ring of
@@ -30,6 +31,9 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void sts128_zero(uint32_t addr) { asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(addr), "r"(0u) : "memory"); }
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ void sts32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void sts16(uint32_t addr, uint32_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"((uint16_t)v) : "memory"); }
 __device__ __forceinline__ void sts8(uint32_t addr, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
@@ -118,7 +122,10 @@ struct FewConfig {
   static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows * 4;     // bytes of the sums that meet in shared memory, over the rings
   // Slabs in the ring: with few tokens two CTAs share an SM, with many one takes what there is.
   static constexpr uint32_t kStages = kSlab == 256 ? 2 : NT <= 2 || sizeof(T) == 4 ? 3 : 4;
-  static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kRings = kKGroups * kStages * kStage, kSmem = kRings > kSums ? kRings : kSums;
+  static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kRings = kKGroups * kStages * kStage;
+  // f32 tokens of the slab at hand, in bf16 terms: [term][token][k]
+  static constexpr uint32_t kTermRow = kSlab * 2, kTerms = sizeof(T) == 4 ? 3 * kTokens * kTermRow : 0, kAll = kRings + kKGroups * kTerms;
+  static constexpr uint32_t kSmem = kAll > kSums ? kAll : kSums;
 };
 
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
@@ -136,7 +143,11 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   const uint32_t slabs = (c.k + kSlab - 1) / kSlab, units = Cfg::kKGroups * ranks, unit = rank * Cfg::kKGroups + kg;
   const uint32_t mine = unit < slabs ? (slabs - unit + units - 1) / units : 0;  // slabs of a tile that this k group takes
   const uint32_t groups = c.k / GROUP;
-  const uint32_t ring = smem_u32(smem) + kg * kStages * kStageBytes;
+  const uint32_t ring = smem_u32(smem) + kg * kStages * kStageBytes, terms = smem_u32(smem) + Cfg::kRings + kg * Cfg::kTerms;
+  auto sync_k_group = [&] {
+    if constexpr (WR == kWarps) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(WR * 32) : "memory");
+  };
   const uint32_t n0 = blockIdx.x / tiles_m * Cfg::kOutputs, m0 = blockIdx.x % tiles_m * Cfg::kTokens, tokens = min(Cfg::kTokens, c.rows - m0);
 
   // First output of a tile of 16 rows within the CTA's; with a gate the first half of a warp's tiles are the gate's.
@@ -146,7 +157,8 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   pdl_wait();
 
   // Scales and zero points of a slab. Where the outputs are whole words (n a multiple of 4) they come by cp.async like the rest, zeros in place of groups
-  // beyond the last. Else they pass through registers: asked for with a slab, stored with the next one, long before they are read.
+  // beyond the last. Else they pass through registers: asked for with the slab's loads, stored after the products of
+  // the slab before, ahead of the barrier that lets the warps at them.
   constexpr uint32_t kScaleWords = Cfg::kOutputs / 2, kZeroWords = Cfg::kOutputs / 4, kRowsOfParams = Cfg::kMatrices * kPerSlab;
   constexpr uint32_t kParamTurns = (kRowsOfParams * Cfg::kOutputs + WR * 32 - 1) / (WR * 32);
   const bool words = (c.n & 3) == 0;
@@ -222,9 +234,9 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   static_assert(kXStep % 2 == 0, "rows of a lane's turns are permuted alike");
   constexpr uint32_t kWPieces = kSlab / 32, kWStep = 32 / kWPieces, kWTurns = kTilesPerMatrix * 16 / kWStep;  // rows from one turn to the next, turns per matrix
   const uint32_t w_row = lane / kWPieces, w_piece = lane % kWPieces;
-  // Where a piece goes within its row, so that the rows that are read together lie in different banks: eight of them 4 bytes a lane (f32, groups of 32),
-  // four 8 bytes (64), two 16 bytes (128). Of rows of 128 bytes every other turn has row & 4 set.
-  constexpr uint32_t kWide = kF32 ? 1 : GROUP / 32, kBlock = 32 * kWide;  // words of a row that a lane takes together, k of the four lanes of a row
+  // Where a piece goes within its row, so that the rows that are read together lie in different banks: eight of them 4 bytes a lane (groups of 32), four 8
+  // bytes (64), two 16 bytes (128). Of rows of 128 bytes every other turn has row & 4 set.
+  constexpr uint32_t kWide = GROUP / 32, kBlock = 32 * kWide;  // words of a row that a lane takes together, k of the four lanes of a row
   auto w_place = [](uint32_t piece, uint32_t row) {
     if (kWPieces == 8) return piece ^ (kWide == 1 ? row & 7 : kWide == 2 ? (row & 3) << 1 : (row & 1) << 2);
     return piece ^ (kWide == 1 ? (row >> 1) & 3 : kWide == 2 ? row & 2 : 0);
@@ -234,7 +246,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   auto x_place = [](uint32_t piece, uint32_t row) {  // likewise: lanes read pieces kWide apart, of two rows together
     return piece ^ (kWide == 1 ? (row & 1) << 2 : row & 1) ^ (kWide == 4 ? (piece >> 3 & 1) << 1 : 0);
   };
-  const uint32_t x_row = in_kg / kPieces, x_piece = in_kg % kPieces, x_to = Cfg::kWStage + x_row * Cfg::kXRow + x_place(x_piece, x_row) * 16;
+  const uint32_t x_row = in_kg / kPieces, x_piece = in_kg % kPieces, x_to = Cfg::kWStage + x_row * Cfg::kXRow + (kF32 ? x_piece ^ (x_row & 1) << 2 : x_place(x_piece, x_row)) * 16;
   const uint64_t w_step = (uint64_t)c.k / 2 * kWStep, x_step = kXStep * c.ldx * sizeof(T);  // bytes
   const uint32_t first_row = n0 + wr * kTilesPerMatrix * 16 + w_row, rows_there = first_row < c.n ? (c.n - first_row + kWStep - 1) / kWStep : 0;  // per matrix
   const uint64_t first_at = ((uint64_t)first_row * (c.k / 8) + unit * (kSlab / 8) + w_piece * 4) * 4;
@@ -280,6 +292,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
     for (uint32_t i = tokens * kPieces + in_kg; i < Cfg::kTokens * kPieces; i += WR * 32) sts128_zero(ring + s * kStageBytes + Cfg::kWStage + i * 16);
 #pragma unroll
   for (uint32_t s = 0; s + 1 < kStages; ++s) load();
+  store_held();
 
   // Offsets in a stage of this lane's words of a block of its weight rows
   uint32_t w_from[kSlab / kBlock];
@@ -298,13 +311,27 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   uint32_t slot = 0;
   for (uint32_t index = 0; index < mine; ++index) {
     cp_async_wait<kStages - 2>();
-    if constexpr (WR == 1) __syncwarp();
-    else if constexpr (WR == kWarps) __syncthreads();
-    else asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(WR * 32) : "memory");
+    sync_k_group();
     load();
 
     const uint32_t base = ring + slot * kStageBytes, s_at = base + Cfg::kWStage + Cfg::kTokens * Cfg::kXRow;
     const uint32_t z_at = s_at + kRowsOfParams * Cfg::kScaleRow;
+    if constexpr (kF32) {  // the terms of the slab's values, once for all warps of the k group
+      for (uint32_t i = in_kg; i < Cfg::kTokens * (kSlab / 8); i += WR * 32) {
+        const uint32_t row = i / (kSlab / 8), piece = i % (kSlab / 8), at = base + Cfg::kWStage + row * Cfg::kXRow + (2 * piece ^ (row & 1) << 2) * 16;
+        const uint4 lo = lds128(at), hi = lds128(at + 16);
+        float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
+                      __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
+#pragma unroll
+        for (uint32_t term = 0; term < 3; ++term) {
+          sts128(terms + (term * Cfg::kTokens + row) * Cfg::kTermRow + x_place(piece, row) * 16, upper_halves(v[0], v[1]), upper_halves(v[2], v[3]),
+                 upper_halves(v[4], v[5]), upper_halves(v[6], v[7]));
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j) v[j] = beyond(v[j], first_bits(v[j]));
+        }
+      }
+      sync_k_group();
+    }
     slot = slot + 1 == kStages ? 0 : slot + 1;
     float part[RT][NT][4];
     uint32_t minus_zero[RT][2], words[RT][2][kWide];
@@ -347,26 +374,16 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
               else mma_bf16_16816(part[rt][nt], frag, b[2 * half], b[2 * half + 1]);
             }
         };
-        // the piece that goes with the word: its 8 k, of which a piece holds 16 / sizeof(T)
-        const uint32_t x_piece_at = (q / kWide * kBlock + t * 8 * kWide + q % kWide * 8) / kPer;
-        const uint32_t x_at = base + Cfg::kWStage + (nt * 8 + g) * Cfg::kXRow + x_place(x_piece_at, g) * 16;
+        const uint32_t x_piece_at = q / kWide * (kBlock / 8) + t * kWide + q % kWide;  // the 8 k of the word
         if constexpr (kF32) {
-          const uint4 lo = lds128(x_at), hi = lds128(x_at + 16);
-          float v[8] = {__uint_as_float(lo.x), __uint_as_float(lo.y), __uint_as_float(lo.z), __uint_as_float(lo.w),
-                        __uint_as_float(hi.x), __uint_as_float(hi.y), __uint_as_float(hi.z), __uint_as_float(hi.w)};
 #pragma unroll
           for (uint32_t term = 0; term < 3; ++term) {
-            uint32_t b[4];
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) {
-              b[i] = upper_halves(v[2 * i], v[2 * i + 1]);
-              v[2 * i] = beyond(v[2 * i], first_bits(v[2 * i]));
-              v[2 * i + 1] = beyond(v[2 * i + 1], first_bits(v[2 * i + 1]));
-            }
+            const uint4 r = lds128(terms + (term * Cfg::kTokens + nt * 8 + g) * Cfg::kTermRow + x_place(x_piece_at, g) * 16);
+            const uint32_t b[4] = {r.x, r.y, r.z, r.w};
             multiply(b, begins && term == 0);
           }
         } else {
-          const uint4 r = lds128(x_at);
+          const uint4 r = lds128(base + Cfg::kWStage + (nt * 8 + g) * Cfg::kXRow + x_place(x_piece_at, g) * 16);
           const uint32_t b[4] = {r.x, r.y, r.z, r.w};
           multiply(b, begins);
         }
@@ -385,6 +402,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
           }
       }
     }
+    store_held();
   }
 
   // The k groups' sums, [k group][token][row], over the rings

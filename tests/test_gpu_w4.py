@@ -264,15 +264,17 @@ def test_feed_forward_of_quantized_weights(pkg, backend, rows):
     plain.check(host(y), *plain.product(host(h), wide[2], step), "bf16")
 
 
-@pytest.mark.parametrize("rows", [1, 40, 260])
-def test_same_results_every_run_and_on_two_streams(pkg, backend, rows):
+@pytest.mark.parametrize("n, zeros", [(600, False), (601, True), (4002, True)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 6, 12, 40, 260])
+def test_same_results_every_run_and_on_two_streams(pkg, backend, rows, dtype, n, zeros):
     rng = np.random.default_rng([13, rows])
-    w = Weight(pkg, rng, 600, 2048, 128, False)
-    x = device(values(rng, (rows, 2048), "bf16"), "bf16")
+    w = Weight(pkg, rng, n, 2048, 128, zeros)
+    x = device(values(rng, (rows, 2048), dtype), dtype)
     first = pkg.linear_w4(backend, x, w.handle)
     torch.cuda.synchronize()
     streams, outs = [torch.cuda.Stream() for _ in range(2)], []
-    for _ in range(5):
+    for _ in range(20):
         for s in streams:
             with torch.cuda.stream(s):
                 outs.append(pkg.linear_w4(backend, x, w.handle))
