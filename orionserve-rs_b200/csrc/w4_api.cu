@@ -66,9 +66,12 @@ int check_product(int dtype, const void *x, uint64_t rows, uint64_t x_stride, co
   return ORION_OK;
 }
 
-// The tiles of tcgen05 take bf16 products of more rows than this, and of at least a stage of k.
-constexpr uint64_t kFewRows = 16;
-bool takes_tiles(int dtype, uint64_t rows, uint64_t k) { return dtype == ORION_DTYPE_BF16 && rows > kFewRows && k >= 256; }
+// Whether a product runs in tiles on tcgen05 (w4_tiles.cu), which needs bf16 and a stage of 256 k, or in the kernel for few rows. The tiles need a kernel ahead
+// of theirs and some 9 us until the first of them is done; the others' rate is that of mma.sync. Times in us, tiles / few, linear 2048 x 2048: 16 rows
+// 12 / 8, 64 rows 12 / 11, 128 rows 16 / 21; 8192 x 8192: 16 rows 19 / 15, 17 rows 19 / 28; 1024 x 2048: 128 rows 14 / 11, 256 rows 19 / 21.
+bool takes_tiles(int dtype, uint64_t rows, uint64_t weight_rows, uint64_t k) {
+  return dtype == ORION_DTYPE_BF16 && rows > 16 && k >= 256 && (double)(rows > 48 ? rows : 48) * (double)weight_rows * (double)k > 268435456.0;
+}
 
 // Address of the projections' error word, looked up once per device.
 int error_word(int device, uint32_t **word) {
@@ -83,12 +86,13 @@ int error_word(int device, uint32_t **word) {
 }
 
 int launch(int device, int dtype, const W4Call &c, void *workspace, uint64_t workspace_bytes, cudaStream_t stream) {
-  if (!takes_tiles(dtype, c.rows, c.k)) {
+  const uint32_t weight_rows = c.up.packed ? 2 * c.n : c.n;
+  if (!takes_tiles(dtype, c.rows, weight_rows, c.k)) {
     ScopedDevice current(device);
     ORION_CUDA_CHECK("set device", current.status);
     return dtype == ORION_DTYPE_F32 ? launch_w4_few<float>(c, stream) : launch_w4_few<bf16>(c, stream);
   }
-  const uint64_t need = w4_tiles_workspace(c.rows, c.up.packed ? 2 * c.n : c.n, c.k, c.group);
+  const uint64_t need = w4_tiles_workspace(c.rows, weight_rows, c.k, c.group);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return set_error(ORION_ERR_INVALID_REQUEST, "a workspace of %llu bytes on a 256-byte boundary is needed, got %llu", (unsigned long long)need,
                      (unsigned long long)(workspace ? workspace_bytes : 0));
@@ -135,7 +139,8 @@ int orion_cuda_w4_workspace(int dtype, uint64_t rows, const OrionW4Weight *weigh
   ORION_TRY(check_dtype(dtype));
   ORION_TRY(check_weight("weight", weight));
   if (rows > kMostRows) return set_error(ORION_ERR_INVALID_REQUEST, "%llu rows: at most 2^30 are possible", (unsigned long long)rows);
-  if (takes_tiles(dtype, rows, weight->in_features)) *bytes = w4_tiles_workspace((uint32_t)rows, (uint32_t)weight->out_features * (gated ? 2 : 1), (uint32_t)weight->in_features, weight->group);
+  const uint64_t weight_rows = weight->out_features * (gated ? 2 : 1);
+  if (takes_tiles(dtype, rows, weight_rows, weight->in_features)) *bytes = w4_tiles_workspace((uint32_t)rows, (uint32_t)weight_rows, (uint32_t)weight->in_features, weight->group);
   return ORION_OK;
 }
 

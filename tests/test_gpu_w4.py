@@ -44,8 +44,13 @@ def host(t):
     return t.double().cpu().numpy()
 
 
+def sizes(rows):
+    """(n, k) of a product that runs in tiles where its rows are more than 16: of one CTA each to 128 rows, of pairs beyond."""
+    return (140, 512) if rows <= 16 else (2602, 2176) if rows <= 64 else (1302, 2112) if rows <= 128 else (902, 1088)
+
+
 ROWS = [1, 2, 7, 8, 9, 16, 17, 31, 33, 64, 65, 130, 257, 300]
-SHAPES = [(1, 32, 32), (15, 128, 128), (17, 96, 32), (33, 64, 64), (100, 352, 32), (256, 1024, 128), (1001, 4160, 64), (130, 8192, 128)]
+SHAPES = [(1, 32, 32), (15, 128, 128), (17, 96, 32), (33, 64, 64), (100, 352, 32), (256, 1024, 128), (1001, 4160, 64), (130, 8192, 128), (2051, 2752, 64), (1400, 4384, 32)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -146,20 +151,21 @@ def test_quantize_strided_rows(pkg, backend):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("rows", [1, 5, 20, 50, 300])
+@pytest.mark.parametrize("rows", [1, 5, 20, 50, 100, 300])
 def test_infinities_and_nan_stay_in_their_rows(pkg, backend, rows, dtype):
     rng = np.random.default_rng([7, rows])
-    w, up = Weight(pkg, rng, 130, 256, 64, True), Weight(pkg, rng, 130, 256, 64, False)
-    x = values(rng, (rows, 256), dtype)
+    n, k = sizes(rows)
+    w, up = Weight(pkg, rng, n, k, 64, True), Weight(pkg, rng, n, k, 64, False)
+    x = values(rng, (rows, k), dtype)
     clean = host(pkg.linear_w4(backend, device(x, dtype), w.handle))
     x[0, 3] = np.inf
     if rows > 2:
         x[1, 70], x[2, 5], x[2, 9] = np.nan, np.inf, -np.inf
     with np.errstate(invalid="ignore"):
         # a code that equals its zero point makes the product of an infinity a NaN
-        want = np.stack([(r[None, :] * w.w).sum(1) for r in x])
+        want = np.stack([(r[None, :] * w.w).sum(1) for r in x[:3]] + [np.zeros(n)] * (rows - 3))
     got = host(pkg.linear_w4(backend, device(x, dtype), w.handle))
-    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(np.isnan(got[:3]), np.isnan(want[:3]))
     assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
     np.testing.assert_array_equal(got[3:], clean[3:])
     y = host(pkg.gated_w4(backend, device(x, dtype), w.handle, up.handle))
@@ -167,13 +173,14 @@ def test_infinities_and_nan_stay_in_their_rows(pkg, backend, rows, dtype):
     assert np.isfinite(y[3:]).all()
 
 
-@pytest.mark.parametrize("rows", [3, 20, 300])
+@pytest.mark.parametrize("rows", [3, 20, 100, 300])
 @pytest.mark.parametrize("scale", [1e-30, 1e-4, 1e4, 1e30])
 def test_rows_of_any_magnitude(pkg, backend, rows, scale):
     """Rows and outputs whose sizes differ by many powers of ten come out as exact as others."""
     rng = np.random.default_rng([8, rows])
-    w = Weight(pkg, rng, 140, 512, 128, True)
-    x = values(rng, (rows, 512), "bf16")
+    n, k = sizes(rows)
+    w = Weight(pkg, rng, n, k, 64 if k % 128 else 128, True)
+    x = values(rng, (rows, k), "bf16")
     x[0] = plain.to_bf16(x[0] * scale)
     x[1, 17] = plain.to_bf16(np.float64(1e5))
     x[2] = 0.0
@@ -181,47 +188,50 @@ def test_rows_of_any_magnitude(pkg, backend, rows, scale):
     plain.check(host(pkg.linear_w4(backend, device(x, "bf16"), w.handle)), want, bound, "bf16")
 
 
-@pytest.mark.parametrize("rows", [1, 20, 300])
+@pytest.mark.parametrize("rows", [1, 20, 100, 300])
 def test_outputs_of_any_magnitude(pkg, backend, rows):
     rng = np.random.default_rng([9, rows])
-    w = Weight(pkg, rng, 140, 512, 128, True)
+    n, k = sizes(rows)
+    w = Weight(pkg, rng, n, k, 64, True)
     w.scales[:, 0] = plain.to_bf16(w.scales[:, 0] * 2.0 ** -60)
     w.scales[:, 1] = plain.to_bf16(w.scales[:, 1] * 2.0 ** 60)
     w.scales[1, 2] = 0.0
     w.scales[:, 3] = 0.0
     w.scales[2, 4] *= 2.0 ** -20
-    handle = pkg.W4Weight(w.handle.packed, device(w.scales, "bf16"), w.handle.zeros, 128)
-    x = values(rng, (rows, 512), "bf16")
-    want, bound = plain.product(x, plain.dequantize(w.codes, w.scales, w.zeros, 128), w.step(rows, "bf16"))
+    handle = pkg.W4Weight(w.handle.packed, device(w.scales, "bf16"), w.handle.zeros, 64)
+    x = values(rng, (rows, k), "bf16")
+    want, bound = plain.product(x, plain.dequantize(w.codes, w.scales, w.zeros, 64), w.step(rows, "bf16"))
     plain.check(host(pkg.linear_w4(backend, device(x, "bf16"), handle)), want, bound, "bf16")
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("rows", [1, 6, 40, 270])
+@pytest.mark.parametrize("rows", [1, 6, 14, 40, 120, 270])
 def test_strided_rows_and_neighbours_of_the_output(pkg, backend, rows, dtype):
     rng = np.random.default_rng([10, rows])
-    w = Weight(pkg, rng, 77, 320, 64, True)
-    x = values(rng, (rows, 320), dtype)
-    wide = torch.full((rows, 352), float("nan"), dtype=DTYPES[dtype], device="cuda")
-    wide[:, 16:336] = device(x, dtype)
-    out = torch.full((rows + 2, 99), -7.0, dtype=DTYPES[dtype], device="cuda")
-    got = pkg.linear_w4(backend, wide[:, 16:336], w.handle, out=out[1:rows + 1, 11:88])
+    n, k = sizes(rows)
+    n -= 3
+    w = Weight(pkg, rng, n, k, 64, True)
+    x = values(rng, (rows, k), dtype)
+    wide = torch.full((rows, k + 32), float("nan"), dtype=DTYPES[dtype], device="cuda")
+    wide[:, 16:k + 16] = device(x, dtype)
+    out = torch.full((rows + 2, n + 22), -7.0, dtype=DTYPES[dtype], device="cuda")
+    got = pkg.linear_w4(backend, wide[:, 16:k + 16], w.handle, out=out[1:rows + 1, 11:n + 11])
     assert got.data_ptr() == out[1:, 11:].data_ptr()
     plain.check(host(got), *plain.product(x, w.w, w.step(rows, dtype)), dtype)
     rest = host(out)
-    rest[1:rows + 1, 11:88] = -7.0
+    rest[1:rows + 1, 11:n + 11] = -7.0
     assert (rest == -7.0).all()
 
 
-@pytest.mark.parametrize("rows", [1, 12, 48, 290])
+@pytest.mark.parametrize("rows", [1, 12, 100, 290])
 def test_captured_and_replayed(pkg, backend, rows):
     """A run of the operators as a feed-forward uses them, in two graphs that are replayed in turn with new inputs, on a stream of its own."""
     rng = np.random.default_rng([11, rows])
+    width, hidden = (256, 320) if rows <= 16 else (1088, 2624)
     gate, up, down = (pkg.quantize_w4(backend, device(values(rng, s, "bf16", 0.05), "bf16"), group=64, zeros=z)
-                      for s, z in (((352, 256), True), ((352, 256), True), ((256, 352 // 64 * 64 + 0), False)))
-    hidden = 352 // 64 * 64
+                      for s, z in (((hidden + 32, width), True), ((hidden + 32, width), True), ((width, hidden), False)))
     stream = torch.cuda.Stream()
-    x = [device(values(rng, (rows, 256), "bf16"), "bf16") for _ in range(2)]
+    x = [device(values(rng, (rows, width), "bf16"), "bf16") for _ in range(2)]
 
     def block(v):
         return pkg.linear_w4(backend, pkg.gated_w4(backend, v, gate, up)[:, :hidden], down)
@@ -236,7 +246,7 @@ def test_captured_and_replayed(pkg, backend, rows):
             outs.append(block(v))
         graphs.append(g)
     for turn in range(3):
-        fresh = [device(values(rng, (rows, 256), "bf16"), "bf16") for _ in x]
+        fresh = [device(values(rng, (rows, width), "bf16"), "bf16") for _ in x]
         for v, f in zip(x, fresh):
             v.copy_(f)
         torch.cuda.synchronize()
@@ -251,11 +261,12 @@ def test_captured_and_replayed(pkg, backend, rows):
 def test_feed_forward_of_quantized_weights(pkg, backend, rows):
     """quantise three matrices, gated product, down projection: against the same in 64 bits with the codes that the quantiser must give."""
     rng = np.random.default_rng([12, rows])
-    shapes = ((448, 256), (448, 256), (256, 448))
+    width, hidden = (256, 448) if rows <= 16 else (1088, 2624)
+    shapes = ((hidden, width), (hidden, width), (width, hidden))
     raw = [values(rng, s, "f32", s[1] ** -0.5) for s in shapes]
     w = [pkg.quantize_w4(backend, device(r, "f32"), group=64, zeros=True) for r in raw]
     wide = [plain.dequantize(*plain.quantize(r, 64, True)[:2], plain.quantize(r, 64, True)[2], 64) for r in raw]
-    x = values(rng, (rows, 256), "bf16")
+    x = values(rng, (rows, width), "bf16")
     h = pkg.gated_w4(backend, device(x, "bf16"), w[0], w[1])
     step = plain.weight_step(rows, "bf16", True)
     want, bound = plain.gated("silu", x, wide[0], wide[1], step, step)
@@ -264,7 +275,7 @@ def test_feed_forward_of_quantized_weights(pkg, backend, rows):
     plain.check(host(y), *plain.product(host(h), wide[2], step), "bf16")
 
 
-@pytest.mark.parametrize("n, zeros", [(600, False), (601, True), (4002, True)])
+@pytest.mark.parametrize("n, zeros", [(600, False), (601, True), (4002, True), (4004, False)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("rows", [1, 6, 12, 40, 260])
 def test_same_results_every_run_and_on_two_streams(pkg, backend, rows, dtype, n, zeros):

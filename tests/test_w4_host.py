@@ -65,7 +65,7 @@ def test_other_refusals(pkg):
 @pytest.mark.parametrize("is_gated", [0, 1])
 def test_workspaces(pkg, is_gated):
     """What a call for many rows needs, and that it is refused with less; few rows and f32 need nothing."""
-    lib, bad, w, need = pkg._ffi.lib(), pkg._ffi.ERR_INVALID_REQUEST, weight(pkg, in_features=512), C.c_uint64(5)
+    lib, bad, w, need = pkg._ffi.lib(), pkg._ffi.ERR_INVALID_REQUEST, weight(pkg, in_features=512, out_features=4096), C.c_uint64(5)
     for dtype, rows in ((0, 1), (0, 5000), (2, 1), (2, 8), (2, 0)):
         assert lib.orion_cuda_w4_workspace(dtype, rows, C.addressof(w), is_gated, C.byref(need)) == pkg._ffi.ORION_OK and need.value == 0
     last = 0
@@ -74,7 +74,7 @@ def test_workspaces(pkg, is_gated):
         assert need.value >= rows * 512 * 2 and need.value > last
         last, call = need.value, gated if is_gated else linear
         for space, size in ((0, 0), (0, last), (P, last - 1), (P + 128, last)):
-            assert call(pkg, w, rows=rows, stride=512, space=space, size=size, **({"up": w} if is_gated else {})) == bad
+            assert call(pkg, w, rows=rows, stride=512, out_stride=4096, space=space, size=size, **({"up": w} if is_gated else {})) == bad
     assert lib.orion_cuda_w4_workspace(1, 8, C.addressof(w), 0, C.byref(need)) == bad
     assert lib.orion_cuda_w4_workspace(2, 1 << 31, C.addressof(w), 0, C.byref(need)) == bad
     assert lib.orion_cuda_w4_workspace(2, 8, None, 0, C.byref(need)) == bad
