@@ -492,12 +492,13 @@ void orion_cuda_attn_bench_destroy(OrionAttnBench *bench);
  * W[n][k] = (code - zero) * scale, codes and zeros 0..15, with one scale and one zero point for every `group` (32, 64 or
  * 128) consecutive k of a row. All pointers are DEVICE pointers; the calls check what can be checked on the host, allocate
  * nothing, only enqueue work on `stream` (a cudaStream_t, NULL = the default stream) of `device`, which is current during the
- * call and put back, and can be captured into a graph. They hold no state: calls on different streams and from different
+ * call and put back, and can be captured into a graph (the first call of a kind on a device sets its kernel up: make it
+ * before a capture). They hold no state: calls on different streams and from different
  * threads do not touch one another, given workspaces of their own. Results do not vary from run to run. A bounded wait inside
  * the kernels for many rows that gives up sets the device's word of the projections (orion_cuda_poll_wait_timeouts, bit 0).
  *   packed  u32 [out_features][in_features / 8], 16-byte aligned. Of eight consecutive k, number 2i is in bits 4i .. 4i + 3
  *           of their word, number 2i + 1 in bits 16 + 4i .. 19 + 4i.
- *   scales  bf16 [in_features / group][out_features], 4-byte aligned
+ *   scales  bf16 [in_features / group][out_features], 4-byte aligned; 0, normal numbers, infinities or NaN
  *   zeros   u8, laid out like scales, 4-byte aligned; NULL: 8 everywhere (the symmetric form). Values above 15 are not allowed.
  * in_features is a multiple of `group`. Rows of values have unit stride and start on 16-byte boundaries. */
 typedef struct OrionW4Weight {

@@ -3,13 +3,12 @@
 ``W[n][k] = (code - zero) * scale`` with a bf16 scale, and in the asymmetric form a zero point, per group of 32, 64 or 128 consecutive ``k`` of a row.
 Codes are packed eight to an int32: of eight consecutive ``k``, number ``2i`` is in bits ``4i .. 4i + 3``, number ``2i + 1`` in bits ``16 + 4i ..
 19 + 4i``. The functions stand beside ``ops.linear`` and ``ops.swiglu`` for tensors that are on the device already: they run on torch's current
-stream of the tensors' device, allocate what they return and, for many rows, a workspace, and can be captured into a CUDA graph. Activations are f32 or bf16. Nothing here
-has a gradient; tensors that require one are refused.
+stream of the tensors' device, allocate what they return and, for many rows, a workspace, and can be captured into a CUDA graph once a call of
+the same kind and size has been made outside of one. Activations are f32 or bf16. Nothing here has a gradient; tensors that require one are refused.
 """
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional
 
 from . import _ffi
 from .backend import CudaBackend
@@ -113,6 +112,19 @@ def _rows(backend: CudaBackend, x, weight: W4Weight):
     return dtype, x.shape[0], stride
 
 
+def _overlap(a, b):
+    """Whether two matrices of one type, their rows' values neighbours, share a byte; those of unequal row strides also where one lies between the other's rows."""
+    size = a.element_size()
+    at, bt = a.data_ptr(), b.data_ptr()
+    if bt >= at + ((a.shape[0] - 1) * a.stride(0) + a.shape[1]) * size or at >= bt + ((b.shape[0] - 1) * b.stride(0) + b.shape[1]) * size:
+        return False
+    stride = a.stride(0) * size
+    if stride != b.stride(0) * size or a.shape[0] == 1:
+        return True
+    apart = (bt - at) % stride
+    return apart < a.shape[1] * size or apart + b.shape[1] * size > stride
+
+
 def _output(x, out, rows, n):
     if out is None:
         return _empty((rows, n), (n, 1), dtype=x.dtype, device=x.device), n
@@ -120,6 +132,8 @@ def _output(x, out, rows, n):
         raise InvalidRequest(f"out: a {x.dtype} tensor of shape [{rows}, {n}] on {x.device} is needed, its rows' values neighbours")
     if out.requires_grad and _torch.is_grad_enabled():
         raise InvalidRequest("out: 4-bit operators have no gradient")
+    if rows and _overlap(x, out):
+        raise InvalidRequest("out: overlaps x")
     return out, out.stride(0)
 
 
@@ -160,6 +174,8 @@ def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
         _on_device("bias", bias, _torch.float32, (n,))
         if bias.get_device() != backend._ordinal:
             raise InvalidRequest(f"bias must be on the backend's device {backend._ordinal}")
+        if bias.requires_grad and _torch.is_grad_enabled():
+            raise InvalidRequest("bias: 4-bit operators have no gradient")
     out, out_stride = _output(x, out, rows, n)
     space, at, size = _workspace(x, dtype, rows, weight, 0)
     check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, weight._address, None if bias is None else bias.data_ptr(), out.data_ptr(),

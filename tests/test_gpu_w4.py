@@ -326,7 +326,15 @@ def test_refusals(pkg, backend):
                 torch.zeros((64, 4), dtype=torch.bfloat16, device="cuda").t()):
         with bad:
             pkg.linear_w4(backend, x, w, out=out)
-    for bias in (torch.zeros(64, dtype=torch.bfloat16, device="cuda"), torch.zeros(63, device="cuda"), torch.zeros(64), torch.zeros(128, device="cuda")[::2]):
+    square = Weight(pkg, rng, 128, 128, 32, False).handle
+    room = torch.zeros((12, 128), dtype=torch.bfloat16, device="cuda")
+    for a, b in ((room[:4], room[:4]), (room[:4], room[3:7]), (room[4:8], room[1:5]), (room[2:10:2], room[4:12:2])):
+        with bad:
+            pkg.linear_w4(backend, a, square, out=b)
+    wide = torch.zeros((4, 256), dtype=torch.bfloat16, device="cuda")
+    for a, b in ((room[:4], room[4:8]), (room[2:10:2], room[3:11:2]), (wide[:, :128], wide[:, 128:]), (wide[:, 128:], wide[:, :128])):
+        pkg.linear_w4(backend, a, square, out=b)
+    for bias in (torch.zeros(64, dtype=torch.bfloat16, device="cuda"), torch.zeros(64, device="cuda", requires_grad=True), torch.zeros(63, device="cuda"), torch.zeros(64), torch.zeros(128, device="cuda")[::2]):
         with bad:
             pkg.linear_w4(backend, x, w, bias=bias)
     with bad:
