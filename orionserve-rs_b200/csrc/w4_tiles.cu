@@ -641,7 +641,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * F::kAccCols;
       const uint32_t r = j.w_row + rank * Pair::kRows + (warp & 3) * 32 + lane, row = GATED ? r >> 1 : r;
       const bool inside = row < c.n;
-      const float row_unit = ws.w_unit[r];
+      const float row_unit = ws.w_unit[r] * 0.0625f;  // 2^-4 is left of the powers that scales (2^14), codes (2^-24) and tokens (2^14) were brought to
       const float bias = !GATED && inside && c.bias && plan.splits == 1 ? c.bias[row] : 0.f;
       if (!wait(&acc_full[buf], (turn >> 1) & 1)) { ok = false; break; }
       tc_fence_after();
@@ -662,36 +662,41 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         tmem_ld_wait();
         if (mb + kStep >= j.cols) release();
         const uint32_t token = j.x_row + mb;
-        float v[16];  // 2^-4 is left of the powers that scales (2^14), codes (2^-24) and tokens (2^14) were brought to
+        float v[16];
 #pragma unroll
         for (uint32_t q = 0; q < 4; ++q) {
           const float4 f = *reinterpret_cast<const float4 *>(ws.x_unit + token + 4 * q);
-          v[4 * q] = __uint_as_float(rr[4 * q]) * 0.0625f * row_unit * f.x, v[4 * q + 1] = __uint_as_float(rr[4 * q + 1]) * 0.0625f * row_unit * f.y;
-          v[4 * q + 2] = __uint_as_float(rr[4 * q + 2]) * 0.0625f * row_unit * f.z, v[4 * q + 3] = __uint_as_float(rr[4 * q + 3]) * 0.0625f * row_unit * f.w;
+          v[4 * q] = __uint_as_float(rr[4 * q]) * row_unit * f.x, v[4 * q + 1] = __uint_as_float(rr[4 * q + 1]) * row_unit * f.y;
+          v[4 * q + 2] = __uint_as_float(rr[4 * q + 2]) * row_unit * f.z, v[4 * q + 3] = __uint_as_float(rr[4 * q + 3]) * row_unit * f.w;
         }
+        // a lane's column of values, `count` of them there, `step` elements apart
+        auto store = [&](auto *p, uint64_t step, uint32_t count, uint32_t most, auto value) {
+          if (count >= most) {
+#pragma unroll
+            for (uint32_t q = 0; q < 16; ++q, p += step)
+              if (q < most) *p = value(q);
+          } else {
+#pragma unroll
+            for (uint32_t q = 0; q < 16; ++q, p += step)
+              if (q < count) *p = value(q);
+          }
+        };
+        const uint32_t there = inside && token < c.rows ? c.rows - token : 0;
         if (!kPair && plan.splits > 1) {  // over the tokens, which nothing reads any more
-          float *p = reinterpret_cast<float *>(smem) + mb * Pair::kRows + (warp & 3) * 32 + lane;
-#pragma unroll
-          for (uint32_t q = 0; q < 16; ++q) p[q * Pair::kRows] = v[q];
+          store(reinterpret_cast<float *>(smem) + mb * Pair::kRows + (warp & 3) * 32 + lane, Pair::kRows, 16, 16, [&](uint32_t q) { return v[q]; });
         } else if (plan.splits > 1) {
-          float *p = ws.parts + ((uint64_t)j.split * c.rows + token) * weight_rows + r;
-#pragma unroll
-          for (uint32_t q = 0; q < 16; ++q)
-            if (inside && token + q < c.rows) p[(uint64_t)q * weight_rows] = v[q];
+          store(ws.parts + ((uint64_t)j.split * c.rows + token) * weight_rows + r, weight_rows, there, 16, [&](uint32_t q) { return v[q]; });
         } else if (GATED) {
           const bool odd = lane & 1;
-          bf16 *p = static_cast<bf16 *>(c.out) + (uint64_t)(token + (odd ? 8 : 0)) * c.ldo + row;
+          float other[8];
 #pragma unroll
-          for (uint32_t q = 0; q < 8; ++q) {
-            const float other = __shfl_xor_sync(0xffffffffu, odd ? v[q] : v[8 + q], 1);
-            const float y = gated<bf16>(GatedAct{c.act, 0.f}, odd ? other : v[q], odd ? v[8 + q] : other);
-            if (inside && token + (odd ? 8 : 0) + q < c.rows) p[q * c.ldo] = __float2bfloat16_rn(y);
-          }
+          for (uint32_t q = 0; q < 8; ++q) other[q] = __shfl_xor_sync(0xffffffffu, odd ? v[q] : v[8 + q], 1);
+          const uint32_t mine = odd ? there > 8 ? there - 8 : 0 : there;
+          store(static_cast<bf16 *>(c.out) + (uint64_t)(token + (odd ? 8 : 0)) * c.ldo + row, c.ldo, mine, 8, [&](uint32_t q) {
+            return __float2bfloat16_rn(gated<bf16>(GatedAct{c.act, 0.f}, odd ? other[q & 7] : v[q & 7], odd ? v[8 + (q & 7)] : other[q & 7]));
+          });
         } else {
-          bf16 *p = static_cast<bf16 *>(c.out) + (uint64_t)token * c.ldo + row;
-#pragma unroll
-          for (uint32_t q = 0; q < 16; ++q)
-            if (inside && token + q < c.rows) p[q * c.ldo] = __float2bfloat16_rn(v[q] + bias);
+          store(static_cast<bf16 *>(c.out) + (uint64_t)token * c.ldo + row, c.ldo, there, 16, [&](uint32_t q) { return __float2bfloat16_rn(v[q] + bias); });
         }
       }
     }
