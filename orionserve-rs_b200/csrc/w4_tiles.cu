@@ -6,11 +6,12 @@
 // registers, a round of stages ahead, and write the operand tiles of a CTA's 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
 //
 // The operands are f16, not bf16. (code - zero) * scale has at most 11 significant bits with a zero of 8 and 12 with any other, f16 holds 11: products are
-// exact, or off by 2^-12 of a weight, where bf16 would round every weight by 2^-9. Range is no matter, since both sides are scaled by powers of two, every
-// row of weights by the exponent of its largest scale and every token by that of its largest value (the same reason keeps every bf16 value exact in f16,
-// down to 2^-28 of the row's largest). A first kernel finds these exponents and converts the tokens; the epilogue scales back. Dequantisation costs a lane
-// 9 instructions for eight weights: the masked pairs, read as f16, are code * 2^-24 or code * 2^-20 (subnormal numbers and the first binade count in steps of
-// 2^-24), and one fused multiply-add each subtracts 8 and multiplies by the scale; zero points are subtracted first, which is exact.
+// exact, or off by 2^-12 of a weight, where bf16 would round every weight by 2^-9. For f16's range both sides are scaled by powers of two, every row of
+// weights by the exponent of its largest scale and every token by that of its largest value: weights keep their bits where their scale is above 2^-22 of the
+// row's largest, tokens down to 2^-31 of the largest value; what is smaller is off by at most 2^-30 of that scale, 2^-39 of that value. A first kernel
+// finds these exponents and converts the tokens; the epilogue scales back. Dequantisation costs a lane 13 instructions for eight weights: the masked pairs, read as f16, are code * 2^-24
+// or code * 2^-20 (subnormal numbers and the first binade count in steps of 2^-24), one fused multiply-add subtracts the zero point, which is exact, and one
+// multiplication applies the scale.
 //
 // Where tiles are too few for the device, k is cut as well: the parts are summed in order, of single CTAs over the distributed shared memory of a cluster, of
 // pairs by a third kernel, so results do not vary.
@@ -280,11 +281,6 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -299,22 +295,20 @@ __device__ __forceinline__ void umma_tmem_a(uint32_t tmem_d, uint32_t tmem_a, ui
       "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// 32 codes of a row, all of one group, as sixteen pairs in f16: (code - zero) * scale * 2^-24
-template <bool ZEROS>
+// 32 codes of a row, all of one group, as sixteen pairs in f16: (code - zero) * 2^-9 * scale. The difference first, which is exact: one fused multiply-add
+// of codes, scale and -8 * scale would save an instruction a pair where zeros are 8, but leaves a weight in steps of 2^-24, which are coarser than its last
+// bits where its scale is below 2^-7 of the row's largest; these are exact down to 2^-22 of it.
 __device__ __forceinline__ void dequant_piece(uint4 codes, uint32_t param, uint32_t *v) {
-  const uint32_t low = __byte_perm(param, 0, 0x1010), high = hmul2(low, 0x2c002c00u);  // of pairs in bits 0-3, and in bits 4-7: 1/16
-  const uint32_t eight = hmul2(low, 0x80088008u);                                     // -8 * 2^-24 * scale
-  const uint32_t zero = __byte_perm(param, 0, 0x3232), zero_high = zero << 4;
+  constexpr uint32_t kLow = 0x78007800u, kHigh = 0x68006800u;  // 2^15, 2^11: of pairs in bits 0-3, and in bits 4-7
+  const uint32_t scale = __byte_perm(param, 0, 0x1010), minus_zero = hmul2(__byte_perm(param, 0, 0x3232), 0xf800f800u);
   const uint32_t words[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
   for (uint32_t j = 0; j < 4; ++j) {
     const uint32_t rest = words[j] >> 8;
-    const uint32_t pairs[4] = {words[j] & 0x000f000fu, words[j] & 0x00f000f0u, rest & 0x000f000fu, rest & 0x00f000f0u};
-#pragma unroll
-    for (uint32_t q = 0; q < 4; ++q) {
-      if (ZEROS) v[4 * j + q] = hmul2(hsub2(pairs[q], q & 1 ? zero_high : zero), q & 1 ? high : low);
-      else v[4 * j + q] = hfma2(pairs[q], q & 1 ? high : low, eight);
-    }
+    v[4 * j] = hmul2(hfma2(words[j] & 0x000f000fu, kLow, minus_zero), scale);
+    v[4 * j + 1] = hmul2(hfma2(words[j] & 0x00f000f0u, kHigh, minus_zero), scale);
+    v[4 * j + 2] = hmul2(hfma2(rest & 0x000f000fu, kLow, minus_zero), scale);
+    v[4 * j + 3] = hmul2(hfma2(rest & 0x00f000f0u, kHigh, minus_zero), scale);
   }
 }
 __device__ __forceinline__ uint4 ld_codes(const uint8_t *p) {
@@ -333,7 +327,7 @@ __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, ui
 // f32 accumulation, f16 x f16
 __device__ __forceinline__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n) { return (1u << 4) | ((n >> 3) << 17) | ((m >> 4) << 24); }
 
-template <typename F, bool GATED, bool ZEROS>
+template <typename F, bool GATED>
 __global__ void __launch_bounds__(F::kWarps * 32, 1)
 w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                const __grid_constant__ CUtensorMap map_up, const Workspace ws, const Plan plan, const uint32_t param_rows, uint32_t *error) {
@@ -506,7 +500,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     const uint32_t code_row = GATED ? (in_tile & 1) * 64 + (in_tile >> 1) : in_tile, code_turn = F::kCodeRow == 128 ? code_row & 7 : (code_row >> 1) & 3;  // how TMA permutes rows of 128 and of 64 bytes
     const uint32_t code_from = smem_u32(smem + F::kCodeRing) + code_row * F::kCodeRow;
     const uint32_t to = tmem_base + (((warp & 3) * 32u) << 16) + F::kTmemWeights;
-    const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
+    const uint32_t group_bits = 31 - __clz((int)c.group), groups = c.k / c.group;
     pdl_wait();
 
     // Jobs and stages. The scales and zero points of the team's next stage are on their way while this one is made; they stay as loaded, since anything done
@@ -522,11 +516,13 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     };
     auto load = [&] {
       if (load_t >= total) return;
-      // beyond the last k the codes meet zeros: any scale does
+      // beyond the last k weights are zeros, as the tokens there
 #pragma unroll
       for (uint32_t i = 0; i < kPieces; ++i)
-        if (i % 4 == 0 || group_bits < 7 - (i & 1 ? 1 : 0))  // one, two or four groups in 128 k
-          next[i] = ld_params(ws.params + (uint64_t)min((load_kb * F::kStageK + i * 32) >> group_bits, last_group) * param_rows + load_row);
+        if (i % 4 == 0 || group_bits < 7 - (i & 1 ? 1 : 0)) {  // one, two or four groups in 128 k
+          const uint32_t group = (load_kb * F::kStageK + i * 32) >> group_bits;
+          next[i] = group < groups ? ld_params(ws.params + (uint64_t)group * param_rows + load_row) : 0u;
+        }
     };
     aim();
     for (uint32_t i = 0; i < team; ++i) advance();
@@ -554,7 +550,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         for (uint32_t half = 0; half < 2; ++half) {
           uint32_t v[32];
 #pragma unroll
-          for (uint32_t i = 0; i < 2; ++i) dequant_piece<ZEROS>(codes[half * 2 + i], param[i0 + half * 2 + i], &v[i * 16]);
+          for (uint32_t i = 0; i < 2; ++i) dequant_piece(codes[half * 2 + i], param[i0 + half * 2 + i], &v[i * 16]);
           tmem_st32(to + s * F::kTmemStage + (i0 + half * 2) * 16, v);
         }
       }
@@ -573,7 +569,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     constexpr uint32_t kTurn = GATED ? 1 : 2;
     const bool turned = piece >= 2;
     const uint32_t to = smem_u32(w_ring) + (piece >> 1) * Pair::kWSlab + in_tile * 128, chunk = (((piece & 1) * 4) ^ (turned ? kTurn : 0) ^ (in_tile & 7)) * 16;
-    const uint32_t group_bits = 31 - __clz((int)c.group), last_group = c.k / c.group - 1;
+    const uint32_t group_bits = 31 - __clz((int)c.group), groups = c.k / c.group;
     const uint8_t *packed = reinterpret_cast<const uint8_t *>(GATED && (in_tile & 1) ? c.up.packed : c.w.packed);
     const uint64_t set_step = (uint64_t)c.k / 2 * (8 / kMatrices);
 
@@ -588,7 +584,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     };
     auto load_codes = [&] {
       if (load_t >= total) return;
-      // beyond the last k the codes meet zeros: any do
+      // beyond the last k scales and tokens are zeros: any codes do
       const uint32_t row = load_row / kMatrices, at = min(load_kb * (Pair::kStageK / 2) + piece * 16, c.k / 2 - 16);
       const uint8_t *p = packed + (uint64_t)row * (c.k / 2) + at;
 #pragma unroll
@@ -599,9 +595,10 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
     };
     auto load = [&] {
       if (load_t >= total) return;
-      const uint32_t *p = ws.params + (uint64_t)min((load_kb * Pair::kStageK + piece * 32) >> group_bits, last_group) * param_rows + load_row;
+      const uint32_t group = (load_kb * Pair::kStageK + piece * 32) >> group_bits;
+      const uint32_t *p = ws.params + (uint64_t)group * param_rows + load_row;
 #pragma unroll
-      for (uint32_t i = 0; i < 4; ++i) next[i] = ld_params(p + i * 8);
+      for (uint32_t i = 0; i < 4; ++i) next[i] = group < groups ? ld_params(p + i * 8) : 0u;
     };
     aim();
     for (uint32_t i = 0; i < team; ++i) advance();
@@ -623,7 +620,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       for (uint32_t i = 0; i < 4; ++i) {
         uint32_t v[16];
         const uint4 w = codes[i];
-        dequant_piece<ZEROS>(!turned ? w : kTurn == 1 ? make_uint4(w.y, w.x, w.w, w.z) : make_uint4(w.z, w.w, w.x, w.y), param[i], v);
+        dequant_piece(!turned ? w : kTurn == 1 ? make_uint4(w.y, w.x, w.w, w.z) : make_uint4(w.z, w.w, w.x, w.y), param[i], v);
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) sts128(to + s * Pair::kWBytes + i * 8 * 128 + (chunk ^ (j * 16)), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
       }
@@ -641,7 +638,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * F::kAccCols;
       const uint32_t r = j.w_row + rank * Pair::kRows + (warp & 3) * 32 + lane, row = GATED ? r >> 1 : r;
       const bool inside = row < c.n;
-      const float row_unit = ws.w_unit[r] * 0.0625f;  // 2^-4 is left of the powers that scales (2^14), codes (2^-24) and tokens (2^14) were brought to
+      const float row_unit = ws.w_unit[r] * 0x1p-19f;  // what is left of the powers that scales (2^14), codes (2^-9) and tokens (2^14) were brought to
       const float bias = !GATED && inside && c.bias && plan.splits == 1 ? c.bias[row] : 0.f;
       if (!wait(&acc_full[buf], (turn >> 1) & 1)) { ok = false; break; }
       tc_fence_after();
@@ -783,10 +780,10 @@ int matrix_map(CUtensorMap *map, bool bytes, CUtensorMapSwizzle swizzle, const v
   return ORION_OK;
 }
 
-template <typename F, bool GATED, bool ZEROS>
+template <typename F, bool GATED>
 int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
   static bool done[kMaxDeviceOrdinals] = {};
-  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_tile_kernel<F, GATED, ZEROS>, F::kSmemBytes, done));
+  ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(w4_tile_kernel<F, GATED>, F::kSmemBytes, done));
   const uint32_t matrices = GATED ? 2 : 1;
   CUtensorMap map_x, map_w, map_up;
   ORION_TRY(matrix_map(&map_x, false, CU_TENSOR_MAP_SWIZZLE_128B, ws.x, c.rows, c.k, Pair::kSlabK, plan.tokens / F::kCtas));
@@ -799,7 +796,7 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   const uint32_t jobs = plan.tiles_w * plan.tiles_x * plan.splits;
   const uint32_t param_rows = (uint32_t)padded_rows(c.n * matrices), token_blocks = c.rows > 512 ? (c.rows + kPrepWarps - 1) / kPrepWarps : c.rows;
   ORION_CUDA_CHECK("4-bit product", launch_pdl(w4_prepare_kernel, dim3(token_blocks + param_rows / 32), dim3(kPrepThreads), 0, stream, c, ws, matrices, param_rows, token_blocks));
-  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED, ZEROS>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(F::kWarps * 32),
+  ORION_CUDA_CHECK("4-bit product", launch_pdl_cluster(w4_tile_kernel<F, GATED>, dim3(F::kCtas * std::min(jobs, kSms / F::kCtas)), dim3(F::kWarps * 32),
                                                        dim3(F::kCtas == 1 ? plan.splits : F::kCtas, 1, 1), F::kSmemBytes, stream, c, map_x, map_w, map_up, ws, plan, param_rows, error));
   count_launch();
   count_launch();
@@ -811,11 +808,11 @@ int launch_form(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t
   return ORION_OK;
 }
 
-template <bool GATED, bool ZEROS>
+template <bool GATED>
 int launch_kind(const W4Call &c, const Workspace &ws, const Plan &plan, uint32_t *error, cudaStream_t stream) {
-  if (plan.ctas == 2) return launch_form<Paired, GATED, ZEROS>(c, ws, plan, error, stream);
-  if (plan.tokens > Single64::kAccCols) return launch_form<Single128, GATED, ZEROS>(c, ws, plan, error, stream);
-  return launch_form<Single64, GATED, ZEROS>(c, ws, plan, error, stream);
+  if (plan.ctas == 2) return launch_form<Paired, GATED>(c, ws, plan, error, stream);
+  if (plan.tokens > Single64::kAccCols) return launch_form<Single128, GATED>(c, ws, plan, error, stream);
+  return launch_form<Single64, GATED>(c, ws, plan, error, stream);
 }
 
 }  // namespace
@@ -833,9 +830,7 @@ int launch_w4_tiles(const W4Call &c, void *workspace, uint32_t *error, cudaStrea
     return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
   uint64_t bytes = 0;
   const Workspace ws = workspace_at(static_cast<uint8_t *>(workspace), c.rows, weight_rows, c.k, c.group, plan, &bytes);
-  const bool zeros = c.w.zeros || c.up.zeros;
-  if (c.up.packed) return zeros ? launch_kind<true, true>(c, ws, plan, error, stream) : launch_kind<true, false>(c, ws, plan, error, stream);
-  return zeros ? launch_kind<false, true>(c, ws, plan, error, stream) : launch_kind<false, false>(c, ws, plan, error, stream);
+  return c.up.packed ? launch_kind<true>(c, ws, plan, error, stream) : launch_kind<false>(c, ws, plan, error, stream);
 }
 
 }  // namespace orion

@@ -204,6 +204,44 @@ def test_outputs_of_any_magnitude(pkg, backend, rows):
     plain.check(host(pkg.linear_w4(backend, device(x, "bf16"), handle)), want, bound, "bf16")
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("rows", [1, 20, 100, 300])
+def test_groups_of_any_magnitude(pkg, backend, rows, zeros):
+    """Groups of a row whose scales differ by up to 2^19 and whose tokens make up for it, so that every group counts as much."""
+    rng = np.random.default_rng([17, rows])
+    n, k = sizes(rows)
+    w = Weight(pkg, rng, n, k, 32, zeros)
+    power = np.arange(k // 32) * 7 % 20
+    scales = w.scales * 2.0 ** -power[:, None]
+    handle = pkg.W4Weight(w.handle.packed, device(scales, "bf16"), w.handle.zeros, 32)
+    x = values(rng, (rows, k), "bf16") * np.repeat(2.0 ** power, 32)
+    want, bound = plain.product(x, plain.dequantize(w.codes, scales, w.zeros, 32), w.step(rows, "bf16"))
+    plain.check(host(pkg.linear_w4(backend, device(x, "bf16"), handle)), want, bound, "bf16")
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 20, 100, 300])
+def test_an_infinite_scale_reaches_its_output_alone(pkg, backend, rows, dtype, zeros):
+    """The last group's, behind which a tile of k is not filled; a scale of NaN likewise."""
+    rng = np.random.default_rng([18, rows])
+    n, k = sizes(rows)
+    w = Weight(pkg, rng, n, k, 32, zeros)
+    x = values(rng, (rows, k), dtype)
+    x[:, -32:] = np.abs(x[:, -32:]) + 1.0
+    clean = host(pkg.linear_w4(backend, device(x, dtype), w.handle))
+    w.codes[[3, 4], -32:] = [[15], [0]]
+    if zeros:
+        w.zeros[-1, [3, 4]] = 7
+    w.scales[-1, [3, 4]] = np.inf
+    w.scales[1, 5] = np.nan
+    handle = pkg.W4Weight(torch.tensor(plain.pack(w.codes)).cuda(), device(w.scales, "bf16"), None if w.zeros is None else torch.tensor(w.zeros, dtype=torch.uint8).cuda(), 32)
+    got = host(pkg.linear_w4(backend, device(x, dtype), handle))
+    assert (got[:, 3] == np.inf).all() and (got[:, 4] == -np.inf).all() and np.isnan(got[:, 5]).all()
+    clean[:, 3:6] = got[:, 3:6] = 0.0
+    np.testing.assert_array_equal(got, clean)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("rows", [1, 6, 14, 40, 120, 270])
 def test_strided_rows_and_neighbours_of_the_output(pkg, backend, rows, dtype):
@@ -346,6 +384,14 @@ def test_refusals(pkg, backend):
                  (w.packed, w.scales[:, :63], None, 32), (w.packed[0], w.scales, None, 32), (w.packed, w.scales.t().contiguous().t(), None, 32)):
         with bad:
             pkg.W4Weight(*args)
+    learned = w.scales.clone().requires_grad_()
+    with bad:
+        pkg.W4Weight(w.packed, learned, None, 32)
+    with bad:
+        pkg.quantize_w4(backend, x.float().requires_grad_(), group=32)
+    with torch.no_grad():
+        pkg.W4Weight(w.packed, learned, None, 32)
+        pkg.quantize_w4(backend, x.float().requires_grad_(), group=32)
     with bad:
         pkg.W4Weight.from_codes(torch.full((64, 128), 16, device="cuda"), w.scales, None, 32)
     for v, g in ((x.half(), 32), (x.cpu(), 32), (x, 48), (x[:, :96].contiguous(), 64), (x[0], 32), (x[:0], 32), (x.t(), 4)):
