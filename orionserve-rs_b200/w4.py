@@ -4,7 +4,8 @@
 Codes are packed eight to an int32: of eight consecutive ``k``, number ``2i`` is in bits ``4i .. 4i + 3``, number ``2i + 1`` in bits ``16 + 4i ..
 19 + 4i``. The functions stand beside ``ops.linear`` and ``ops.swiglu`` for tensors that are on the device already: they run on torch's current
 stream of the tensors' device, allocate what they return and, for many rows, a workspace, and can be captured into a CUDA graph once a call of
-the same kind and size has been made outside of one. Activations are f32 or bf16. Nothing here has a gradient; tensors that require one are refused.
+the same kind and size has been made outside of one. Activations are f32 or bf16. Nothing here has a gradient; tensors that require
+one are refused, unless gradients are off (``torch.no_grad()``).
 """
 from __future__ import annotations
 
@@ -42,6 +43,8 @@ def _on_device(name, t, dtype, shape=None):
         raise InvalidRequest(f"{name}: shape {shape} is needed, got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise InvalidRequest(f"{name}: not contiguous")
+    if t.requires_grad and _torch.is_grad_enabled():
+        raise InvalidRequest(f"{name}: 4-bit operators have no gradient")
 
 
 class W4Weight:
@@ -174,8 +177,6 @@ def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
         _on_device("bias", bias, _torch.float32, (n,))
         if bias.get_device() != backend._ordinal:
             raise InvalidRequest(f"bias must be on the backend's device {backend._ordinal}")
-        if bias.requires_grad and _torch.is_grad_enabled():
-            raise InvalidRequest("bias: 4-bit operators have no gradient")
     out, out_stride = _output(x, out, rows, n)
     space, at, size = _workspace(x, dtype, rows, weight, 0)
     check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, weight._address, None if bias is None else bias.data_ptr(), out.data_ptr(),
@@ -216,6 +217,8 @@ def quantize_w4(backend: CudaBackend, weight, group: int = 128, zeros: bool = Fa
     n, k = weight.shape
     if group not in GROUPS or n == 0 or k == 0 or k % group != 0:
         raise InvalidRequest(f"a matrix of {n} x {k} has no whole groups of {group} (32, 64 or 128)")
+    if weight.requires_grad and _torch.is_grad_enabled():
+        raise InvalidRequest("weight: 4-bit operators have no gradient")
     if weight.stride(1) != 1:
         raise InvalidRequest("weight: the values of a row must be neighbours")
     w = W4Weight.__new__(W4Weight)
