@@ -331,6 +331,31 @@ def test_same_results_every_run_and_on_two_streams(pkg, backend, rows, dtype, n,
     assert all(torch.equal(first, o) for o in outs)
 
 
+def test_offsets_beyond_32_bits(pkg, backend):
+    """Matrices of more than 2^33 weights, rows of activations and of outputs more than 2^32 bytes apart in all: what repeats in one comes back repeated."""
+    period, times, k = 1024, 520, 16384
+    rng = np.random.default_rng(19)
+    base = torch.randn((period, k), generator=torch.Generator("cuda").manual_seed(19), device="cuda").to(torch.bfloat16)
+    n = period * times
+    w = pkg.quantize_w4(backend, base.repeat(times, 1), group=64, zeros=True)
+    one = pkg.quantize_w4(backend, base, group=64, zeros=True)
+    assert w.packed.numel() * 4 > 1 << 32
+    for whole, part in ((w.packed.view(times, period, -1), one.packed), (w.scales.view(-1, times, period).transpose(0, 1), one.scales),
+                        (w.zeros.view(-1, times, period).transpose(0, 1), one.zeros)):
+        assert all(torch.equal(v, part) for v in whole)
+    plain_w = plain.dequantize(plain.unpack(one.packed.cpu().numpy()), host(one.scales), host(one.zeros), 64)
+    for rows, apart in ((3, 1 << 30), (20, 1 << 27), (140, 1 << 24)):
+        x = values(rng, (rows, k), "bf16")
+        wide = torch.empty(((rows - 1) * apart + k,), dtype=torch.bfloat16, device="cuda").as_strided((rows, k), (apart, 1))
+        wide.copy_(device(x, "bf16"))
+        room = torch.empty(((rows - 1) * apart + n,), dtype=torch.bfloat16, device="cuda").as_strided((rows, n), (apart, 1))
+        got = pkg.linear_w4(backend, wide, w, out=room)
+        first = got[:, :period]
+        assert all(torch.equal(got[:, i * period:(i + 1) * period], first) for i in range(times))
+        plain.check(host(first), *plain.product(x, plain_w, plain.weight_step(rows, "bf16", True)), "bf16", f"{rows} rows")
+        del wide, room, got, first
+
+
 def test_no_rows_and_values_written_in_place(pkg, backend):
     rng = np.random.default_rng(14)
     w = Weight(pkg, rng, 64, 128, 32, False)
