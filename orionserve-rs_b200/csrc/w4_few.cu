@@ -8,7 +8,9 @@
 // fma(pair, 2^120 or 2^116, -zero * 2^-13) = (code - zero) * 2^-13, exactly.
 //
 // f32 activations go through the same instructions as three bf16 terms of eight bits each (hi + mid + lo = x exactly), so f32 results have f32 accuracy.
-// The warps that share a slab of tokens make its terms together (211 rows of k 2048 to 5504 outputs: 98 us with each warp making its own).
+// The warps that share a slab of tokens make its terms together (211 rows of k 2048 to 5504 outputs: 98 us with each warp making its own, 90 together). More than
+// 16 rows are bound by these instructions, so two CTAs share an SM there too (512 rows of k 4096 to 14336: 734 us with one of up to 210 registers a thread,
+// 562 with two of 128; 211 rows as above 90 and 79).
 //
 // A CTA of eight warps: WR of them side by side over weight rows, 8 / WR groups of them over k. Few tokens: WR = 1, every warp streams k slabs of its own
 // and only reads the tokens' values it needs; more tokens: warps share the tokens' slab, so that L2 delivers it less often. Each k group has a ring of
@@ -108,6 +110,7 @@ __device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __by
 
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
 struct FewConfig {
+  static_assert(RT % (GATED ? 2 : 1) == 0, "with a gate half of a warp's tiles are the gate's");
   static constexpr uint32_t kKGroups = kWarps / WR;
   static constexpr uint32_t kTileRows = 16 * RT * WR;                       // rows of weights per CTA, gate and up together
   static constexpr uint32_t kMatrices = GATED ? 2 : 1;
@@ -120,16 +123,18 @@ struct FewConfig {
   static constexpr uint32_t kScaleRow = kOutputs * 2, kZeroRow = kOutputs;  // scales, and zero points, of a group and matrix
   static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + (ZEROS ? kZeroRow : 0));
   static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows * 4;     // bytes of the sums that meet in shared memory, over the rings
-  // Slabs in the ring: with few tokens two CTAs share an SM, with many one takes what there is.
-  static constexpr uint32_t kStages = kSlab == 256 ? 2 : NT <= 2 || sizeof(T) == 4 ? 3 : 4;
+  // Two CTAs share an SM, but for 9 to 16 tokens in f32 and more than 16 in bf16, and the ring has as many slabs as there is room for.
+  static constexpr bool kTwo = NT == 1 || (sizeof(T) == 4 ? NT == 4 : NT == 2);
+  static constexpr uint32_t kStages = kSlab == 256 || (sizeof(T) == 4 && NT == 4 && RT == 2) ? 2 : NT <= 2 || sizeof(T) == 4 ? 3 : 4;
   static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kRings = kKGroups * kStages * kStage;
   // f32 tokens of the slab at hand, in bf16 terms: [term][token][k]
   static constexpr uint32_t kTermRow = kSlab * 2, kTerms = sizeof(T) == 4 ? 3 * kTokens * kTermRow : 0, kAll = kRings + kKGroups * kTerms;
   static constexpr uint32_t kSmem = kAll > kSums ? kAll : kSums;
+  static_assert(kSmem <= (kTwo ? 113 * 1024 : 227 * 1024), "rings exceed the shared memory of an SM");
 };
 
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
-__global__ void __launch_bounds__(kThreads, NT == 1 || (NT == 2 && sizeof(T) == 2) ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>::kTwo ? 2 : 1)
 w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   using Cfg = FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   constexpr bool kF32 = sizeof(T) == 4;
@@ -477,7 +482,15 @@ int launch_shape(const W4Call &c, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
     if (c.rows > 32) return launch_config<T, GATED, ZEROS, GROUP, 2, 8, 8>(c, stream);
   }
-  return launch_config<T, GATED, ZEROS, GROUP, 2, 4, 4>(c, stream);
+  if constexpr (sizeof(T) == 2) {
+    return launch_config<T, GATED, ZEROS, GROUP, 2, 4, 4>(c, stream);
+  } else {
+    if constexpr (!GATED) {  // narrow tiles where wide ones would not fill the device: 24 rows of k 4096 to 4096 17 us, 26 with wide ones; 512 to 14336 604 and 562
+      const uint64_t wide = (uint64_t)((c.n + 255) / 256) * ((c.rows + 31) / 32);
+      if (wide < 296) return launch_config<T, GATED, ZEROS, GROUP, 1, 4, 8>(c, stream);
+    }
+    return launch_config<T, GATED, ZEROS, GROUP, 2, 4, 8>(c, stream);
+  }
 }
 
 template <typename T, bool GATED, bool ZEROS>
