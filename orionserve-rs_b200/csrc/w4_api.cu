@@ -67,10 +67,11 @@ int check_product(int dtype, const void *x, uint64_t rows, uint64_t x_stride, co
 }
 
 // Whether a product runs in tiles on tcgen05 (w4_tiles.cu), which needs bf16 and a stage of 256 k, or in the kernel for few rows. The tiles need a kernel ahead
-// of theirs and some 9 us until the first of them is done; the others' rate is that of mma.sync. Times in us, tiles / few, linear 2048 x 2048: 16 rows
-// 12 / 8, 64 rows 12 / 11, 128 rows 16 / 21; 8192 x 8192: 16 rows 19 / 15, 17 rows 19 / 28; 1024 x 2048: 128 rows 14 / 11, 256 rows 19 / 21.
+// of theirs and some 9 us until the first of them is done; the others' rate is that of mma.sync. Times in us, tiles / few, weights from HBM: k 2048 to 2048,
+// 64 rows 14 / 9, 192 rows 18 / 16, 400 rows 19 / 26; k 4096 to 4096, 32 rows 14 / 10, 64 rows 16 / 15, 128 rows 19 / 23; k 3584 to 4608, 64 rows 15 / 17;
+// k 2048 to 16384, 24 rows 14 / 16, 128 rows 19 / 40.
 bool takes_tiles(int dtype, uint64_t rows, uint64_t weight_rows, uint64_t k) {
-  return dtype == ORION_DTYPE_BF16 && rows > 16 && k >= 256 && (double)(rows > 48 ? rows : 48) * (double)weight_rows * (double)k > 268435456.0;
+  return dtype == ORION_DTYPE_BF16 && rows > 16 && k >= 256 && (double)(rows > 48 ? rows : 48) * (double)weight_rows * (double)k > 1e9;
 }
 
 // Address of the projections' error word, looked up once per device.

@@ -12,11 +12,16 @@
 // 16 rows are bound by these instructions, so two CTAs share an SM there too (512 rows of k 4096 to 14336: 734 us with one of up to 210 registers a thread,
 // 562 with two of 128; 211 rows as above 90 and 79).
 //
-// A CTA of eight warps: WR of them side by side over weight rows, 8 / WR groups of them over k. Few tokens: WR = 1, every warp streams k slabs of its own
-// and only reads the tokens' values it needs; more tokens: warps share the tokens' slab, so that L2 delivers it less often. Each k group has a ring of
-// slabs of 128 or 256 k, weights, tokens and scales, filled by cp.async (no waits on barriers). A CTA has one tile: CTAs that went from tile to tile, the
-// rings running ahead, left more of the device idle at the end (8 rows of k 4096 to 128256 outputs: 68 us against 62). Sums of k groups meet in shared memory, and where the rows of weights give too few CTAs the k of a tile is dealt to the CTAs of a cluster, whose sums meet over
-// distributed shared memory: in both places in a fixed order, so results do not vary from run to run, and no workspace is needed.
+// A CTA of eight warps, two CTAs to an SM: WR warps side by side over weight rows, 8 / WR groups of them over k. Few tokens: WR = 4, and the tokens' slab of a
+// k group serves 128 rows; more tokens: all eight warps share it, so that L2 delivers it less often. Each k group has a ring of slabs of 128 or 256 k, weights,
+// tokens and scales, filled by cp.async (no waits on barriers). A CTA has one tile: CTAs that went from tile to tile, the rings running ahead, left more of
+// the device idle at the end (8 rows of k 4096 to 128256 outputs: 68 us against 62). Sums of k groups meet in shared memory, and where the rows of weights
+// give too few CTAs the k of a tile is dealt to the CTAs of a cluster, whose sums meet over distributed shared memory: in both places in a fixed order, so
+// results do not vary from run to run, and no workspace is needed.
+//
+// Measured: 8 rows of k 4096 to 128256 outputs 64 to 67 us, 4.2 to 4.4 TB/s (0.64 to 0.67 of a copy's rate), 1 row of k 4096 with a gate to 14336 16.7 us,
+// 3.6 TB/s. Instructions are issued in 54 % of all cycles (k 4096 to 32768: 17 for the eight weights of a lane, nine of which are the dequantisation), from
+// 16 warps to an SM that also wait for each other's slabs: neither bound is reached alone. Of many f32 rows mma.sync is the bound, three terms a product.
 #include "kernels.h"
 #include "mma.cuh"
 #include "w4.cuh"
@@ -123,18 +128,17 @@ struct FewConfig {
   static constexpr uint32_t kScaleRow = kOutputs * 2, kZeroRow = kOutputs;  // scales, and zero points, of a group and matrix
   static constexpr uint32_t kSStage = kMatrices * kPerSlab * (kScaleRow + (ZEROS ? kZeroRow : 0));
   static constexpr uint32_t kSums = kKGroups * kTokens * kTileRows * 4;     // bytes of the sums that meet in shared memory, over the rings
-  // Two CTAs share an SM, but for 9 to 16 tokens in f32 and more than 16 in bf16, and the ring has as many slabs as there is room for.
-  static constexpr bool kTwo = NT == 1 || (sizeof(T) == 4 ? NT == 4 : NT == 2);
+  // Slabs in the ring: what leaves room for two CTAs in an SM.
   static constexpr uint32_t kStages = kSlab == 256 || (sizeof(T) == 4 && NT == 4 && RT == 2) ? 2 : NT <= 2 || sizeof(T) == 4 ? 3 : 4;
   static constexpr uint32_t kStage = kWStage + kTokens * kXRow + kSStage, kRings = kKGroups * kStages * kStage;
   // f32 tokens of the slab at hand, in bf16 terms: [term][token][k]
   static constexpr uint32_t kTermRow = kSlab * 2, kTerms = sizeof(T) == 4 ? 3 * kTokens * kTermRow : 0, kAll = kRings + kKGroups * kTerms;
   static constexpr uint32_t kSmem = kAll > kSums ? kAll : kSums;
-  static_assert(kSmem <= (kTwo ? 113 * 1024 : 227 * 1024), "rings exceed the shared memory of an SM");
+  static_assert(kSmem <= 113 * 1024, "rings of two CTAs exceed the shared memory of an SM");
 };
 
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
-__global__ void __launch_bounds__(kThreads, FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>::kTwo ? 2 : 1)
+__global__ void __launch_bounds__(kThreads, 2)
 w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   using Cfg = FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   constexpr bool kF32 = sizeof(T) == 4;
@@ -452,21 +456,36 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
   if (ranks > 1) cluster_barrier();  // nobody leaves while its sums are being read
 }
 
+template <typename Cfg>
+uint32_t tiles_m_of(const W4Call &c) { return (c.rows + Cfg::kTokens - 1) / Cfg::kTokens; }
+template <typename Cfg>
+uint64_t tiles_of(const W4Call &c) { return (uint64_t)((c.n + Cfg::kOutputs - 1) / Cfg::kOutputs) * tiles_m_of<Cfg>(c); }
+
+// CTAs that share the k of a tile, a cluster of up to eight where there are few tiles: as many as are at work together, two to an SM, less those that would
+// not shorten the most slabs a k group has. A cluster starts when it has room for all of its CTAs, so one too many costs a second turn: 64 rows of k 3584 to
+// 4608 outputs (36 tiles) take 40, 33, 29, 21, 20, 18, 17 and 21 us with one to eight, 1 row of k 4096 to 28672 (224 tiles) 18, 30 with two and 45 with four.
+template <typename Cfg>
+uint32_t ranks_of(const W4Call &c) {
+  const uint64_t tiles = tiles_of<Cfg>(c);
+  const uint32_t slabs = (c.k + Cfg::kSlab - 1) / Cfg::kSlab;
+  auto steps = [&](uint32_t ranks) { return (slabs + Cfg::kKGroups * ranks - 1) / (Cfg::kKGroups * ranks); };
+  uint32_t ranks = 1;
+  for (uint32_t r = 2; r <= 8 && tiles * r <= 256; ++r)
+    if (steps(r) < steps(ranks)) ranks = r;
+  return ranks;
+}
+template <typename Cfg>
+uint64_t ctas_of(const W4Call &c) { return tiles_of<Cfg>(c) * ranks_of<Cfg>(c); }
+
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t RT, uint32_t NT, uint32_t WR>
 int launch_config(const W4Call &c, cudaStream_t stream) {
   using Cfg = FewConfig<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   static bool done[kMaxDeviceOrdinals] = {};
   const auto kernel = w4_few_kernel<T, GATED, ZEROS, GROUP, RT, NT, WR>;
   ORION_CUDA_CHECK("4-bit product", ensure_dynamic_smem(kernel, (int)Cfg::kSmem, done));
-  const uint32_t tiles_n = (c.n + Cfg::kOutputs - 1) / Cfg::kOutputs, tiles_m = (c.rows + Cfg::kTokens - 1) / Cfg::kTokens;
-  const uint64_t tiles = (uint64_t)tiles_n * tiles_m;
+  const uint32_t tiles_m = tiles_m_of<Cfg>(c), ranks = ranks_of<Cfg>(c);
+  const uint64_t tiles = tiles_of<Cfg>(c);
   if (tiles > 0x7fffffffull) return set_error(ORION_ERR_INVALID_REQUEST, "4-bit product: %u rows x %u outputs are too many for one call", c.rows, c.n);
-  // k over a cluster of up to eight CTAs where there are few tiles, as long as every k group has a slab. A cluster starts when it has room for all of its
-  // CTAs, so it is not for launches that fill the device anyway: 1 row of k 14336 to 4096 outputs (32 tiles) takes 33 us with one CTA a tile, 15 with
-  // four, 11 with eight, of k 4096 to 28672 (224 tiles) 18, 30 and 45.
-  const uint32_t slabs = (c.k + Cfg::kSlab - 1) / Cfg::kSlab;
-  uint32_t ranks = 1;
-  while (ranks < 8 && tiles * ranks * 2 <= 256 && slabs >= Cfg::kKGroups * ranks * 2) ranks *= 2;
   if (ranks == 1)
     ORION_CUDA_CHECK("4-bit product", launch_pdl(kernel, dim3((uint32_t)tiles), dim3(kThreads), Cfg::kSmem, stream, c, tiles_m));
   else
@@ -475,22 +494,30 @@ int launch_config(const W4Call &c, cudaStream_t stream) {
   return ORION_OK;
 }
 
+// Eight warps side by side: tiles of 256 rows, or of 128 where the CTAs of the wide ones would not fill the device (f32, 24 rows of k 4096 to 4096: 17 us, 26
+// with wide ones; 12 rows of k 4096 to 14336: 32 and 27). A gate needs two tiles a warp.
+template <typename T, bool GATED, bool ZEROS, uint32_t GROUP, uint32_t NT>
+int launch_wide(const W4Call &c, cudaStream_t stream) {
+  if constexpr (!GATED) {
+    if (ctas_of<FewConfig<T, GATED, ZEROS, GROUP, 2, NT, 8>>(c) < 224) return launch_config<T, GATED, ZEROS, GROUP, 1, NT, 8>(c, stream);
+  }
+  return launch_config<T, GATED, ZEROS, GROUP, 2, NT, 8>(c, stream);
+}
+
 template <typename T, bool GATED, bool ZEROS, uint32_t GROUP>
 int launch_shape(const W4Call &c, cudaStream_t stream) {
   if (c.rows <= 8) return launch_config<T, GATED, ZEROS, GROUP, 2, 1, 4>(c, stream);
-  if (c.rows <= 16) return launch_config<T, GATED, ZEROS, GROUP, 2, 2, 4>(c, stream);
   if constexpr (sizeof(T) == 2) {
-    if (c.rows > 32) return launch_config<T, GATED, ZEROS, GROUP, 2, 8, 8>(c, stream);
-  }
-  if constexpr (sizeof(T) == 2) {
-    return launch_config<T, GATED, ZEROS, GROUP, 2, 4, 4>(c, stream);
-  } else {
-    if constexpr (!GATED) {  // narrow tiles where wide ones would not fill the device: 24 rows of k 4096 to 4096 17 us, 26 with wide ones; 512 to 14336 604 and 562
-      const uint64_t wide = (uint64_t)((c.n + 255) / 256) * ((c.rows + 31) / 32);
-      if (wide < 296) return launch_config<T, GATED, ZEROS, GROUP, 1, 4, 8>(c, stream);
+    if (c.rows <= 16) return launch_config<T, GATED, ZEROS, GROUP, 2, 2, 4>(c, stream);
+    if constexpr (!GATED) {
+      // 64 tokens a tile unless 32 give more CTAs and the device is not full
+      using Long = FewConfig<T, GATED, ZEROS, GROUP, 1, 8, 8>;
+      if (c.rows > 32 && ctas_of<Long>(c) >= std::min<uint64_t>(148, ctas_of<FewConfig<T, GATED, ZEROS, GROUP, 1, 4, 8>>(c))) return launch_config<T, GATED, ZEROS, GROUP, 1, 8, 8>(c, stream);
     }
-    return launch_config<T, GATED, ZEROS, GROUP, 2, 4, 8>(c, stream);
+  } else {
+    if (c.rows <= 16) return launch_wide<T, GATED, ZEROS, GROUP, 2>(c, stream);
   }
+  return launch_wide<T, GATED, ZEROS, GROUP, 4>(c, stream);
 }
 
 template <typename T, bool GATED, bool ZEROS>

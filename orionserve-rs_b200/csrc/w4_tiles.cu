@@ -1,7 +1,9 @@
 // Products with 4-bit weights for many rows of bf16 activations (w4.cuh has the layout): persistent CTA pairs on tcgen05, weights dequantised on their way
 // into shared memory.
 //
-// From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05. A pair of CTAs works as one MMA unit on 256 weight rows x
+// From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05: 4096 rows of k 4096 with a gate to 14336 take 742 us, 1.3
+// PFLOP/s (0.93 of a library product's rate at the power limit); 64 rows of k 3584 with a gate to 18944 35 us, of which the weights' way from HBM is 12 and the first
+// kernel, which is not hidden, some 7. A pair of CTAs works as one MMA unit on 256 weight rows x
 // up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: teams of warps read them into
 // registers, a round of stages ahead, and write the operand tiles of a CTA's 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.
 //
@@ -78,8 +80,8 @@ struct Plan {
 // cluster, all parts of a launch at once; of pairs they are written and read again.
 Plan make_plan(uint32_t rows, uint32_t weight_rows, uint32_t k) {
   // CTAs of one to an SM that are at work together in clusters of so many, with the SMs of a GPC that are left over (36 clusters of four took two turns, 22 us
-  // instead of 12 for 32 of them)
-  constexpr uint32_t kClustered[9] = {0, 148, 144, 132, 128, 120, 126, 112, 112};
+  // instead of 12 for 32 of them; 16 of seven 31, 16 of six 20)
+  constexpr uint32_t kClustered[9] = {0, 148, 144, 132, 128, 120, 126, 105, 112};
   Plan best;
   double cost = 1e300;
   const uint32_t ctas = rows <= Single128::kAccCols ? 1 : 2, units = kSms / ctas;

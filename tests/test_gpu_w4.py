@@ -1,4 +1,6 @@
 """4-bit weights on the device: quantiser, projection, gated feed-forward, against plain 64-bit forms."""
+import functools
+
 import numpy as np
 import pytest
 
@@ -45,8 +47,8 @@ def host(t):
 
 
 def sizes(rows):
-    """(n, k) of a product that runs in tiles where its rows are more than 16: of one CTA each to 128 rows, of pairs beyond."""
-    return (140, 512) if rows <= 16 else (2602, 2176) if rows <= 64 else (1302, 2112) if rows <= 128 else (902, 1088)
+    """(n, k) of a product that runs in tiles where its rows are more than 16, or 100 of more than 64: of one CTA each to 128 rows, of pairs beyond."""
+    return (140, 512) if rows <= 16 else (5602, 4160) if rows <= 64 else (2602, 4160) if rows <= 128 else (1002, 4160)
 
 
 ROWS = [1, 2, 7, 8, 9, 16, 17, 31, 33, 64, 65, 130, 257, 300]
@@ -81,7 +83,38 @@ def test_gated(pkg, backend, rows, dtype, act):
         plain.check(host(got), *plain.gated(act, x, gate.w, up.w, gate.step(rows, dtype), up.step(rows, dtype)), dtype, f"{rows} x {k} to {n}, groups of {group}")
 
 
-@pytest.mark.parametrize("rows, n, k", [(3, 38000, 160), (14, 39001, 128), (30, 38001, 288), (100, 39000, 256), (129, 20001, 384), (1100, 6001, 512), (520, 20000, 160)])
+@functools.lru_cache(maxsize=None)
+def large_weight(pkg, n, k, group, zeros, seed):
+    return Weight(pkg, np.random.default_rng([n, zeros, seed]), n, k, group, zeros)
+
+
+LARGE = [(5602, 4128, 32), (3001, 7488, 64), (4097, 5504, 128)]
+
+
+@pytest.mark.parametrize("n, k, group", LARGE)
+@pytest.mark.parametrize("rows", [17, 33, 64, 65, 100, 128, 130])
+def test_linear_of_large_matrices(pkg, backend, rows, n, k, group):
+    rng = np.random.default_rng([20, rows, n])
+    for zeros in (False, True):
+        w = large_weight(pkg, n, k, group, zeros, 0)
+        x, bias = values(rng, (rows, k), "bf16"), values(rng, n, "f32")
+        got = pkg.linear_w4(backend, device(x, "bf16"), w.handle, bias=device(bias, "f32"))
+        want, bound = plain.product(x, w.w, w.step(rows, "bf16"))
+        plain.check(host(got), want + bias, bound + 2.0 ** -23 * (np.abs(want) + np.abs(bias)), "bf16")
+
+
+@pytest.mark.parametrize("n, k, group", LARGE)
+@pytest.mark.parametrize("rows", [17, 64, 65, 128, 130])
+def test_gated_of_large_matrices(pkg, backend, rows, n, k, group):
+    x = values(np.random.default_rng([21, rows, n]), (rows, k), "bf16", 0.5)
+    for act, zeros in (("silu", (False, True)), ("gelu_tanh", (True, False)), ("silu", (False, False))):
+        gate, up = (large_weight(pkg, n, k, group, z, i) for i, z in enumerate(zeros))
+        got = pkg.gated_w4(backend, device(x, "bf16"), gate.handle, up.handle, activation=act)
+        plain.check(host(got), *plain.gated(act, x, gate.w, up.w, gate.step(rows, "bf16"), up.step(rows, "bf16")), "bf16")
+
+
+@pytest.mark.parametrize("rows, n, k", [(3, 38000, 160), (14, 39001, 128), (30, 38001, 288), (100, 39000, 256), (129, 20001, 384), (1100, 6001, 512), (520, 20000, 160),
+                                        (30, 78001, 288), (100, 42000, 288), (129, 22001, 384)])
 def test_more_tiles_than_the_device_takes_at_once(pkg, backend, rows, n, k):
     """Resident CTAs go from tile to tile, their rings running on."""
     rng = np.random.default_rng([rows, n])
@@ -313,7 +346,7 @@ def test_feed_forward_of_quantized_weights(pkg, backend, rows):
     plain.check(host(y), *plain.product(host(h), wide[2], step), "bf16")
 
 
-@pytest.mark.parametrize("n, zeros", [(600, False), (601, True), (4002, True), (4004, False)])
+@pytest.mark.parametrize("n, zeros", [(600, False), (601, True), (4002, True), (4004, False), (11201, True), (11204, False)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("rows", [1, 6, 12, 40, 260])
 def test_same_results_every_run_and_on_two_streams(pkg, backend, rows, dtype, n, zeros):

@@ -69,7 +69,7 @@ def test_workspaces(pkg, is_gated):
     for dtype, rows in ((0, 1), (0, 5000), (2, 1), (2, 8), (2, 0)):
         assert lib.orion_cuda_w4_workspace(dtype, rows, C.addressof(w), is_gated, C.byref(need)) == pkg._ffi.ORION_OK and need.value == 0
     last = 0
-    for rows in (200, 1000, 5000, 70000):
+    for rows in (600, 1000, 5000, 70000):
         assert lib.orion_cuda_w4_workspace(2, rows, C.addressof(w), is_gated, C.byref(need)) == pkg._ffi.ORION_OK
         assert need.value >= rows * 512 * 2 and need.value > last
         last, call = need.value, gated if is_gated else linear
