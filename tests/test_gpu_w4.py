@@ -83,6 +83,22 @@ def test_gated(pkg, backend, rows, dtype, act):
         plain.check(host(got), *plain.gated(act, x, gate.w, up.w, gate.step(rows, dtype), up.step(rows, dtype)), dtype, f"{rows} x {k} to {n}, groups of {group}")
 
 
+@pytest.mark.parametrize("n, k", [(10880, 1536), (6528, 2560), (5376, 6144), (4608, 3584)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows", [1, 12, 40])
+def test_clusters_of_any_size(pkg, backend, rows, dtype, n, k):
+    """k dealt to 3, 5, 6 and 7 CTAs and to other numbers of them."""
+    rng = np.random.default_rng([22, rows, n])
+    w = Weight(pkg, rng, n, k, 128, zeros=rows == 12)
+    x = values(rng, (rows, k), dtype)
+    plain.check(host(pkg.linear_w4(backend, device(x, dtype), w.handle)), *plain.product(x, w.w, w.step(rows, dtype)), dtype)
+    half = n // 2
+    top, low = (pkg.W4Weight(w.handle.packed[i:i + half], w.handle.scales[:, i:i + half].contiguous(), None if w.zeros is None else w.handle.zeros[:, i:i + half].contiguous(), 128)
+                for i in (0, half))
+    step = w.step(rows, dtype)
+    plain.check(host(pkg.gated_w4(backend, device(x, dtype), top, low)), *plain.gated("silu", x, w.w[:half], w.w[half:], step, step), dtype)
+
+
 @functools.lru_cache(maxsize=None)
 def large_weight(pkg, n, k, group, zeros, seed):
     return Weight(pkg, np.random.default_rng([n, zeros, seed]), n, k, group, zeros)
