@@ -161,8 +161,9 @@ __device__ __forceinline__ void prepare_weights(const W4Call &c, const Workspace
 #pragma unroll
     for (uint32_t j = 0; j < kAtOnce; ++j) {
       const uint32_t g = first + j * kPrepWarps, p = scale[j], e = p >> 7 & 255u;
-      // infinities and NaN stay, what is far below the row's largest scale vanishes
-      const uint32_t f = e == 255u ? p << 16 : (int32_t)e + raise <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise << 23);
+      // infinities and NaN stay; 0 (whose exponent field would count as a power of two where the row's largest scale is small) and what is far below the row's
+      // largest scale vanish
+      const uint32_t f = e == 255u ? p << 16 : e == 0u || (int32_t)e + raise <= 127 - 30 ? 0u : (p << 16) + ((uint32_t)raise << 23);
       if (g < groups) ws.params[(uint64_t)g * param_rows + r] = (uint32_t)__half_as_ushort(__float2half_rn(__uint_as_float(f))) | zero[j] << 16;
     }
   }
