@@ -520,7 +520,7 @@ int orion_cuda_w4_workspace(int dtype, uint64_t rows, const OrionW4Weight *weigh
 /* y = x W^T + bias: tensor::linear (tensor.rs:96-130) with such weights. x and out hold values of `dtype` (f32 or bf16), rows
  * x_stride and out_stride values apart; bias is f32 [out_features] or NULL. Sums are held in f32 and rounded once; with
  * many rows of bf16 a weight is held in 11 bits (exact with a zero point of 8, else off by up to 2^-12 of itself), less what is
- * below 2^-30 of its row's largest scale. `out` overlaps no input. `workspace` (256-byte aligned, orion_cuda_w4_workspace bytes; NULL where that is 0) belongs to the call
+ * below 2^-29 of its row's largest scale. `out` overlaps no input. `workspace` (256-byte aligned, orion_cuda_w4_workspace bytes; NULL where that is 0) belongs to the call
  * until its work has ended; its contents need no preparation and are of no use afterwards. */
 int orion_cuda_w4_linear(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *weight,
                          const float *bias, void *out, uint64_t out_stride, void *workspace, uint64_t workspace_bytes,

@@ -9,8 +9,8 @@
 //
 // The operands are f16, not bf16. (code - zero) * scale has at most 11 significant bits with a zero of 8 and 12 with any other, f16 holds 11: products are
 // exact, or off by 2^-12 of a weight, where bf16 would round every weight by 2^-9. For f16's range both sides are scaled by powers of two, every row of
-// weights by the exponent of its largest scale and every token by that of its largest value: weights keep their bits where their scale is above 2^-22 of the
-// row's largest, tokens down to 2^-31 of the largest value; what is smaller is off by at most 2^-30 of that scale, 2^-39 of that value. A first kernel
+// weights by the exponent of its largest scale and every token by that of its largest value: weights keep their bits where their scale is above 2^-21 of the
+// row's largest, tokens down to 2^-30 of the largest value; what is smaller is off by at most 2^-29 of that scale, 2^-38 of that value. A first kernel
 // finds these exponents and converts the tokens; the epilogue scales back. Dequantisation costs a lane 13 instructions for eight weights: the masked pairs, read as f16, are code * 2^-24
 // or code * 2^-20 (subnormal numbers and the first binade count in steps of 2^-24), one fused multiply-add subtracts the zero point, which is exact, and one
 // multiplication applies the scale.
@@ -58,15 +58,18 @@ using Single64 = Form<1, 64, 256, 3>;
 using Single128 = Form<1, 128, 128, 4>;
 using Paired = Form<2, 128, 128, 3>;
 constexpr uint32_t kSms = 2 * kPairs;
-constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to
+constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to, or one less
 
 // What the first kernel leaves for the second, and the parts of k that the third one sums.
 struct Workspace {
   __half *x = nullptr;        // [rows][k], scaled
-  float *x_unit = nullptr;    // [rows, rounded up to 32] what a token was divided by, but for 2^kTop
+  // Square roots of what the epilogue multiplies a sum by: it does so with (row's x token's), twice. Both are at most 1 or both at least 1, so what is infinite
+  // or loses bits on the way would in the end; in other orders a scale of 2^124 and tokens of 2^-110 passed through infinities, and 2^-120 and 2^118 through
+  // subnormal numbers. So these powers of two are squares of others: rows and tokens are brought to within a factor of four instead of two.
+  float *x_unit = nullptr;    // [rows, rounded up to 32] of what a token was divided by, but for 2^kTop
   // Weight rows as tiles hold them: with a gate its rows and the other matrix's in turn. Rounded up to whole tiles.
-  float *w_unit = nullptr;    // [weight rows] 2^exponent of the largest scale
-  uint32_t *params = nullptr; // [k / group][weight rows] scale, in f16 and with the largest at 2^kTop .. 2^(kTop + 1), | zero << 16
+  float *w_unit = nullptr;    // [weight rows] likewise, with the powers that scales (2^14), codes (2^-9) and tokens (2^14) are brought to
+  uint32_t *params = nullptr; // [k / group][weight rows] scale, in f16 and with the largest at 2^(kTop - 1) .. 2^(kTop + 1), | zero << 16
   float *parts = nullptr;     // [splits][rows][weight rows]
 };
 
@@ -125,6 +128,8 @@ Workspace workspace_at(uint8_t *base, uint32_t rows, uint32_t weight_rows, uint3
 
 constexpr uint32_t kPrepThreads = 256, kPrepWarps = kPrepThreads / 32;
 
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+
 // 32 weight rows, their groups dealt to eight warps; eight groups of a thread's are on their way together.
 __device__ __forceinline__ void prepare_weights(const W4Call &c, const Workspace &ws, uint32_t matrices, uint32_t param_rows, uint32_t block) {
   constexpr uint32_t kAtOnce = 8;
@@ -155,6 +160,7 @@ __device__ __forceinline__ void prepare_weights(const W4Call &c, const Workspace
   __syncthreads();
 #pragma unroll
   for (uint32_t i = 0; i < kPrepWarps; ++i) top = max(top, tops[i][lane]);
+  top += top & 1;  // an odd power of two (its field in a float, 127 more, is even): with the 2^19 that the epilogue takes off too, a square
   const int32_t raise = top ? kTop + 127 - (int32_t)top : 0;
   for (uint32_t first = warp; first < groups; first += kAtOnce * kPrepWarps) {
     if (groups > kAtOnce * kPrepWarps) load(first);  // else they are still there
@@ -167,7 +173,7 @@ __device__ __forceinline__ void prepare_weights(const W4Call &c, const Workspace
       if (g < groups) ws.params[(uint64_t)g * param_rows + r] = (uint32_t)__half_as_ushort(__float2half_rn(__uint_as_float(f))) | zero[j] << 16;
     }
   }
-  if (warp == 0) ws.w_unit[r] = top ? __uint_as_float(top << 23) : 1.f;
+  if (warp == 0) ws.w_unit[r] = top ? power_of_two(((int)top - 127 - 19) / 2) : 1.f;
 }
 
 // A token, by THREADS threads (a block or a warp), HELD pieces of eight values each in registers.
@@ -201,9 +207,11 @@ __device__ __forceinline__ void prepare_token(const W4Call &c, const Workspace &
 #pragma unroll
     for (uint32_t i = 0; i < kPrepWarps; ++i) top = max(top, tops[i]);
   }
-  const int e = top == 0 ? 0 : top >= 0x80u ? (int)(top >> 7) - 127 : 31 - __clz((int)top) - 133, up = kTop - e, half = up / 2;
+  int e = top == 0 ? 0 : top >= 0x80u ? (int)(top >> 7) - 127 : 31 - __clz((int)top) - 133;
+  e += e & 1;
+  const int up = kTop - e, half = up / 2;
   // two factors: one alone would not be finite where the token's values are the smallest there are
-  const float f0 = __uint_as_float((uint32_t)(half + 127) << 23), f1 = __uint_as_float((uint32_t)(up - half + 127) << 23);
+  const float f0 = power_of_two(half), f1 = power_of_two(up - half);
   uint4 *out = reinterpret_cast<uint4 *>(ws.x + (uint64_t)m * c.k);
   for (uint32_t first = thread; first < pieces; first += HELD * THREADS) {
     if (pieces > HELD * THREADS) load(first);
@@ -219,7 +227,7 @@ __device__ __forceinline__ void prepare_token(const W4Call &c, const Workspace &
       if (first + j * THREADS < pieces) out[first + j * THREADS] = make_uint4(r[0], r[1], r[2], r[3]);
     }
   }
-  if (thread == 0) ws.x_unit[m] = ldexpf(1.f, e);
+  if (thread == 0) ws.x_unit[m] = power_of_two(e / 2);
 }
 
 // Blocks 0 .. token_blocks - 1 make tokens, one each or, of many tokens, one a warp: a block to a row is there sooner, a warp to a row needs no barrier so that more
@@ -300,7 +308,7 @@ __device__ __forceinline__ void umma_tmem_a(uint32_t tmem_d, uint32_t tmem_a, ui
 }
 // 32 codes of a row, all of one group, as sixteen pairs in f16: (code - zero) * 2^-9 * scale. The difference first, which is exact: one fused multiply-add
 // of codes, scale and -8 * scale would save an instruction a pair where zeros are 8, but leaves a weight in steps of 2^-24, which are coarser than its last
-// bits where its scale is below 2^-7 of the row's largest; these are exact down to 2^-22 of it.
+// bits where its scale is below 2^-7 of the row's largest; these are exact down to 2^-21 of it.
 __device__ __forceinline__ void dequant_piece(uint4 codes, uint32_t param, uint32_t *v) {
   constexpr uint32_t kLow = 0x78007800u, kHigh = 0x68006800u;  // 2^15, 2^11: of pairs in bits 0-3, and in bits 4-7
   const uint32_t scale = __byte_perm(param, 0, 0x1010), minus_zero = hmul2(__byte_perm(param, 0, 0x3232), 0xf800f800u);
@@ -641,7 +649,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
       const uint32_t buf = turn & 1, acc = tmem_base + (((warp & 3) * 32u) << 16) + buf * F::kAccCols;
       const uint32_t r = j.w_row + rank * Pair::kRows + (warp & 3) * 32 + lane, row = GATED ? r >> 1 : r;
       const bool inside = row < c.n;
-      const float row_unit = ws.w_unit[r] * 0x1p-19f;  // what is left of the powers that scales (2^14), codes (2^-9) and tokens (2^14) were brought to
+      const float row_unit = ws.w_unit[r];
       const float bias = !GATED && inside && c.bias && plan.splits == 1 ? c.bias[row] : 0.f;
       if (!wait(&acc_full[buf], (turn >> 1) & 1)) { ok = false; break; }
       tc_fence_after();
@@ -666,8 +674,9 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
 #pragma unroll
         for (uint32_t q = 0; q < 4; ++q) {
           const float4 f = *reinterpret_cast<const float4 *>(ws.x_unit + token + 4 * q);
-          v[4 * q] = __uint_as_float(rr[4 * q]) * row_unit * f.x, v[4 * q + 1] = __uint_as_float(rr[4 * q + 1]) * row_unit * f.y;
-          v[4 * q + 2] = __uint_as_float(rr[4 * q + 2]) * row_unit * f.z, v[4 * q + 3] = __uint_as_float(rr[4 * q + 3]) * row_unit * f.w;
+          const float unit[4] = {row_unit * f.x, row_unit * f.y, row_unit * f.z, row_unit * f.w};
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) v[4 * q + i] = __uint_as_float(rr[4 * q + i]) * unit[i] * unit[i];
         }
         // a lane's column of values, `count` of them there, `step` elements apart
         auto store = [&](auto *p, uint64_t step, uint32_t count, uint32_t most, auto value) {

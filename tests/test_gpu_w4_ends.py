@@ -69,3 +69,18 @@ def test_groups_of_scale_zero_have_no_weights(pkg, backend, rows, power, dtype):
     scales[np.arange(k // GROUP)[:, None] % 8 != np.arange(n)[None, :] % 8] = 0.0  # one group in eight is left
     size = 40 if power < 0 else 0
     compare(pkg, backend, values(rng, (rows, k), {"bf16": 8, "f32": 24}[dtype]) * 2.0 ** size, codes, scales, dtype, size)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("scale, token, rest", [(118, -100, 0), (124, -110, 0), (-126, 110, 0), (-120, 118, -24), (99, 48, -30), (60, 70, -20), (115, -120, -4), (-90, -20, 0)])
+@pytest.mark.parametrize("rows", [3, 20, 100, 300])
+def test_scales_and_tokens_of_opposite_ends(pkg, backend, rows, scale, token, rest, dtype):
+    """Scales of 2^scale, a largest token of 2^token whose weights are 0, others of 2^(token + rest), with codes that keep the largest sums finite. f32 tokens are
+    taken as multiples of 2^-133: those of less than 2^-109 have fewer than 24 bits, and here eight."""
+    rng = np.random.default_rng([32, rows, 200 + scale, 200 + token])
+    n, k = sizes(rows)
+    codes = rng.integers(7, 10, (n, k))
+    codes[:, 77] = 8
+    x = values(rng, (rows, k), 24 if dtype == "f32" and token + rest >= -109 else 8) * 2.0 ** (token + rest)
+    x[:, 77] = 2.0 ** token
+    compare(pkg, backend, x, codes, scales_near(rng, k // GROUP, n, scale), dtype, token + rest)
