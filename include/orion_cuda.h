@@ -518,10 +518,12 @@ int orion_cuda_w4_quantize(int device, int dtype, const void *weight, uint64_t o
  * `rows` rows: 0 for f32 and for few rows. */
 int orion_cuda_w4_workspace(int dtype, uint64_t rows, const OrionW4Weight *weight, int gated, uint64_t *bytes);
 /* y = x W^T + bias: tensor::linear (tensor.rs:96-130) with such weights. x and out hold values of `dtype` (f32 or bf16), rows
- * x_stride and out_stride values apart; bias is f32 [out_features] or NULL. Sums are held in f32 and rounded once; with
- * many rows of bf16 a weight is held in 11 bits (exact with a zero point of 8, else off by up to 2^-12 of itself), less what is
- * below 2^-29 of its row's largest scale. `out` overlaps no input. `workspace` (256-byte aligned, orion_cuda_w4_workspace bytes; NULL where that is 0) belongs to the call
- * until its work has ended; its contents need no preparation and are of no use afterwards. */
+ * x_stride and out_stride values apart; bias is f32 [out_features] or NULL. Sums are held in f32 (those of
+ * bf16 rows as multiples of 2^-136) and rounded once. f32 values of x count as multiples of 2^-133: all of their bits from 2^-109 on.
+ * With many rows of bf16 a weight is held in 11 bits (exact with a zero point of 8, else off by up to 2^-12 of itself), less what is
+ * below 2^-29 of its row's largest scale. `out` overlaps no input. `workspace` (256-byte aligned, orion_cuda_w4_workspace bytes;
+ * NULL where that is 0) belongs to the call until its work has ended; its contents need no preparation and are of no use
+ * afterwards. */
 int orion_cuda_w4_linear(int device, int dtype, const void *x, uint64_t rows, uint64_t x_stride, const OrionW4Weight *weight,
                          const float *bias, void *out, uint64_t out_stride, void *workspace, uint64_t workspace_bytes,
                          void *stream);

@@ -7,7 +7,8 @@
 // as bf16, is code * 2^-133 or code * 2^-129 (subnormal numbers are multiples of 2^-133, and so are those of the first binade above them), and
 // fma(pair, 2^120 or 2^116, -zero * 2^-13) = (code - zero) * 2^-13, exactly.
 //
-// f32 activations go through the same instructions as three bf16 terms of eight bits each (hi + mid + lo = x exactly), so f32 results have f32 accuracy.
+// f32 activations go through the same instructions as three bf16 terms of eight bits each: hi + mid + lo = x exactly down to the smallest bf16 number, 2^-133, so
+// that values of 2^-109 and more have all of their 24 bits, and f32 results f32 accuracy.
 // The warps that share a slab of tokens make its terms together (211 rows of k 2048 to 5504 outputs: 98 us with each warp making its own, 90 together). More than
 // 16 rows are bound by these instructions, so two CTAs share an SM there too (512 rows of k 4096 to 14336: 734 us with one of up to 210 registers a thread,
 // 562 with two of 128; 211 rows as above 90 and 79).
@@ -404,10 +405,19 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
           for (uint32_t h = 0; h < 2; ++h) {
             const uint32_t row = matrix_of(rt) * kPerSlab + q * 32 / GROUP;
             const float scale = __uint_as_float(lds16(s_at + row * Cfg::kScaleRow + (col_of(rt) + h * 8 + g) * 2) << 16);
+            // Sums of f32 are held as they are: in kUnit they would lose bits below 2^-113, where those of bf16 have bits to spare. So kUnit goes to the scale, or
+            // to the group's sums where the scale times kUnit would not be finite. (One test for all of a lane's scales is no faster: 211 rows of k 2048 to 5504
+            // outputs 78.9 us without, 81.4 so, 82.5 with one.)
+            const bool large = kF32 && fabsf(scale) >= 0x1p114f;
+            const float per_unit = kF32 && !large ? scale * kUnit : scale;
+            if (large) {
+#pragma unroll
+              for (uint32_t nt = 0; nt < NT; ++nt) part[rt][nt][2 * h] *= kUnit, part[rt][nt][2 * h + 1] *= kUnit;
+            }
 #pragma unroll
             for (uint32_t nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (uint32_t i = 2 * h; i < 2 * h + 2; ++i) sum[rt][nt][i] = fmaf(part[rt][nt][i], scale, sum[rt][nt][i]);
+              for (uint32_t i = 2 * h; i < 2 * h + 2; ++i) sum[rt][nt][i] = fmaf(part[rt][nt][i], per_unit, sum[rt][nt][i]);
           }
       }
     }
@@ -425,7 +435,7 @@ w4_few_kernel(const W4Call c, const uint32_t tiles_m) {
 #pragma unroll
       for (uint32_t i = 0; i < 4; ++i) {
         const uint32_t token = nt * 8 + t * 2 + (i & 1);
-        if (token < tokens) sums[(kg * Cfg::kTokens + token) * Cfg::kTileRows + (wr * RT + rt) * 16 + (i >> 1) * 8 + g] = sum[rt][nt][i] * kUnit;
+        if (token < tokens) sums[(kg * Cfg::kTokens + token) * Cfg::kTileRows + (wr * RT + rt) * 16 + (i >> 1) * 8 + g] = kF32 ? sum[rt][nt][i] : sum[rt][nt][i] * kUnit;
       }
   if (ranks > 1) cluster_barrier();
   else __syncthreads();

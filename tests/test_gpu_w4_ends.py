@@ -84,3 +84,18 @@ def test_scales_and_tokens_of_opposite_ends(pkg, backend, rows, scale, token, re
     x = values(rng, (rows, k), 24 if dtype == "f32" and token + rest >= -109 else 8) * 2.0 ** (token + rest)
     x[:, 77] = 2.0 ** token
     compare(pkg, backend, x, codes, scales_near(rng, k // GROUP, n, scale), dtype, token + rest)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("power", [-126, -122, -116])
+@pytest.mark.parametrize("rows", [1, 8, 12, 40])
+def test_small_f32_results_keep_their_bits(pkg, backend, rows, power, group):
+    """Results of about 2^power: f32 has their 24 bits down to 2^-126."""
+    rng = np.random.default_rng([33, rows, 200 + power, group])
+    n, k = 140, 1024
+    codes = rng.integers(7, 10, (n, k))
+    scales = scales_near(rng, k // group, n, power + 60)
+    x = values(rng, (rows, k), 24) * 2.0 ** -65  # sums of 1024 random signs: five powers of two
+    w = plain.dequantize(codes, scales, None, group)
+    weight = pkg.W4Weight(torch.tensor(plain.pack(codes)).cuda(), device(scales, "bf16"), None, group)
+    bounds.check(host(pkg.linear_w4(backend, device(x, "f32"), weight)), x @ w.T, bounds.error(x, w, group, "f32", False), "f32")
