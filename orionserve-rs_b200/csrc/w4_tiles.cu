@@ -57,6 +57,7 @@ struct Form {
 using Single64 = Form<1, 64, 256, 3>;
 using Single128 = Form<1, 128, 128, 4>;
 using Paired = Form<2, 128, 128, 3>;
+constexpr uint32_t kWordBytes = 4;       // by which a pair's second CTA tells of its weights
 constexpr uint32_t kSms = 2 * kPairs;
 constexpr int kTop = 14;                 // exponent that the largest scale of a row, and the largest value of a token, are brought to, or one less
 
@@ -274,8 +275,9 @@ __device__ __forceinline__ bool wait_for(uint64_t *bar, uint32_t parity) {
   }
   return false;
 }
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t bar_cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+// Four bytes to the other CTA's shared memory, counted on its barrier.
+__device__ __forceinline__ void st_async(uint32_t cluster_addr, uint32_t v, uint32_t bar_cluster_addr) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.u32 [%0], %1, [%2];" ::"r"(cluster_addr), "r"(v), "r"(bar_cluster_addr) : "memory");
 }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   float v;
@@ -349,7 +351,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
   uint8_t *w_ring = smem, *x_ring = smem + F::kXRing;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + F::kBarriers);
   uint64_t *empty = full + kStages, *acc_full = empty + kStages, *acc_empty = acc_full + 2, *code_full = acc_empty + 2, *code_empty = code_full + F::kCodeStages;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + F::kCodeStages);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(code_empty + F::kCodeStages), *word = tmem_slot + 1;  // word: of a pair's leader, one a stage
 
   const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = blockIdx.x % F::kCtas, unit = blockIdx.x / F::kCtas, units = gridDim.x / F::kCtas;
@@ -358,8 +360,8 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
 
   if (threadIdx.x == 0) {
     for (uint32_t s = 0; s < kStages; ++s) {
-      // leader: the announcement of the tokens' bytes, its own weights, word of the peer's; peer: its weights
-      mbar_init(&full[s], !leader ? kDequantWarps : F::kCtas + kDequantWarps);
+      // leader: its own weights, the announcement of bytes (both CTAs' tokens, word of the peer's weights); peer: its weights
+      mbar_init(&full[s], !leader ? kDequantWarps : 1 + kDequantWarps);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -422,7 +424,7 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         const uint32_t s = it % kStages;
         if (it >= kStages && !wait(&empty[s], ((it / kStages) & 1) ^ 1)) { ok = false; break; }
         if (elected) {
-          if (leader) mbar_arrive_expect_tx(&full[s], F::kCtas * F::kSlabs * box * Pair::kSlabK * 2);
+          if (leader) mbar_arrive_expect_tx(&full[s], F::kCtas * F::kSlabs * box * Pair::kSlabK * 2 + (kPair ? kWordBytes : 0));
 #pragma unroll
           for (uint32_t h = 0; h < F::kSlabs; ++h) {
             uint8_t *to = x_ring + s * F::kXBytes + h * F::kXSlab;
@@ -468,15 +470,15 @@ w4_tile_kernel(const W4Call c, const __grid_constant__ CUtensorMap map_x, const 
         if (ok && elected) commit(&acc_full[buf]);
       }
     } else {
-      // Hands word of this CTA's weights on to the leader. They are stores to this SM's own shared memory, which this SM's tensor cores read; the barrier that
-      // is waited for here has ordered them, and the arrival needs no more than that. (Released to the cluster it waits some hundred cycles at every stage:
-      // gated 4096 x 4096 to 14336 in 785 us against 704.)
+      // Hands word of this CTA's weights on to the leader, whose MMA reads them: an asynchronous store, whose completion on the leader's barrier is a release at
+      // cluster scope that follows its issue here, behind the wait for the weights. (An arrival released to the cluster waits some hundred cycles at every stage:
+      // 2048 x 4096 to 4096 in 109 us against 67.7, gated 4096 x 4096 to 14336 in 763 against 656. One at CTA scope, 67.0 and 651, orders nothing between the two.)
       uint32_t it = 0;
       for (uint32_t t = unit; ok && t < total; t += units) {
         const Job j = job(t);
         for (uint32_t kb = j.kb; kb < j.end; ++kb, ++it) {
           if (!wait(&full[it % kStages], (it / kStages) & 1)) { ok = false; break; }
-          if (lane == 0) mbar_arrive_remote(mapa_u32(smem_u32(&full[it % kStages]), 0));
+          if (lane == 0) st_async(mapa_u32(smem_u32(&word[it % kStages]), 0), it, mapa_u32(smem_u32(&full[it % kStages]), 0));
           __syncwarp();
         }
       }
