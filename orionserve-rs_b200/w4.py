@@ -51,7 +51,8 @@ class W4Weight:
     """A matrix of 4-bit codes ``[out_features, in_features]``, kept by a program for as long as it uses the matrix.
 
     ``packed`` is int32 ``[out, in / 8]``, ``scales`` bf16 ``[in / group, out]``, ``zeros`` uint8 like ``scales`` with values of at most 15, or None:
-    8 everywhere. The tensors are kept and must not be resized; their values may be written."""
+    8 everywhere. The tensors are kept for good, as is everything else of the handle, since the kernels are given their addresses: they must not be resized
+    or given other storage; their values may be written."""
 
     __slots__ = ("packed", "scales", "zeros", "group", "out_features", "in_features", "device_index", "_desc", "_address", "_spaces")
 
@@ -76,11 +77,18 @@ class W4Weight:
         self._hold(packed, scales, zeros, group, n, k, packed.device.index)
 
     def _hold(self, packed, scales, zeros, group, n, k, device_index):
-        self.packed, self.scales, self.zeros, self.group = packed, scales, zeros, group
-        self.out_features, self.in_features, self.device_index = n, k, device_index
-        self._desc = _ffi.OrionW4Weight(packed.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), n, k, group)
-        self._address = C.addressof(self._desc)
-        self._spaces = {}
+        desc = _ffi.OrionW4Weight(packed.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), n, k, group)
+        for name, value in zip(W4Weight.__slots__, (packed, scales, zeros, group, n, k, device_index, desc, C.addressof(desc), {})):
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name}: what a W4Weight holds stays; make another one")
+
+    def __delattr__(self, name):
+        raise AttributeError(f"{name}: what a W4Weight holds stays; make another one")
+
+    def __copy__(self):
+        return self
 
     @classmethod
     def from_codes(cls, codes, scales, zeros=None, group: int = 128) -> "W4Weight":

@@ -1,0 +1,39 @@
+"""What the torch veneer of the 4-bit operators refuses, on tensors of the host: the checks come ahead of any device."""
+import copy
+import types
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+HOST = types.SimpleNamespace(_ordinal=-1)  # the "device" of a tensor that is on the host
+
+
+@pytest.fixture
+def w4(pkg):
+    import sys
+
+    module = sys.modules[pkg.linear_w4.__module__]
+    module._load()
+    return module
+
+
+def weight(w4, n=8, k=64, group=32, zeros=False):
+    w = w4.W4Weight.__new__(w4.W4Weight)
+    w._hold(torch.zeros((n, k // 8), dtype=torch.int32), torch.zeros((k // group, n), dtype=torch.bfloat16),
+            torch.zeros((k // group, n), dtype=torch.uint8) if zeros else None, group, n, k, -1)
+    return w
+
+
+def test_what_a_weight_holds_stays(w4):
+    """The kernels are given the addresses that its tensors had when it was made."""
+    w = weight(w4, zeros=True)
+    for name in ("packed", "scales", "zeros", "group", "out_features", "in_features", "device_index", "other"):
+        before = getattr(w, name, None)
+        with pytest.raises(AttributeError):
+            setattr(w, name, before)
+        with pytest.raises(AttributeError):
+            delattr(w, name)
+        assert getattr(w, name, None) is before
+    assert copy.copy(w) is w
+    assert w._desc.packed == w.packed.data_ptr() and w._desc.zeros == w.zeros.data_ptr()
