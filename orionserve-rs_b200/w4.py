@@ -115,8 +115,8 @@ def _rows(backend: CudaBackend, x, weight: W4Weight):
         raise InvalidRequest(f"x: shape [rows, {weight.in_features}] is needed, got {tuple(x.shape)}")
     if x.get_device() != backend._ordinal or weight.device_index != backend._ordinal:
         raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
-    if x.requires_grad and _torch.is_grad_enabled():
-        raise InvalidRequest("x: 4-bit operators have no gradient")
+    if (x.requires_grad or weight.scales.requires_grad) and _torch.is_grad_enabled():
+        raise InvalidRequest("x and the weight's scales: 4-bit operators have no gradient")
     stride, unit = x.stride()
     if unit != 1:
         raise InvalidRequest("x: the values of a row must be neighbours")
@@ -203,6 +203,8 @@ def gated_w4(backend: CudaBackend, x, gate: W4Weight, up: W4Weight, activation: 
     dtype, rows, stride = _rows(backend, x, gate)
     if up.device_index != backend._ordinal:
         raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
+    if up.scales.requires_grad and _torch.is_grad_enabled():
+        raise InvalidRequest("the weight's scales: 4-bit operators have no gradient")
     out, out_stride = _output(x, out, rows, gate.out_features)
     space, at, size = _workspace(x, dtype, rows, gate, 1)
     check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride, at, size,

@@ -37,3 +37,15 @@ def test_what_a_weight_holds_stays(w4):
         assert getattr(w, name, None) is before
     assert copy.copy(w) is w
     assert w._desc.packed == w.packed.data_ptr() and w._desc.zeros == w.zeros.data_ptr()
+
+
+def test_scales_that_need_a_gradient_are_refused_at_the_call(pkg, w4):
+    """A weight may be made under no_grad, or its scales may need a gradient later."""
+    x = torch.zeros((3, 64), dtype=torch.bfloat16)
+    w, learned = weight(w4), weight(w4)
+    learned.scales.requires_grad_()
+    for call in (lambda: pkg.linear_w4(HOST, x, learned), lambda: pkg.gated_w4(HOST, x, learned, w), lambda: pkg.gated_w4(HOST, x, w, learned)):
+        with pytest.raises(pkg.InvalidRequest, match="gradient"):
+            call()
+    with torch.no_grad():
+        assert w4._rows(HOST, x, learned) == (2, 3, 64)
