@@ -5,7 +5,8 @@ Codes are packed eight to an int32: of eight consecutive ``k``, number ``2i`` is
 19 + 4i``. The functions stand beside ``ops.linear`` and ``ops.swiglu`` for tensors that are on the device already: they run on torch's current
 stream of the tensors' device, allocate what they return and, for many rows, a workspace, and can be captured into a CUDA graph once a call of
 the same kind and size has been made outside of one. Activations are f32 or bf16. Nothing here has a gradient; tensors that require
-one are refused, unless gradients are off (``torch.no_grad()``).
+one are refused, unless gradients are off (``torch.no_grad()``), as are tensors with a forward-mode tangent and calls under ``torch.jit.trace``, which
+would not see the kernels.
 """
 from __future__ import annotations
 
@@ -17,21 +18,32 @@ from .errors import InvalidRequest, check
 
 GROUPS = (32, 64, 128)
 _ACTIVATIONS = {"silu": _ffi.GATE_SILU, "gelu_tanh": _ffi.GATE_GELU_TANH}
-_torch = None
+_torch = _forward_ad = None
 _dtypes = {}  # torch dtype -> OrionDType
-_empty = _linear = _gated = _quantize = None  # torch.empty_strided, the fastest of its kind, and entry points of the library
+_empty = _linear = _gated = _quantize = _is_tracing = None  # torch.empty_strided, the fastest of its kind, entry points of the library, torch.jit.is_tracing
 
 
 def _load():
     """torch and the library, at the first call: the rest of the package does without torch."""
-    global _torch, _empty, _linear, _gated, _quantize, _stream
+    global _torch, _forward_ad, _empty, _linear, _gated, _quantize, _stream, _is_tracing
     import torch
+    import torch.autograd.forward_ad
 
     lib = _ffi.lib()
     _linear, _gated, _quantize = lib.orion_cuda_w4_linear, lib.orion_cuda_w4_gated, lib.orion_cuda_w4_quantize
     _dtypes.update({torch.float32: 0, torch.bfloat16: 2})
-    _torch, _empty = torch, torch.empty_strided
+    _torch, _forward_ad, _empty = torch, torch.autograd.forward_ad, torch.empty_strided
     _stream = _raw_stream()
+    _is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
+def _unrecorded(*tensors):
+    """Refuses what torch records by other means than ``requires_grad``: forward-mode derivatives, which ``torch.no_grad()`` leaves on, and traces."""
+    if _is_tracing():
+        raise InvalidRequest("4-bit operators cannot be traced")
+    for t in tensors:
+        if isinstance(t, _torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            raise InvalidRequest("4-bit operators have no forward-mode derivative")
 
 
 def _on_device(name, t, dtype, shape=None):
@@ -180,6 +192,8 @@ def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
     if _torch is None:
         _load()
     dtype, rows, stride = _rows(backend, x, weight)
+    if _is_tracing() or _forward_ad._current_level >= 0:
+        _unrecorded(x, weight.scales, bias, out)
     n = weight.out_features
     if bias is not None:
         _on_device("bias", bias, _torch.float32, (n,))
@@ -205,6 +219,8 @@ def gated_w4(backend: CudaBackend, x, gate: W4Weight, up: W4Weight, activation: 
         raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
     if up.scales.requires_grad and _torch.is_grad_enabled():
         raise InvalidRequest("the weight's scales: 4-bit operators have no gradient")
+    if _is_tracing() or _forward_ad._current_level >= 0:
+        _unrecorded(x, gate.scales, up.scales, out)
     out, out_stride = _output(x, out, rows, gate.out_features)
     space, at, size = _workspace(x, dtype, rows, gate, 1)
     check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride, at, size,
@@ -229,6 +245,8 @@ def quantize_w4(backend: CudaBackend, weight, group: int = 128, zeros: bool = Fa
         raise InvalidRequest(f"a matrix of {n} x {k} has no whole groups of {group} (32, 64 or 128)")
     if weight.requires_grad and _torch.is_grad_enabled():
         raise InvalidRequest("weight: 4-bit operators have no gradient")
+    if _is_tracing() or _forward_ad._current_level >= 0:
+        _unrecorded(weight)
     if weight.stride(1) != 1:
         raise InvalidRequest("weight: the values of a row must be neighbours")
     w = W4Weight.__new__(W4Weight)

@@ -49,3 +49,32 @@ def test_scales_that_need_a_gradient_are_refused_at_the_call(pkg, w4):
             call()
     with torch.no_grad():
         assert w4._rows(HOST, x, learned) == (2, 3, 64)
+
+
+def test_forward_mode_tangents_are_refused(pkg, w4):
+    """Under no_grad too, which leaves them on."""
+    import torch.autograd.forward_ad as fw
+
+    x, w, dual = torch.zeros((3, 64)), weight(w4), weight(w4)
+    with fw.dual_level():
+        for t in (x, w.scales):  # other tensors of a dual level are as good as ever
+            w4._unrecorded(t, None)
+        held = {name: getattr(dual, name) for name in ("packed", "scales", "zeros")}
+        held["scales"] = fw.make_dual(held["scales"], torch.ones_like(held["scales"]))
+        dual._hold(**held, group=32, n=8, k=64, device_index=-1)
+        tangent, bias = fw.make_dual(x, torch.ones_like(x)), fw.make_dual(torch.zeros(8), torch.ones(8))
+        calls = (lambda: pkg.linear_w4(HOST, tangent, w), lambda: pkg.linear_w4(HOST, x, dual), lambda: pkg.linear_w4(HOST, x, w, bias=bias),
+                 lambda: pkg.gated_w4(HOST, tangent, w, w), lambda: pkg.gated_w4(HOST, x, w, dual), lambda: pkg.gated_w4(HOST, x, dual, w),
+                 lambda: pkg.quantize_w4(HOST, tangent, group=32))
+        for call in calls:
+            with pytest.raises(pkg.InvalidRequest, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(pkg.InvalidRequest, match="forward-mode"):
+                call()
+
+
+def test_traces_are_refused(pkg, w4):
+    x, w = torch.zeros((3, 64)), weight(w4)
+    for call in (lambda x: pkg.linear_w4(HOST, x, w), lambda x: pkg.gated_w4(HOST, x, w, w), lambda x: pkg.quantize_w4(HOST, x, group=32).scales):
+        with pytest.raises(pkg.InvalidRequest, match="traced"):
+            torch.jit.trace(call, (x,))
