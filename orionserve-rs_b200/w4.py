@@ -32,9 +32,10 @@ def _load():
     lib = _ffi.lib()
     _linear, _gated, _quantize = lib.orion_cuda_w4_linear, lib.orion_cuda_w4_gated, lib.orion_cuda_w4_quantize
     _dtypes.update({torch.float32: 0, torch.bfloat16: 2})
-    _torch, _forward_ad, _empty = torch, torch.autograd.forward_ad, torch.empty_strided
-    _stream = _raw_stream()
+    _forward_ad, _empty = torch.autograd.forward_ad, torch.empty_strided
+    _stream = _raw_stream(torch)
     _is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+    _torch = torch  # last: calls on other threads take it for a sign that the others are there
 
 
 def _unrecorded(*tensors):
@@ -164,9 +165,9 @@ def _stream(device: int) -> int:
     return _torch.cuda.current_stream(device).cuda_stream
 
 
-def _raw_stream():
+def _raw_stream(torch):
     """torch's own lookup of the current stream's handle, without a Stream object around it (1.2 us of a call), where this torch has it."""
-    return getattr(_torch._C, "_cuda_getCurrentRawStream", _stream)
+    return getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
 
 
 def _workspace(x, dtype, rows, weight, gated):

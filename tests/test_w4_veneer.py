@@ -78,3 +78,19 @@ def test_traces_are_refused(pkg, w4):
     for call in (lambda x: pkg.linear_w4(HOST, x, w), lambda x: pkg.gated_w4(HOST, x, w, w), lambda x: pkg.quantize_w4(HOST, x, group=32).scales):
         with pytest.raises(pkg.InvalidRequest, match="traced"):
             torch.jit.trace(call, (x,))
+
+
+def test_two_first_calls_at_once(pkg, w4, monkeypatch):
+    """What one thread's first call loads is there in full before another thread's takes it for loaded."""
+    names = ("_forward_ad", "_empty", "_linear", "_gated", "_quantize", "_is_tracing", "_torch")
+    for name in names:
+        monkeypatch.setattr(w4, name, None)
+    seen, real = [], w4._raw_stream
+
+    def watched(*args):
+        seen.append(w4._torch)
+        return real(*args)
+
+    monkeypatch.setattr(w4, "_raw_stream", watched)
+    w4._load()
+    assert seen == [None] and all(getattr(w4, name) is not None for name in names)
