@@ -161,6 +161,11 @@ def _output(x, out, rows, n):
     return out, out.stride(0)
 
 
+def _written(out):
+    """Tells torch that a tensor of the caller's was written: a backward pass that has kept it has to fail, as after torch's own writes."""
+    _torch.autograd.graph.increment_version(out)
+
+
 def _stream(device: int) -> int:
     return _torch.cuda.current_stream(device).cuda_stream
 
@@ -200,10 +205,13 @@ def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
         _on_device("bias", bias, _torch.float32, (n,))
         if bias.get_device() != backend._ordinal:
             raise InvalidRequest(f"bias must be on the backend's device {backend._ordinal}")
+    given = out
     out, out_stride = _output(x, out, rows, n)
     space, at, size = _workspace(x, dtype, rows, weight, 0)
     check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, weight._address, None if bias is None else bias.data_ptr(), out.data_ptr(),
                   out_stride, at, size, _stream(backend._ordinal)))
+    if given is not None:
+        _written(given)
     return out
 
 
@@ -222,10 +230,13 @@ def gated_w4(backend: CudaBackend, x, gate: W4Weight, up: W4Weight, activation: 
         raise InvalidRequest("the weight's scales: 4-bit operators have no gradient")
     if _is_tracing() or _forward_ad._current_level >= 0:
         _unrecorded(x, gate.scales, up.scales, out)
+    given = out
     out, out_stride = _output(x, out, rows, gate.out_features)
     space, at, size = _workspace(x, dtype, rows, gate, 1)
     check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride, at, size,
                  _stream(backend._ordinal)))
+    if given is not None:
+        _written(given)
     return out
 
 

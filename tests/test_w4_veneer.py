@@ -94,3 +94,27 @@ def test_two_first_calls_at_once(pkg, w4, monkeypatch):
     monkeypatch.setattr(w4, "_raw_stream", watched)
     w4._load()
     assert seen == [None] and all(getattr(w4, name) is not None for name in names)
+
+
+@pytest.fixture
+def no_device(w4, monkeypatch):
+    """Calls that end where the library would be called."""
+    for name in ("_linear", "_gated"):
+        monkeypatch.setattr(w4, name, lambda *args: 0)
+    monkeypatch.setattr(w4, "_stream", lambda device: 0)
+
+
+def test_outputs_that_a_backward_pass_has_kept(pkg, w4, no_device):
+    """Written by a call, they no longer serve it."""
+    x, w = torch.zeros((3, 64)), weight(w4)
+    for call in (lambda out: pkg.linear_w4(HOST, x, w, out=out), lambda out: pkg.gated_w4(HOST, x, w, w, out=out)):
+        whole = torch.ones((4, 12))
+        learned = torch.ones((4, 12), requires_grad=True)
+        loss = (learned * whole).sum()
+        before = whole._version
+        assert call(whole[1:, 2:10]).data_ptr() == whole[1:, 2:].data_ptr()
+        assert whole._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+        with torch.inference_mode():
+            call(torch.zeros((3, 8)))
