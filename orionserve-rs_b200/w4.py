@@ -149,7 +149,15 @@ def _overlap(a, b):
     return apart < a.shape[1] * size or apart + b.shape[1] * size > stride
 
 
-def _output(x, out, rows, n):
+def _meets(out, t):
+    """Whether a row of a matrix, its values neighbours, shares a byte with a tensor without gaps."""
+    size = out.element_size()
+    row, apart, at = out.shape[1] * size, out.stride(0) * size, t.data_ptr() - out.data_ptr()  # from here: rows at i * apart, the tensor at `at`
+    first = max(0, (at - row) // apart + 1) if apart > 0 else 0  # the first row that ends behind the tensor's beginning
+    return first < out.shape[0] and first * apart < at + t.numel() * t.element_size() and first * apart + row > at
+
+
+def _output(x, out, rows, n, *others):
     if out is None:
         return _empty((rows, n), (n, 1), dtype=x.dtype, device=x.device), n
     if not isinstance(out, _torch.Tensor) or out.dtype != x.dtype or out.device != x.device or tuple(out.shape) != (rows, n) or (n > 1 and out.stride(1) != 1):
@@ -158,6 +166,8 @@ def _output(x, out, rows, n):
         raise InvalidRequest("out: 4-bit operators have no gradient")
     if rows and _overlap(x, out):
         raise InvalidRequest("out: overlaps x")
+    if rows and any(t is not None and _meets(out, t) for t in others):
+        raise InvalidRequest("out: overlaps the bias or a weight")
     return out, out.stride(0)
 
 
@@ -194,7 +204,8 @@ def _workspace(x, dtype, rows, weight, gated):
 
 def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
     """``x W^T + bias`` (tensor.rs:96-130) over ``x`` ``[rows, in]``, f32 or bf16; ``bias`` f32 ``[out]``. Sums are f32, rounded once to the type of
-    ``x``. Rows may be apart (any stride that keeps them on 16-byte boundaries); ``out``, if given, is written and returned."""
+    ``x``. Rows may be apart (any stride that keeps them on 16-byte boundaries); ``out``, if given, overlaps none of
+    the others, is written and returned."""
     if _torch is None:
         _load()
     dtype, rows, stride = _rows(backend, x, weight)
@@ -206,7 +217,7 @@ def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
         if bias.get_device() != backend._ordinal:
             raise InvalidRequest(f"bias must be on the backend's device {backend._ordinal}")
     given = out
-    out, out_stride = _output(x, out, rows, n)
+    out, out_stride = _output(x, out, rows, n, bias, weight.packed, weight.scales, weight.zeros)
     space, at, size = _workspace(x, dtype, rows, weight, 0)
     check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, weight._address, None if bias is None else bias.data_ptr(), out.data_ptr(),
                   out_stride, at, size, _stream(backend._ordinal)))
@@ -231,7 +242,7 @@ def gated_w4(backend: CudaBackend, x, gate: W4Weight, up: W4Weight, activation: 
     if _is_tracing() or _forward_ad._current_level >= 0:
         _unrecorded(x, gate.scales, up.scales, out)
     given = out
-    out, out_stride = _output(x, out, rows, gate.out_features)
+    out, out_stride = _output(x, out, rows, gate.out_features, gate.packed, gate.scales, gate.zeros, up.packed, up.scales, up.zeros)
     space, at, size = _workspace(x, dtype, rows, gate, 1)
     check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride, at, size,
                  _stream(backend._ordinal)))

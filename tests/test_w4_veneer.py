@@ -118,3 +118,43 @@ def test_outputs_that_a_backward_pass_has_kept(pkg, w4, no_device):
             loss.backward()
         with torch.inference_mode():
             call(torch.zeros((3, 8)))
+
+
+def test_outputs_that_overlap_a_bias_or_a_weight_are_refused(pkg, w4, no_device, monkeypatch):
+    """CTAs that have ended write while others still read."""
+    monkeypatch.setattr(w4, "_on_device", lambda *args: None)  # which asks for a CUDA tensor
+    room = torch.zeros(4096, dtype=torch.uint8)
+    room = room[-room.data_ptr() % 16:]
+
+    def piece(start, shape, dtype):
+        size = torch.empty((), dtype=dtype).element_size()
+        n = 1
+        for d in shape:
+            n *= d
+        return room[start:start + n * size].view(dtype).view(shape)
+
+    def made(packed, scales, zeros):
+        w = w4.W4Weight.__new__(w4.W4Weight)
+        w._hold(packed, scales, zeros, 32, 8, 64, -1)
+        return w
+
+    x, bias = torch.zeros((3, 64)), torch.zeros(8)
+    inside = made(piece(512, (8, 8), torch.int32), piece(1024, (2, 8), torch.bfloat16), piece(1280, (2, 8), torch.uint8))
+    apart = weight(w4)
+    for start, length in ((512, 256), (1024, 32), (1280, 16)):
+        for at in (start - 64, start - 96 + 4, start, start + length - 4):  # three rows of 32 bytes
+            for call in (lambda out: pkg.linear_w4(HOST, x, inside, out=out), lambda out: pkg.gated_w4(HOST, x, inside, apart, out=out),
+                         lambda out: pkg.gated_w4(HOST, x, apart, inside, out=out)):
+                with pytest.raises(pkg.InvalidRequest, match="overlaps"):
+                    call(piece(at, (3, 8), torch.float32))
+        for at in (start - 96, start + length):
+            pkg.linear_w4(HOST, x, inside, out=piece(at, (3, 8), torch.float32))
+    wide = piece(2048, (4, 24), torch.float32)
+    for out in (wide[:3, :8], wide[1:4, 16:], wide[::2, 8:16][:2]):
+        lone = x[:out.shape[0]]
+        pkg.linear_w4(HOST, lone, apart, bias=wide[3, :8], out=out)  # between the rows, or behind them
+        pkg.linear_w4(HOST, lone, apart, bias=wide[1, :8] if out.shape[0] == 2 else wide[0, 8:16], out=out)
+        for row in range(out.shape[0]):
+            with pytest.raises(pkg.InvalidRequest, match="overlaps"):
+                pkg.linear_w4(HOST, lone, apart, bias=out[row], out=out)
+    pkg.linear_w4(HOST, x[:1], apart, bias=bias, out=torch.zeros((1, 8)))
