@@ -108,12 +108,12 @@ class W4Weight:
         """Packs codes ``[out, in]`` of 0..15, as other formats hold them, on their device; ``scales`` and ``zeros`` as in the constructor."""
         if _torch is None:
             _load()
-        if not isinstance(codes, _torch.Tensor) or codes.dim() != 2 or codes.shape[1] % 8 or codes.dtype.is_floating_point:
+        if not isinstance(codes, _torch.Tensor) or codes.dim() != 2 or codes.shape[1] % 8 or codes.dtype.is_floating_point or codes.dtype.is_complex:
             raise InvalidRequest("codes: a matrix of whole numbers is needed, with a multiple of 8 columns")
         if codes.numel() and (int(codes.min()) < 0 or int(codes.max()) > 15):
             raise InvalidRequest("codes: values of 0 to 15 are needed")
         at = _torch.tensor([0, 16, 4, 20, 8, 24, 12, 28], dtype=_torch.int32, device=codes.device)
-        words = (codes.to(_torch.int32).view(codes.shape[0], -1, 8) << at).sum(-1, dtype=_torch.int32)
+        words = (codes.to(_torch.int32).reshape(codes.shape[0], codes.shape[1] // 8, 8) << at).sum(-1, dtype=_torch.int32)
         return cls(words, scales, zeros, group)
 
 

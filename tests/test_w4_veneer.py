@@ -158,3 +158,22 @@ def test_outputs_that_overlap_a_bias_or_a_weight_are_refused(pkg, w4, no_device,
             with pytest.raises(pkg.InvalidRequest, match="overlaps"):
                 pkg.linear_w4(HOST, lone, apart, bias=out[row], out=out)
     pkg.linear_w4(HOST, x[:1], apart, bias=bias, out=torch.zeros((1, 8)))
+
+
+def test_codes_of_any_strides_are_packed(pkg, w4, monkeypatch):
+    gen = torch.Generator().manual_seed(5)
+    codes = torch.randint(0, 16, (64, 24), generator=gen)
+    monkeypatch.setattr(w4, "_on_device", lambda *args: None)  # which asks for a CUDA tensor
+    scales, shifts = torch.zeros((2, 24), dtype=torch.bfloat16), torch.tensor([0, 16, 4, 20, 8, 24, 12, 28])
+    for dtype in (torch.uint8, torch.int8, torch.int32, torch.int64):
+        for c in (codes.to(dtype).t(), codes.to(dtype).t().contiguous(), torch.cat([codes.to(dtype).t()] * 2, dim=1)[:, ::1][:, 64:], codes.to(dtype).t().repeat_interleave(2, 1)[:, ::2]):
+            words = pkg.W4Weight.from_codes(c, scales, None, 32).packed
+            assert torch.equal((words[:, :, None] >> shifts) & 15, codes.t().reshape(24, 8, 8).to(torch.int32))
+
+
+def test_codes_that_are_refused(pkg, w4):
+    scales = torch.zeros((2, 24), dtype=torch.bfloat16)
+    for c in (torch.zeros((24, 64)), torch.zeros((24, 64), dtype=torch.complex64), torch.zeros((24, 60), dtype=torch.int32), torch.zeros((0, 64), dtype=torch.int32), torch.zeros((24, 0), dtype=torch.int32),
+              torch.full((24, 64), 16), torch.full((24, 64), -1), torch.zeros(64, dtype=torch.int32)):
+        with pytest.raises(pkg.InvalidRequest):
+            pkg.W4Weight.from_codes(c, scales, None, 32)
