@@ -12,6 +12,7 @@
 #include <cstdio>
 
 #include "../../include/orion_cuda.h"
+#include "scoped_device.h"
 
 namespace orion {
 
@@ -42,21 +43,6 @@ inline const void *device_symbol(const S &symbol) {
   void *p = nullptr;
   return cudaGetSymbolAddress(&p, symbol) == cudaSuccess ? p : nullptr;
 }
-
-// Makes `device` current for the scope and puts the caller's device back afterwards.
-struct ScopedDevice {
-  int prev = -1;
-  bool changed = false;
-  cudaError_t status;
-  explicit ScopedDevice(int device) {
-    status = cudaGetDevice(&prev);
-    changed = status == cudaSuccess && prev != device;
-    if (changed) status = cudaSetDevice(device);
-  }
-  ~ScopedDevice() {
-    if (changed) cudaSetDevice(prev);
-  }
-};
 
 // Number of kernels launched through launch accounting since the last reset.
 extern thread_local uint64_t g_launch_count;
