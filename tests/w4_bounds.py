@@ -8,8 +8,9 @@ the nearest: sqrt(m) 2^-24 q, with a few sums more of parts of k. Weights that a
 step / sqrt(3) q.
 
 An output v that is off by d before it is rounded to its type, with spacing u there, ends in another place than v with probability |d| / u and is then off by u: on
-average by |d|, whatever the spacing. So the sum of |got - round(want)| over N outputs is that of |d|, with a standard deviation of at most sqrt(sum |d| u);
-four of those are allowed."""
+average by |d|, whatever the spacing. So the sum of |got - round(want)| over all outputs is that of |d|, with a variance V of at most sum |d| u. Where |d| is far
+below u few outputs change place, and the sum is not normally distributed: by Bernstein's inequality it exceeds its mean by t with a probability of at most
+exp(-t^2 / (2 V + 2 t U / 3)), U the largest u, and that is e^-16 for t = 16 U / 3 + sqrt((16 U / 3)^2 + 32 V)."""
 import numpy as np
 
 import w4_plain as plain
@@ -70,5 +71,7 @@ def check(got, want, bound, dtype, what=""):
     """The outputs as a whole: sum |got - round(want)| against the sum of their bounds."""
     got = np.asarray(got, np.float64)
     assert got.shape == want.shape and np.isfinite(want).all()
-    off, most = np.abs(got - rounded(want, dtype)).sum(), bound.sum() + 4.0 * np.sqrt((bound * spacing(want, dtype)).sum())
+    u = spacing(want, dtype)
+    rare = 16.0 / 3.0 * u.max()
+    off, most = np.abs(got - rounded(want, dtype)).sum(), bound.sum() + rare + np.sqrt(rare ** 2 + 32.0 * (bound * u).sum())
     assert off <= most, f"{what}: {off / most:.3g} times the bound"
