@@ -67,7 +67,11 @@ class W4Weight:
     8 everywhere. The tensors are kept for good, as is everything else of the handle, since the kernels are given their addresses: they must not be resized
     or given other storage; their values may be written."""
 
-    __slots__ = ("packed", "scales", "zeros", "group", "out_features", "in_features", "device_index", "_desc", "_address", "_spaces")
+    # One tuple, which the calls take apart and nothing else writes: packed, scales, zeros, group, out_features, in_features, device_index, the descriptor of
+    # the library, its address, and the sizes of workspaces by key.
+    __slots__ = ("_held",)
+
+    packed, scales, zeros, group, out_features, in_features, device_index, _desc = (property(lambda self, i=i: self._held[i]) for i in range(8))
 
     def __init__(self, packed, scales, zeros=None, group: int = 128):
         if _torch is None:
@@ -91,14 +95,7 @@ class W4Weight:
 
     def _hold(self, packed, scales, zeros, group, n, k, device_index):
         desc = _ffi.OrionW4Weight(packed.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), n, k, group)
-        for name, value in zip(W4Weight.__slots__, (packed, scales, zeros, group, n, k, device_index, desc, C.addressof(desc), {})):
-            object.__setattr__(self, name, value)
-
-    def __setattr__(self, name, value):
-        raise AttributeError(f"{name}: what a W4Weight holds stays; make another one")
-
-    def __delattr__(self, name):
-        raise AttributeError(f"{name}: what a W4Weight holds stays; make another one")
+        self._held = packed, scales, zeros, group, n, k, device_index, desc, C.addressof(desc), {}
 
     def __copy__(self):
         return self
@@ -117,18 +114,18 @@ class W4Weight:
         return cls(words, scales, zeros, group)
 
 
-def _rows(backend: CudaBackend, x, weight: W4Weight):
-    """Checks a call's activations; returns (dtype, rows, row stride)."""
+def _rows(backend: CudaBackend, x, scales, in_features, device_index):
+    """Checks a call's activations and its weight's place; returns (dtype, rows, row stride)."""
     if x.__class__ is not _torch.Tensor and not isinstance(x, _torch.Tensor):
         raise InvalidRequest("x: a CUDA tensor is needed")
     dtype = _dtypes.get(x.dtype)
     if dtype is None:
         raise InvalidRequest(f"x: float32 or bfloat16 is needed, got {x.dtype}")
-    if x.dim() != 2 or x.shape[1] != weight.in_features:
-        raise InvalidRequest(f"x: shape [rows, {weight.in_features}] is needed, got {tuple(x.shape)}")
-    if x.get_device() != backend._ordinal or weight.device_index != backend._ordinal:
+    if x.dim() != 2 or x.shape[1] != in_features:
+        raise InvalidRequest(f"x: shape [rows, {in_features}] is needed, got {tuple(x.shape)}")
+    if x.get_device() != backend._ordinal or device_index != backend._ordinal:
         raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
-    if (x.requires_grad or weight.scales.requires_grad) and _torch.is_grad_enabled():
+    if (x.requires_grad or scales.requires_grad) and _torch.is_grad_enabled():
         raise InvalidRequest("x and the weight's scales: 4-bit operators have no gradient")
     stride, unit = x.stride()
     if unit != 1:
@@ -149,25 +146,33 @@ def _overlap(a, b):
     return apart < a.shape[1] * size or apart + b.shape[1] * size > stride
 
 
-def _meets(out, t):
-    """Whether a row of a matrix, its values neighbours, shares a byte with a tensor without gaps."""
-    size = out.element_size()
-    row, apart, at = out.shape[1] * size, out.stride(0) * size, t.data_ptr() - out.data_ptr()  # from here: rows at i * apart, the tensor at `at`
-    first = max(0, (at - row) // apart + 1) if apart > 0 else 0  # the first row that ends behind the tensor's beginning
-    return first < out.shape[0] and first * apart < at + t.numel() * t.element_size() and first * apart + row > at
+def _meets(rows, row, apart, at, length):
+    """Whether one of `rows` pieces of `row` bytes, `apart` bytes from one to the next, shares a byte with `length` bytes that begin `at` bytes behind the first's
+    beginning."""
+    first = max(0, (at - row) // apart + 1) if apart > 0 else 0  # the first that ends behind the beginning of the others
+    return first < rows and first * apart < at + length and first * apart + row > at
 
 
-def _output(x, out, rows, n, *others):
+def _output(x, out, rows, n, bias, *weights):
     if out is None:
         return _empty((rows, n), (n, 1), dtype=x.dtype, device=x.device), n
     if not isinstance(out, _torch.Tensor) or out.dtype != x.dtype or out.device != x.device or tuple(out.shape) != (rows, n) or (n > 1 and out.stride(1) != 1):
         raise InvalidRequest(f"out: a {x.dtype} tensor of shape [{rows}, {n}] on {x.device} is needed, its rows' values neighbours")
     if out.requires_grad and _torch.is_grad_enabled():
         raise InvalidRequest("out: 4-bit operators have no gradient")
-    if rows and _overlap(x, out):
-        raise InvalidRequest("out: overlaps x")
-    if rows and any(t is not None and _meets(out, t) for t in others):
-        raise InvalidRequest("out: overlaps the bias or a weight")
+    if rows:
+        if _overlap(x, out):
+            raise InvalidRequest("out: overlaps x")
+        size, apart, begin = out.element_size(), out.stride(0), out.data_ptr()
+        end = begin + ((rows - 1) * apart + n) * size
+        others = [] if bias is None else [(bias.data_ptr(), 4 * n)]
+        for _, _, _, group, w_n, k, _, desc, _, _ in weights:
+            others += (desc.packed, w_n * k // 2), (desc.scales, w_n * (k // group) * 2)
+            if desc.zeros is not None:
+                others.append((desc.zeros, w_n * (k // group)))
+        for at, length in others:
+            if at < end and at + length > begin and _meets(rows, n * size, apart * size, at - begin, length):
+                raise InvalidRequest("out: overlaps the bias or a weight")
     return out, out.stride(0)
 
 
@@ -185,17 +190,17 @@ def _raw_stream(torch):
     return getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
 
 
-def _workspace(x, dtype, rows, weight, gated):
+def _workspace(x, dtype, rows, address, spaces, gated):
     """(tensor or None, address, bytes) of what a call needs beside its arguments, from torch's allocator: its own until later work of the stream. The sizes
     are kept with the weight."""
     key = rows << 3 | dtype << 1 | gated
-    need = weight._spaces.get(key)
+    need = spaces.get(key)
     if need is None:
         size = C.c_uint64()
-        check(_ffi.lib().orion_cuda_w4_workspace(dtype, rows, weight._address, gated, C.byref(size)))
-        if len(weight._spaces) >= 256:
-            weight._spaces.clear()
-        need = weight._spaces[key] = size.value
+        check(_ffi.lib().orion_cuda_w4_workspace(dtype, rows, address, gated, C.byref(size)))
+        if len(spaces) >= 256:
+            spaces.clear()
+        need = spaces[key] = size.value
     if need == 0:
         return None, None, 0
     t = _empty((need,), (1,), dtype=_torch.uint8, device=x.device)
@@ -208,19 +213,20 @@ def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
     the others, is written and returned."""
     if _torch is None:
         _load()
-    dtype, rows, stride = _rows(backend, x, weight)
-    if _is_tracing() or _forward_ad._current_level >= 0:
-        _unrecorded(x, weight.scales, bias, out)
-    n = weight.out_features
+    held = weight._held
+    _, scales, _, _, n, k, device_index, _, address, spaces = held
+    dtype, rows, stride = _rows(backend, x, scales, k, device_index)
+    if rows.__class__ is not int or _forward_ad._current_level >= 0:  # under a trace sizes are tensors
+        _unrecorded(x, scales, bias, out)
     if bias is not None:
         _on_device("bias", bias, _torch.float32, (n,))
         if bias.get_device() != backend._ordinal:
             raise InvalidRequest(f"bias must be on the backend's device {backend._ordinal}")
     given = out
-    out, out_stride = _output(x, out, rows, n, bias, weight.packed, weight.scales, weight.zeros)
-    space, at, size = _workspace(x, dtype, rows, weight, 0)
-    check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, weight._address, None if bias is None else bias.data_ptr(), out.data_ptr(),
-                  out_stride, at, size, _stream(backend._ordinal)))
+    out, out_stride = _output(x, out, rows, n, bias, held)
+    space, at, size = _workspace(x, dtype, rows, address, spaces, 0)
+    check(_linear(backend._ordinal, dtype, x.data_ptr(), rows, stride, address, None if bias is None else bias.data_ptr(), out.data_ptr(), out_stride, at, size,
+                  _stream(backend._ordinal)))
     if given is not None:
         _written(given)
     return out
@@ -234,17 +240,20 @@ def gated_w4(backend: CudaBackend, x, gate: W4Weight, up: W4Weight, activation: 
     kind = _ACTIVATIONS.get(activation)
     if kind is None:
         raise InvalidRequest(f"unknown activation {activation!r}")
-    dtype, rows, stride = _rows(backend, x, gate)
-    if up.device_index != backend._ordinal:
+    held, up_held = gate._held, up._held
+    _, scales, _, _, n, k, device_index, _, address, spaces = held
+    up_scales = up_held[1]
+    dtype, rows, stride = _rows(backend, x, scales, k, device_index)
+    if up_held[6] != backend._ordinal:
         raise InvalidRequest(f"x and the weight must be on the backend's device {backend._ordinal}")
-    if up.scales.requires_grad and _torch.is_grad_enabled():
+    if up_scales.requires_grad and _torch.is_grad_enabled():
         raise InvalidRequest("the weight's scales: 4-bit operators have no gradient")
-    if _is_tracing() or _forward_ad._current_level >= 0:
-        _unrecorded(x, gate.scales, up.scales, out)
+    if rows.__class__ is not int or _forward_ad._current_level >= 0:
+        _unrecorded(x, scales, up_scales, out)
     given = out
-    out, out_stride = _output(x, out, rows, gate.out_features, gate.packed, gate.scales, gate.zeros, up.packed, up.scales, up.zeros)
-    space, at, size = _workspace(x, dtype, rows, gate, 1)
-    check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, gate._address, up._address, kind, out.data_ptr(), out_stride, at, size,
+    out, out_stride = _output(x, out, rows, n, None, held, up_held)
+    space, at, size = _workspace(x, dtype, rows, address, spaces, 1)
+    check(_gated(backend._ordinal, dtype, x.data_ptr(), rows, stride, address, up_held[8], kind, out.data_ptr(), out_stride, at, size,
                  _stream(backend._ordinal)))
     if given is not None:
         _written(given)
@@ -268,7 +277,7 @@ def quantize_w4(backend: CudaBackend, weight, group: int = 128, zeros: bool = Fa
         raise InvalidRequest(f"a matrix of {n} x {k} has no whole groups of {group} (32, 64 or 128)")
     if weight.requires_grad and _torch.is_grad_enabled():
         raise InvalidRequest("weight: 4-bit operators have no gradient")
-    if _is_tracing() or _forward_ad._current_level >= 0:
+    if n.__class__ is not int or _forward_ad._current_level >= 0:
         _unrecorded(weight)
     if weight.stride(1) != 1:
         raise InvalidRequest("weight: the values of a row must be neighbours")
@@ -276,7 +285,7 @@ def quantize_w4(backend: CudaBackend, weight, group: int = 128, zeros: bool = Fa
     groups, device = k // group, weight.device
     w._hold(_empty((n, k // 8), (k // 8, 1), dtype=_torch.int32, device=device), _empty((groups, n), (n, 1), dtype=_torch.bfloat16, device=device),
             _empty((groups, n), (n, 1), dtype=_torch.uint8, device=device) if zeros else None, group, n, k, backend._ordinal)
-    d = w._desc
+    d = w._held[7]
     check(_quantize(backend._ordinal, _dtypes[weight.dtype], weight.data_ptr(), n, k, weight.stride(0), group, d.packed, d.scales, d.zeros,
                     _stream(backend._ordinal)))
     return w

@@ -25,6 +25,14 @@ def weight(w4, n=8, k=64, group=32, zeros=False):
     return w
 
 
+@pytest.fixture
+def no_device(w4, monkeypatch):
+    """Calls that end where the library would be called."""
+    for name in ("_linear", "_gated"):
+        monkeypatch.setattr(w4, name, lambda *args: 0)
+    monkeypatch.setattr(w4, "_stream", lambda device: 0)
+
+
 def test_what_a_weight_holds_stays(w4):
     """The kernels are given the addresses that its tensors had when it was made."""
     w = weight(w4, zeros=True)
@@ -39,7 +47,7 @@ def test_what_a_weight_holds_stays(w4):
     assert w._desc.packed == w.packed.data_ptr() and w._desc.zeros == w.zeros.data_ptr()
 
 
-def test_scales_that_need_a_gradient_are_refused_at_the_call(pkg, w4):
+def test_scales_that_need_a_gradient_are_refused_at_the_call(pkg, w4, no_device):
     """A weight may be made under no_grad, or its scales may need a gradient later."""
     x = torch.zeros((3, 64), dtype=torch.bfloat16)
     w, learned = weight(w4), weight(w4)
@@ -48,7 +56,7 @@ def test_scales_that_need_a_gradient_are_refused_at_the_call(pkg, w4):
         with pytest.raises(pkg.InvalidRequest, match="gradient"):
             call()
     with torch.no_grad():
-        assert w4._rows(HOST, x, learned) == (2, 3, 64)
+        assert pkg.linear_w4(HOST, x, learned).shape == (3, 8)
 
 
 def test_forward_mode_tangents_are_refused(pkg, w4):
@@ -94,14 +102,6 @@ def test_two_first_calls_at_once(pkg, w4, monkeypatch):
     monkeypatch.setattr(w4, "_raw_stream", watched)
     w4._load()
     assert seen == [None] and all(getattr(w4, name) is not None for name in names)
-
-
-@pytest.fixture
-def no_device(w4, monkeypatch):
-    """Calls that end where the library would be called."""
-    for name in ("_linear", "_gated"):
-        monkeypatch.setattr(w4, name, lambda *args: 0)
-    monkeypatch.setattr(w4, "_stream", lambda device: 0)
 
 
 def test_outputs_that_a_backward_pass_has_kept(pkg, w4, no_device):
