@@ -11,7 +11,7 @@
 // that values of 2^-109 and more have all of their 24 bits, and f32 results f32 accuracy.
 // The warps that share a slab of tokens make its terms together (211 rows of k 2048 to 5504 outputs: 98 us with each warp making its own, 90 together). More than
 // 16 rows are bound by these instructions, so two CTAs share an SM there too (512 rows of k 4096 to 14336: 734 us with one of up to 210 registers a thread,
-// 562 with two of 128; 211 rows as above 90 and 79).
+// 562 with two of 128, which spill some registers; 211 rows as above 90 and 79. With small results kept, below, 569 and 81).
 //
 // A CTA of eight warps, two CTAs to an SM: WR warps side by side over weight rows, 8 / WR groups of them over k. Few tokens: WR = 4, and the tokens' slab of a
 // k group serves 128 rows; more tokens: all eight warps share it, so that L2 delivers it less often. Each k group has a ring of slabs of 128 or 256 k, weights,
@@ -33,7 +33,7 @@ namespace orion {
 namespace {
 
 constexpr uint32_t kThreads = 256, kWarps = 8;
-constexpr float kUnit = 8192.f;        // dequantised codes are multiples of 1 / kUnit
+constexpr float kUnit = 8192.f;        // dequantised codes are multiples of 1 / kUnit: a group's sum stays finite for any tokens that are
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

@@ -33,7 +33,9 @@ __device__ __forceinline__ float max_or_nan(float a, float b) {
 }
 
 // (d + e) / divisor rounded to bf16 in one rounding, d >= 0, inv the f32 number next to 1 / divisor: the quotient in f32, corrected once, is moved to the
-// neighbour with an odd last bit where it is not exact (rounding to odd), after which rounding to 8 bits gives what a single rounding would.
+// neighbour with an odd last bit where it is not exact (rounding to odd), after which rounding to 8 bits gives what a single rounding would. The correction
+// by a remainder that a fused multiply-add makes exact is Markstein's (Computation of elementary functions on the IBM RISC System/6000, 1990), rounding to odd ahead
+// of a second rounding Boldo and Melquiond's (Emulation of a FMA and correctly rounded sums, 2008).
 __device__ __forceinline__ float scale_of(float d, float e, float divisor, float inv) {
   const float guess = d * inv, q = fmaf(fmaf(-guess, divisor, d), inv, guess);
   const float rest = fmaf(-q, divisor, d) + e;

@@ -1,8 +1,8 @@
 // Products with 4-bit weights for many rows of bf16 activations (w4.cuh has the layout): persistent CTA pairs on tcgen05, weights dequantised on their way
 // into shared memory.
 //
-// From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05: 4096 rows of k 4096 with a gate to 14336 take 742 us, 1.3
-// PFLOP/s (0.93 of a library product's rate at the power limit); 64 rows of k 3584 with a gate to 18944 35 us, of which the weights' way from HBM is 12 and the first
+// From some 20 rows on the tensor cores of mma.sync are the bound, from some 100 those of tcgen05: 4096 rows of k 4096 with a gate to 14336 take 751 us, 1.3
+// PFLOP/s (0.92 of a library product's rate at the power limit); 64 rows of k 3584 with a gate to 18944 35 us, of which the weights' way from HBM is 12 and the first
 // kernel, which is not hidden, some 7. A pair of CTAs works as one MMA unit on 256 weight rows x
 // up to 256 tokens, as for 16-bit weights (gemm_pair.cuh), but its weights come as codes: teams of warps read them into
 // registers, a round of stages ahead, and write the operand tiles of a CTA's 128 rows into the 128-byte-swizzled ring, so HBM delivers half a byte a weight.

@@ -210,7 +210,12 @@ def _workspace(x, dtype, rows, address, spaces, gated):
 def linear_w4(backend: CudaBackend, x, weight: W4Weight, bias=None, out=None):
     """``x W^T + bias`` (tensor.rs:96-130) over ``x`` ``[rows, in]``, f32 or bf16; ``bias`` f32 ``[out]``. Sums are f32, rounded once to the type of
     ``x``. Rows may be apart (any stride that keeps them on 16-byte boundaries); ``out``, if given, overlaps none of
-    the others, is written and returned."""
+    the others, is written and returned.
+
+    f32 values count as multiples of 2^-133, with all of their bits from 2^-109 on. With many rows of bf16 a weight has 11 bits: all of them with a zero point
+    of 8, else off by up to 2^-12 of itself; scales below 2^-21 of their row's largest, and values below 2^-30 of their row's, lose bits. A bounded wait of
+    those kernels that gives up leaves outputs of no use and sets bit 0 of ``CudaBackend.poll_wait_timeouts()``, which a program reads when it has waited for the
+    stream: the call itself has returned by then."""
     if _torch is None:
         _load()
     held = weight._held
